@@ -8,6 +8,10 @@
  *       Jacobi-2D 5-point, Jacobi-3D 7-point)
  *   (3) ReduceToHierarchicalGPU spmd.reduce     (f32 sum, i32 sum)
  *
+ * and, built from the same maps and reductions, the memory-bound operators of
+ * a training step (layer norm and its gradients, the norm of a gradient, the
+ * AdamW step).
+ *
  * Memref descriptors follow MLIR's unpacked memref-to-LLVM convention
  * (harness/run_host.py:8-11,41-65 in the reference):
  *   rank-0 memref : (T* base, T* aligned, int64 offset)
@@ -478,6 +482,83 @@ int spmdb200_jacobi3d(float *U_base, float *U_aligned, int64_t U_offset,
                       int64_t V_stride0, int64_t V_stride1, int64_t V_stride2,
                       int64_t sweeps, int64_t res_every, double *res_out,
                       void *ws, size_t ws_bytes, void *stream);
+
+/* ---- training-step operators ------------------------------------------------ */
+/* No reference counterpart: row reductions joined to a map (layer norm), column
+ * reductions (its weight gradient), a reduction over many tensors (the gradient
+ * norm) and a map over many tensors (the AdamW step).  Element types: */
+#define SPMDB200_F32 0
+#define SPMDB200_F16 1
+#define SPMDB200_BF16 2
+
+/* y = (x - mean) rstd * weight + bias over the last dimension of a rank 1-3
+ * view: per row mean = sum(x) / N, rstd = 1 / sqrt(sum((x - mean)^2) / N + eps).
+ * sizes[rank] is x's shape (host array; the last size N >= 1, others >= 0);
+ * strides are in elements, >= 0 for x and >= 1 for y where the size is above
+ * 1.  weight and bias hold N
+ * elements of w_type, unit stride; either may be NULL (1 and 0).  mean and
+ * rstd (device f32, one per row in row order) may be NULL.  x_type and y_type
+ * are equal, or one of them is SPMDB200_F32.  Sums are f32; y is rounded once.
+ * y may be x (same view); other overlaps are undefined. */
+int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_type, const int64_t *x_strides,
+                        void *y, int y_type, const int64_t *y_strides, const void *weight, const void *bias,
+                        int w_type, float eps, float *mean, float *rstd, void *stream);
+
+/* Gradients of spmdb200_layer_norm.  dy has y's shape and type, mean and rstd
+ * are what the forward entry wrote.  With xh = (x - mean) rstd and a = dy *
+ * weight: dx = rstd (a - sum(a) / N - xh sum(a xh) / N) in x's type, dweight =
+ * sum over rows of dy xh, dbias = sum over rows of dy (N elements of dw_type,
+ * zero when there is no row).  dx, dweight and dbias may each be NULL.
+ * dx may be dy (where the types are equal) or x (same view); other overlaps
+ * are undefined.  ws: device memory of at least
+ * spmdb200_layer_norm_workspace_bytes(rows, N) bytes, 16-byte aligned, contents
+ * irrelevant; calls that share ws must not overlap on the GPU.  Every sum has
+ * a fixed order: equal inputs give equal bits. */
+size_t spmdb200_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+int spmdb200_layer_norm_backward(int rank, const int64_t *sizes, const void *dy, int dy_type,
+                                 const int64_t *dy_strides, const void *x, int x_type, const int64_t *x_strides,
+                                 const float *mean, const float *rstd, const void *weight, int w_type, void *dx,
+                                 const int64_t *dx_strides, void *dweight, void *dbias, int dw_type, void *ws,
+                                 size_t ws_bytes, void *stream);
+
+/* *norm = sqrt(sum of squares of every element of `count` tensors) and, where
+ * scale is not NULL, *scale = min(1, max_norm / *norm), NaN when the norm is
+ * not finite (device f32 scalars).  grads[k] holds sizes[k] elements of
+ * types[k], unit stride (host arrays of `count` entries; a size may be 0).
+ * Squares and sums are f64, one rounding, identical bits on every call.  ws:
+ * spmdb200_grad_norm_workspace_bytes(count) bytes of device memory, 16-byte
+ * aligned, contents irrelevant; calls that share ws must not overlap on the
+ * GPU. */
+size_t spmdb200_grad_norm_workspace_bytes(int count);
+int spmdb200_grad_norm(int count, const void *const *grads, const int64_t *sizes, const int *types, float max_norm,
+                       float *norm, float *scale, void *ws, size_t ws_bytes, void *stream);
+
+/* One AdamW step over `count` tensors in place; step counts from 1:
+ *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in f32; a parameter is rounded once to its type, and once more to that of
+ * copies[k] (SPMDB200_F16 or BF16), where copies and copies[k] are not NULL.
+ * Host arrays of `count` entries: params, param_types, grads, grad_types,
+ * sizes (elements; 0 allowed), exp_avg, exp_avg_sq, decay.  All tensors have
+ * unit stride.  state_bits 32: exp_avg and exp_avg_sq hold f32.  state_bits 8:
+ * they hold one byte per element, in blocks of SPMDB200_STATE_BLOCK
+ * consecutive elements (the last may be shorter) with one f32 scale each in
+ * exp_avg_scales / exp_avg_sq_scales: m = e4m3 code * scale and sqrt(v) = e4m3
+ * code * scale, scale = max(largest magnitude / 448, 2^-120); a root above
+ * zero keeps the smallest code at least.  A NaN or infinity makes its block's
+ * states NaN.
+ * lr_dev, step_dev: device scalars read in place of lr and step where not NULL
+ * (a step below 1 counts as 1), so that a captured launch can be replayed with
+ * new values.  grad_scale: device factor, NULL for 1; when it is NaN or
+ * infinite the call leaves everything as it was.  Tensors that are written may
+ * not overlap one another or a gradient (checked). */
+#define SPMDB200_STATE_BLOCK 256
+int spmdb200_adamw(int count, void *const *params, const int *param_types, const void *const *grads,
+                   const int *grad_types, const int64_t *sizes, void *const *exp_avg, void *const *exp_avg_sq,
+                   int state_bits, float *const *exp_avg_scales, float *const *exp_avg_sq_scales,
+                   void *const *copies, const int *copy_types, const double *decay, double lr, const float *lr_dev,
+                   double beta1, double beta2, double eps, int64_t step, const int64_t *step_dev,
+                   const float *grad_scale, void *stream);
 
 /* =========================================================================
  * C. End-to-end host entries for configurations without a reference entry.

@@ -20,6 +20,7 @@ CUBIN_PATH = PKG_DIR / "spmdb200_kernels.cubin"
 c_p = ctypes.c_void_p
 c_i = ctypes.c_int64
 c_f = ctypes.c_float
+c_d = ctypes.c_double
 c_sz = ctypes.c_size_t
 
 # Unpacked memref descriptor argtypes (harness/run_host.py:41-65 convention).
@@ -90,6 +91,17 @@ _SIGS = {
     "spmdb200_ipc_close": (ctypes.c_int, [c_p]),
     "spmdb200_fill_jacobi_input": (ctypes.c_int, [c_p, c_i, c_i, c_i, c_i, c_i, ctypes.c_uint64, c_p]),
     "spmdb200_fill_jacobi3d_input": (ctypes.c_int, [c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, ctypes.c_uint64, c_p]),
+    # training-step operators
+    "spmdb200_layer_norm": (ctypes.c_int, [ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, c_p,
+                                           ctypes.c_int, c_f, c_p, c_p, c_p]),
+    "spmdb200_layer_norm_workspace_bytes": (c_sz, [c_i, c_i]),
+    "spmdb200_layer_norm_backward": (ctypes.c_int, [ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, ctypes.c_int, c_p,
+                                                    c_p, c_p, c_p, ctypes.c_int, c_p, c_p, c_p, c_p, ctypes.c_int,
+                                                    c_p, c_sz, c_p]),
+    "spmdb200_grad_norm_workspace_bytes": (c_sz, [ctypes.c_int]),
+    "spmdb200_grad_norm": (ctypes.c_int, [ctypes.c_int, c_p, c_p, c_p, c_f, c_p, c_p, c_p, c_sz, c_p]),
+    "spmdb200_adamw": (ctypes.c_int, [ctypes.c_int, c_p, c_p, c_p, c_p, c_p, c_p, c_p, ctypes.c_int, c_p, c_p, c_p, c_p,
+                                      c_p, c_d, c_p, c_d, c_d, c_d, c_i, c_p, c_p, c_p]),
     # family C: end-to-end host entries
     "spmdb200_axpy_host": (ctypes.c_int, [c_f] + D1 + D1 + [c_i]),
     "spmdb200_sum_f32_host": (ctypes.c_int, D1 + D0 + [c_i]),

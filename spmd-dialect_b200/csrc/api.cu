@@ -7,11 +7,13 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <atomic>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "../../include/spmd_b200.h"
@@ -92,6 +94,111 @@ int have_device() {
     return fail(SPMDB200_ERR_NO_DEVICE, "no CUDA device visible (%s)", cudaGetErrorString(e));
   }
   return SPMDB200_OK;
+}
+
+// ---- arguments of the training-step operators -----------------------------------
+int type_bytes(int type) { return type == SPMDB200_F32 ? 4 : 2; }
+int check_type(const char *nm, int type) {
+  if (type != SPMDB200_F32 && type != SPMDB200_F16 && type != SPMDB200_BF16)
+    return fail(SPMDB200_ERR_INVALID_ARG, "%s: type %d must be SPMDB200_F32, F16 or BF16", nm, type);
+  return SPMDB200_OK;
+}
+// Null passes: whether a tensor may be absent is its entry's matter.
+int check_aligned(const char *nm, const void *p, int type) {
+  if ((uintptr_t)p % type_bytes(type) != 0)
+    return fail(SPMDB200_ERR_INVALID_ARG, "%s: pointer is not aligned to its elements", nm);
+  return SPMDB200_OK;
+}
+int check_listed(const char *nm, int k, const void *p, int64_t n, int type) {
+  CHECK(check_type(nm, type));
+  if (n < 0) return fail(SPMDB200_ERR_INVALID_ARG, "%s %d: negative size", nm, k);
+  if (n > 0 && !p) return fail(SPMDB200_ERR_INVALID_ARG, "%s %d: null pointer", nm, k);
+  return check_aligned(nm, p, type);
+}
+
+// Rows and columns of a rank 1-3 shape, and the type pair.
+int norm_shape(int rank, const int64_t *sizes, int x_type, int y_type, LayerNormProblem *p) {
+  if (rank < 1 || rank > 3) return fail(SPMDB200_ERR_INVALID_ARG, "rank %d: must be 1, 2 or 3", rank);
+  if (!sizes) return fail(SPMDB200_ERR_INVALID_ARG, "null sizes");
+  CHECK(check_type("x", x_type));
+  CHECK(check_type("y", y_type));
+  if (x_type != y_type && x_type != SPMDB200_F32 && y_type != SPMDB200_F32)
+    return fail(SPMDB200_ERR_UNSUPPORTED, "types of x and y: equal, or one of them f32");
+  p->rows = 1;
+  p->cols = sizes[rank - 1];
+  for (int d = 0; d < rank; ++d) {
+    if (sizes[d] < 0 || sizes[d] > (int64_t(1) << 40))
+      return fail(SPMDB200_ERR_INVALID_ARG, "size %lld in dimension %d", (long long)sizes[d], d);
+    if (d + 1 < rank && sizes[d] > 0 && p->rows > (int64_t(1) << 40) / sizes[d])
+      return fail(SPMDB200_ERR_INVALID_ARG, "more than 2^40 rows");
+    if (d + 1 < rank) p->rows *= sizes[d];
+  }
+  if (p->cols < 1) return fail(SPMDB200_ERR_INVALID_ARG, "the last dimension holds no element");
+  return SPMDB200_OK;
+}
+// A view's rows.  A view that is written may not meet itself: taken by
+// ascending stride, each stride reaches past what lies below it.
+int norm_view(const char *nm, const void *p, int type, int rank, const int64_t *sizes, const int64_t *strides,
+              bool written, Rows *r) {
+  if (!p || !strides) return fail(SPMDB200_ERR_INVALID_ARG, "%s: null pointer or strides", nm);
+  CHECK(check_aligned(nm, p, type));
+  for (int d = 0; d < rank; ++d)
+    if (strides[d] < 0) return fail(SPMDB200_ERR_INVALID_ARG, "%s: negative stride in dimension %d", nm, d);
+  if (written) {
+    int64_t span = 0;  // elements past the first that the dimensions taken so far reach
+    bool taken[3] = {false, false, false};
+    for (int k = 0; k < rank; ++k) {
+      int at = -1;
+      for (int d = 0; d < rank; ++d)
+        if (!taken[d] && (at < 0 || strides[d] < strides[at] || (strides[d] == strides[at] && sizes[d] < sizes[at]))) at = d;
+      taken[at] = true;
+      if (sizes[at] < 2) continue;
+      if (strides[at] <= span) return fail(SPMDB200_ERR_INVALID_ARG, "%s: the view overlaps itself", nm);
+      span += (sizes[at] - 1) * strides[at];
+    }
+  }
+  r->sc = strides[rank - 1];
+  r->s1 = rank >= 2 ? strides[rank - 2] : 0;
+  r->s0 = rank == 3 ? strides[0] : 0;
+  r->n1 = rank == 3 ? sizes[1] : rank == 2 ? sizes[0] : 1;
+  if (rank == 3 && (sizes[0] == 1 || r->s0 == r->n1 * r->s1)) r->n1 = sizes[0] * sizes[1];  // one row stride
+  return SPMDB200_OK;
+}
+
+// The first tensor of the list with memory that is written and that another
+// tensor of the call reads or writes; -1 if there is none.
+int overlapping(const AdamWProblem &p) {
+  struct Span {
+    uintptr_t lo, hi;
+    int k;
+    bool written;
+  };
+  std::vector<Span> spans;
+  spans.reserve((size_t)p.count * 7);
+  auto add = [&](const void *q, int64_t bytes, int k, bool written) {
+    spans.push_back({(uintptr_t)q, (uintptr_t)q + (uintptr_t)bytes, k, written});
+  };
+  for (int k = 0; k < p.count; ++k) {
+    const int64_t n = p.sizes[k], blocks = (n + kStateBlock - 1) / kStateBlock;
+    if (n == 0) continue;
+    add(p.params[k], n * type_bytes(p.param_types[k]), k, true);
+    add(p.grads[k], n * type_bytes(p.grad_types[k]), k, false);
+    add(p.m[k], p.bits8 ? n : 4 * n, k, true);
+    add(p.v[k], p.bits8 ? n : 4 * n, k, true);
+    if (p.bits8) {
+      add(p.m_scales[k], 4 * blocks, k, true);
+      add(p.v_scales[k], 4 * blocks, k, true);
+    }
+    if (p.copies && p.copies[k]) add(p.copies[k], n * type_bytes(p.copy_types[k]), k, true);
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
+  uintptr_t any = 0, written = 0;  // the furthest ends so far
+  for (const Span &s : spans) {
+    if (s.lo < (s.written ? any : written)) return s.k;
+    any = s.hi > any ? s.hi : any;
+    if (s.written) written = s.hi > written ? s.hi : written;
+  }
+  return -1;
 }
 
 // ---- staging buffers for the host entries --------------------------------------
@@ -893,6 +1000,142 @@ void hierarchical_sum(float *A_base, float *A, int64_t A_off, int64_t A_size, in
   (void)A_base; (void)o_base;
   report_void("hierarchical_sum", sum_host_impl(A, A_off, A_size, A_st, o, o_off, N));
 }
+
+// ------------------------------------------------------- training-step operators
+size_t spmdb200_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows < 0 || cols < 1 ? 0 : layer_norm_workspace_bytes(rows, cols);
+}
+
+int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_type, const int64_t *x_strides, void *y,
+                        int y_type, const int64_t *y_strides, const void *weight, const void *bias, int w_type,
+                        float eps, float *mean, float *rstd, void *stream) {
+  LayerNormProblem p{};
+  CHECK(norm_shape(rank, sizes, x_type, y_type, &p));
+  if (!(eps >= 0.0f)) return fail(SPMDB200_ERR_INVALID_ARG, "eps must be >= 0");
+  if (weight || bias) CHECK(check_type("weight", w_type));
+  if (p.rows == 0) return ok();
+  CHECK(norm_view("x", x, x_type, rank, sizes, x_strides, false, &p.xr));
+  CHECK(norm_view("y", y, y_type, rank, sizes, y_strides, true, &p.yr));
+  CHECK(check_aligned("weight", weight, w_type));
+  CHECK(check_aligned("bias", bias, w_type));
+  CHECK(check_aligned("mean", mean, SPMDB200_F32));
+  CHECK(check_aligned("rstd", rstd, SPMDB200_F32));
+  p.x = x, p.xtype = x_type, p.y = y, p.ytype = y_type;
+  p.w = weight, p.b = bias, p.wtype = w_type;
+  p.eps = eps, p.mean = mean, p.rstd = rstd;
+  CHECK(have_device());
+  CUDA_TRY(launch_layer_norm(p, (cudaStream_t)stream));
+  return ok();
+}
+
+int spmdb200_layer_norm_backward(int rank, const int64_t *sizes, const void *dy, int dy_type,
+                                 const int64_t *dy_strides, const void *x, int x_type, const int64_t *x_strides,
+                                 const float *mean, const float *rstd, const void *weight, int w_type, void *dx,
+                                 const int64_t *dx_strides, void *dweight, void *dbias, int dw_type, void *ws,
+                                 size_t ws_bytes, void *stream) {
+  LayerNormProblem p{};
+  CHECK(norm_shape(rank, sizes, x_type, dy_type, &p));
+  if (weight) CHECK(check_type("weight", w_type));
+  if (dweight || dbias) CHECK(check_type("dweight", dw_type));
+  if (!dx && !dweight && !dbias) return ok();
+  if (p.rows > 0) {
+    CHECK(norm_view("x", x, x_type, rank, sizes, x_strides, false, &p.xr));
+    CHECK(norm_view("dy", dy, dy_type, rank, sizes, dy_strides, false, &p.yr));
+    if (dx) CHECK(norm_view("dx", dx, x_type, rank, sizes, dx_strides, true, &p.dr));
+    if (!mean || !rstd) return fail(SPMDB200_ERR_INVALID_ARG, "null mean or rstd");
+    CHECK(check_aligned("mean", mean, SPMDB200_F32));
+    CHECK(check_aligned("rstd", rstd, SPMDB200_F32));
+  } else if (!dweight && !dbias) {
+    return ok();
+  }
+  CHECK(check_aligned("weight", weight, w_type));
+  CHECK(check_aligned("dweight", dweight, dw_type));
+  CHECK(check_aligned("dbias", dbias, dw_type));
+  if (!ws || ((uintptr_t)ws & 15u) != 0 || ws_bytes < layer_norm_workspace_bytes(p.rows, p.cols))
+    return fail(SPMDB200_ERR_WORKSPACE, "workspace must be >= %zu bytes and 16-byte aligned",
+                layer_norm_workspace_bytes(p.rows, p.cols));
+  p.x = x, p.xtype = x_type, p.y = const_cast<void *>(dy), p.ytype = dy_type;
+  p.w = weight, p.wtype = w_type;
+  p.mean = const_cast<float *>(mean), p.rstd = const_cast<float *>(rstd);
+  p.dx = dx, p.dw = dweight, p.db = dbias, p.dwtype = dw_type, p.ws = ws;
+  CHECK(have_device());
+  CUDA_TRY(launch_layer_norm_backward(p, (cudaStream_t)stream));
+  return ok();
+}
+
+size_t spmdb200_grad_norm_workspace_bytes(int count) { return grad_norm_workspace_bytes(count); }
+
+int spmdb200_grad_norm(int count, const void *const *grads, const int64_t *sizes, const int *types, float max_norm,
+                       float *norm, float *scale, void *ws, size_t ws_bytes, void *stream) {
+  if (count < 0 || (count > 0 && (!grads || !sizes || !types)))
+    return fail(SPMDB200_ERR_INVALID_ARG, "negative count or null list");
+  if (!norm) return fail(SPMDB200_ERR_INVALID_ARG, "null norm");
+  CHECK(check_aligned("norm", norm, SPMDB200_F32));
+  CHECK(check_aligned("scale", scale, SPMDB200_F32));
+  if (scale && !(max_norm >= 0.0f)) return fail(SPMDB200_ERR_INVALID_ARG, "max_norm must be >= 0");
+  for (int k = 0; k < count; ++k) CHECK(check_listed("gradient", k, grads[k], sizes[k], types[k]));
+  if (!ws || ((uintptr_t)ws & 15u) != 0 || ws_bytes < grad_norm_workspace_bytes(count))
+    return fail(SPMDB200_ERR_WORKSPACE, "workspace must be >= %zu bytes and 16-byte aligned",
+                grad_norm_workspace_bytes(count));
+  CHECK(have_device());
+  const GradNormProblem p{count, grads, types, sizes, max_norm, norm, scale, static_cast<double *>(ws)};
+  CUDA_TRY(launch_grad_norm(p, (cudaStream_t)stream));
+  return ok();
+}
+
+int spmdb200_adamw(int count, void *const *params, const int *param_types, const void *const *grads,
+                   const int *grad_types, const int64_t *sizes, void *const *exp_avg, void *const *exp_avg_sq,
+                   int state_bits, float *const *exp_avg_scales, float *const *exp_avg_sq_scales,
+                   void *const *copies, const int *copy_types, const double *decay, double lr, const float *lr_dev,
+                   double beta1, double beta2, double eps, int64_t step, const int64_t *step_dev,
+                   const float *grad_scale, void *stream) {
+  const bool bits8 = state_bits == 8;
+  if (state_bits != 8 && state_bits != 32) return fail(SPMDB200_ERR_INVALID_ARG, "state_bits must be 8 or 32");
+  if (count < 0 || (count > 0 && (!params || !param_types || !grads || !grad_types || !sizes || !exp_avg ||
+                                  !exp_avg_sq || !decay || (copies && !copy_types) ||
+                                  (bits8 && (!exp_avg_scales || !exp_avg_sq_scales)))))
+    return fail(SPMDB200_ERR_INVALID_ARG, "negative count or null list");
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
+    return fail(SPMDB200_ERR_INVALID_ARG, "beta1 and beta2 must lie in [0, 1)");
+  if (!(eps >= 0.0)) return fail(SPMDB200_ERR_INVALID_ARG, "eps must be >= 0");
+  if (!lr_dev && !(lr >= 0.0)) return fail(SPMDB200_ERR_INVALID_ARG, "lr must be >= 0");
+  if (!step_dev && step < 1) return fail(SPMDB200_ERR_INVALID_ARG, "step counts from 1");
+  CHECK(check_aligned("lr_dev", lr_dev, SPMDB200_F32));
+  CHECK(check_aligned("grad_scale", grad_scale, SPMDB200_F32));
+  if (((uintptr_t)step_dev & 7u) != 0) return fail(SPMDB200_ERR_INVALID_ARG, "step_dev is not 8-byte aligned");
+  bool any = false;
+  for (int k = 0; k < count; ++k) {
+    CHECK(check_listed("parameter", k, params[k], sizes[k], param_types[k]));
+    CHECK(check_listed("gradient", k, grads[k], sizes[k], grad_types[k]));
+    if (!(decay[k] >= 0.0)) return fail(SPMDB200_ERR_INVALID_ARG, "decay of tensor %d must be >= 0", k);
+    if (sizes[k] == 0) continue;
+    any = true;
+    if (!exp_avg[k] || !exp_avg_sq[k] || (bits8 && (!exp_avg_scales[k] || !exp_avg_sq_scales[k])))
+      return fail(SPMDB200_ERR_INVALID_ARG, "null state of tensor %d", k);
+    const uintptr_t at = bits8 ? (uintptr_t)exp_avg_scales[k] | (uintptr_t)exp_avg_sq_scales[k]
+                               : (uintptr_t)exp_avg[k] | (uintptr_t)exp_avg_sq[k];
+    if (at & 3u) return fail(SPMDB200_ERR_INVALID_ARG, "state of tensor %d is not aligned to its elements", k);
+    if (copies && copies[k]) {
+      if (copy_types[k] != SPMDB200_F16 && copy_types[k] != SPMDB200_BF16)
+        return fail(SPMDB200_ERR_INVALID_ARG, "copy of tensor %d: type must be SPMDB200_F16 or SPMDB200_BF16", k);
+      CHECK(check_aligned("copy", copies[k], copy_types[k]));
+    }
+  }
+  if (!any) return ok();
+  const AdamWProblem p{count,      params,      grads, exp_avg, exp_avg_sq, exp_avg_scales, exp_avg_sq_scales, copies,
+                       sizes,      param_types, grad_types, copy_types, decay, bits8, lr, beta1, beta2, eps, step,
+                       lr_dev,     step_dev,    grad_scale};
+  try {
+    const int k = overlapping(p);
+    if (k >= 0) return fail(SPMDB200_ERR_INVALID_ARG, "a tensor that tensor %d writes overlaps another tensor", k);
+  } catch (const std::bad_alloc &) {
+    return fail(SPMDB200_ERR_INVALID_ARG, "no host memory to check %d tensors", count);
+  }
+  CHECK(have_device());
+  CUDA_TRY(launch_adamw(p, (cudaStream_t)stream));
+  return ok();
+}
+
 
 // ---------------------------------------------------------------- host entries (C)
 int spmdb200_axpy_host(float a, float *X_base, float *X, int64_t X_off, int64_t X_size, int64_t X_st,

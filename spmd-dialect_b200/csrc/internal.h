@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "dtypes.cuh"
 
 namespace spmdb200 {
 
@@ -168,6 +169,65 @@ struct StencilNdProblem {
   float scale;             // 1: no final multiply
 };
 cudaError_t launch_stencil_nd(const StencilNdProblem &p, int promote, cudaStream_t s);
+
+// ---- layer norm (layer_norm.cu) -----------------------------------------------------
+// One struct for both directions: y is the output going forward and dy going
+// back; mean and rstd are written going forward (where not null) and read
+// going back.  rows, cols as checked by the entry (cols >= 1).
+struct LayerNormProblem {
+  int64_t rows, cols;
+  const void *x;
+  int xtype;
+  Rows xr;
+  void *y;
+  int ytype;
+  Rows yr;
+  const void *w, *b;  // cols elements of wtype, or null
+  int wtype;
+  float eps;
+  float *mean, *rstd;  // one per row, dense
+  void *dx;            // xtype, or null
+  Rows dr;
+  void *dw, *db;  // cols elements of dwtype, or null
+  int dwtype;
+  void *ws;  // layer_norm_workspace_bytes(rows, cols), contents irrelevant
+};
+size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+cudaError_t launch_layer_norm(const LayerNormProblem &p, cudaStream_t s);
+cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s);
+
+// ---- many tensors at once (grad_norm.cu, adamw.cu) ----------------------------------
+struct GradNormProblem {
+  int count;
+  const void *const *grads;
+  const int *types;
+  const int64_t *sizes;
+  float max_norm;
+  float *norm, *scale;  // scale may be null
+  double *ws;           // grad_norm_workspace_bytes(count), contents irrelevant
+};
+size_t grad_norm_workspace_bytes(int count);
+cudaError_t launch_grad_norm(const GradNormProblem &p, cudaStream_t s);
+
+constexpr int kStateBlock = 256;  // elements that share one scale of an 8-bit state
+struct AdamWProblem {
+  int count;
+  void *const *params;
+  const void *const *grads;
+  void *const *m, *const *v;                // f32, or e4m3 codes when bits8
+  float *const *m_scales, *const *v_scales;  // bits8: one per kStateBlock elements
+  void *const *copies;                      // null, or per tensor null or a low-precision copy
+  const int64_t *sizes;
+  const int *param_types, *grad_types, *copy_types;
+  const double *decay;  // per tensor
+  bool bits8;
+  double lr, beta1, beta2, eps;
+  int64_t step;
+  const float *lr_dev;        // in place of lr where not null
+  const int64_t *step_dev;    // in place of step where not null
+  const float *grad_scale;    // device factor of every gradient, or null
+};
+cudaError_t launch_adamw(const AdamWProblem &p, cudaStream_t s);
 
 // ---- driver entry points resolved at run time (no link-time libcuda) ----------------
 // Encodes a row-major f32 tensor map (innermost dimension first).  Returns 0 on success.

@@ -1,0 +1,335 @@
+"""Layer norm and its gradients against 64-bit formulas, with bounds counted in
+roundings (train_ref.py)."""
+from __future__ import annotations
+
+import pytest
+
+from conftest import spmd_mod
+
+torch = pytest.importorskip("torch")
+from train_ref import U, assert_within, norm_back_ref, norm_ref, rounded  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+PAIRS = [(F32, F32), (F16, F16), (BF16, BF16), (F32, F16), (F32, BF16), (F16, F32), (BF16, F32)]
+COLS = [1, 2, 3, 7, 8, 31, 64, 100, 128, 257, 512, 1000, 1001, 1024, 2040, 4096, 5003, 8192, 8200, 12288, 16385, 20000,
+        32768, 40001, 70000, 131072, 300001]
+EPS = 1e-5
+
+
+def make(shape, dtype, seed, shift=0.5):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = torch.randn(shape, generator=g, device="cuda")
+    if len(shape) > 1 and shift:
+        t = t + shift * torch.randn((*shape[:-1], 1), generator=g, device="cuda")
+    return t.to(dtype)
+
+
+def weights(cols, dtype, seed):
+    if dtype is None:
+        return None, None
+    return (1 + 0.2 * make((cols,), F32, seed)).to(dtype), (0.2 * make((cols,), F32, seed + 1)).to(dtype)
+
+
+def check_forward(k, x, w, b, eps=EPS, ydtype=None, **kw):
+    y, mean, rstd = k.layer_norm(x, w, b, eps=eps, dtype=ydtype, **kw)
+    want, m, r, e_m, e_r, e_y = norm_ref(x, w, b, eps)
+    assert y.dtype == (ydtype or x.dtype) and y.shape == x.shape
+    assert_within(mean, m, e_m, "mean")
+    assert_within(rstd, r, e_r, "rstd")
+    assert_within(y, want, e_y + rounded(want.abs() + e_y, y.dtype), "y")
+    return y, mean, rstd
+
+
+def check_backward(k, dy, x, w, eps=EPS, stats=None, **kw):
+    n = x.shape[-1]
+    if stats is None:
+        xd = x.double()
+        stats = xd.mean(-1).float(), (1 / (xd.var(-1, unbiased=False) + eps).sqrt()).float()
+    want = norm_back_ref(dy, x, *stats, w)  # before dx may overwrite an input
+    kind = x.dtype
+    dx, dw, db = k.layer_norm_backward(dy, x, *stats, w, **kw)
+    assert dx.dtype == kind and dx.shape == dy.shape
+    assert_within(dx, want[0], want[3] + rounded(want[0].abs() + want[3], kind), "dx")
+    if dw is not None:
+        assert dw.shape == db.shape == (n,)
+        assert_within(dw, want[1], want[4] + rounded(want[1].abs() + want[4], dw.dtype), "dweight")
+        assert_within(db, want[2], want[5] + rounded(want[2].abs() + want[5], db.dtype), "dbias")
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("cols", COLS)
+def test_row_lengths(kernels, cols):
+    """Every row length class with f32 and 16-bit rows, odd row counts."""
+    rows = 5 if cols > 20000 else 37
+    for x_t, y_t, w_t in ((F32, F32, F32), (BF16, BF16, F32), (F16, F16, F16), (F32, BF16, F32), (BF16, F32, None)):
+        x, dy = make((rows, cols), x_t, cols), make((rows, cols), y_t, cols + 1)
+        w, b = weights(cols, w_t, cols + 2)
+        _, mean, rstd = check_forward(kernels, x, w, b, ydtype=y_t)
+        check_backward(kernels, dy, x, w, stats=(mean, rstd))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 148, 149, 1000, 4099])
+@pytest.mark.parametrize("cols", [24, 1001, 4096])
+def test_row_counts(kernels, rows, cols):
+    x, dy = make((rows, cols), BF16, rows), make((rows, cols), BF16, rows + 1)
+    w, b = weights(cols, BF16, rows + 2)
+    _, mean, rstd = check_forward(kernels, x, w, b)
+    check_backward(kernels, dy, x, w, stats=(mean, rstd))
+
+
+@pytest.mark.parametrize("x_t,y_t", PAIRS)
+@pytest.mark.parametrize("w_t", [None, F32, F16, BF16])
+def test_types(kernels, x_t, y_t, w_t):
+    for rows, cols in ((33, 320), (9, 1026)):
+        x, dy = make((rows, cols), x_t, 1), make((rows, cols), y_t, 2)
+        w, b = weights(cols, w_t, 3)
+        check_forward(kernels, x, w, b, ydtype=y_t)
+        _, dw, _ = check_backward(kernels, dy, x, w)
+        assert (dw is None) == (w is None) and (w is None or dw.dtype == w_t)
+
+
+def layouts(t_wide):
+    """Views of one buffer [12, 30, 700]: (name, view)."""
+    return [
+        ("pitched", t_wide[:, 0, :640]),
+        ("shifted by one element", t_wide[:, 3, 1:601]),
+        ("rank 3 slice", t_wide[:, 2:9, :512]),
+        ("rank 3, odd", t_wide[1:, 5:, 3:404]),
+        ("every second column", t_wide[:, :4, ::2]),
+        ("columns as rows", t_wide[:, 0, :].t()),
+        ("swapped leading dimensions", t_wide[:, :, :96].transpose(0, 1)),
+        ("one row", t_wide[0, 0]),
+        ("rank 4", t_wide.view(3, 4, 30, 700)),
+    ]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("at", range(9))
+def test_layouts(kernels, dtype, at):
+    name, x = layouts(make((12, 30, 700), dtype, 5))[at]
+    _, dy = layouts(make((12, 30, 700), dtype, 6))[at]
+    w, b = weights(x.shape[-1], F32, 7)
+    check_forward(kernels, x, w, b)
+    check_backward(kernels, dy, x, w)
+    # Into views of the same layout: what lies between the rows stays as it was.
+    buf = torch.full((12, 30, 700), 7.0, device="cuda", dtype=dtype)
+    out = layouts(buf)[at][1]
+    want = kernels.layer_norm(x, w, b)[0]
+    kernels.layer_norm(x, w, b, out=out)
+    assert torch.equal(out, want), name
+    mask = torch.zeros(12, 30, 700, device="cuda", dtype=torch.bool)
+    layouts(mask)[at][1].fill_(True)
+    assert bool((buf[~mask] == 7.0).all()), name
+    buf.fill_(7.0)
+    xd = x.double()
+    stats = xd.mean(-1).float(), (1 / (xd.var(-1, unbiased=False) + EPS).sqrt()).float()
+    want = kernels.layer_norm_backward(dy, x, *stats, w)[0]
+    kernels.layer_norm_backward(dy, x, *stats, w, dx=out)
+    assert torch.equal(out, want) and bool((buf[~mask] == 7.0).all()), name
+
+
+@pytest.mark.parametrize("cols", [64, 1001, 4096, 20000, 100000])
+def test_broadcast_inputs(kernels, cols):
+    """Inputs of stride 0: one row for all, one value for a whole row."""
+    x, dy = make((1, cols), F32, 1).expand(6, cols), make((6, cols), F32, 2)
+    w, b = weights(cols, F32, 3)
+    check_forward(kernels, x, w, b)
+    check_backward(kernels, dy, x, w)
+    check_backward(kernels, make((6, 1), F32, 4).expand(6, cols), make((6, cols), F32, 5), w)
+    check_backward(kernels, torch.ones((), device="cuda").expand(6, cols), make((6, cols), F32, 5), w)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("cols", [40, 1001, 4096, 9000, 20000, 100000])
+def test_in_place(kernels, dtype, cols):
+    x, dy = make((11, cols), dtype, 1), make((11, cols), dtype, 2)
+    w, b = weights(cols, F32, 3)
+    want, mean, rstd = kernels.layer_norm(x, w, b)
+    dx, dw, db = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+    for target in ("dy", "x"):
+        a, c = dy.clone(), x.clone()
+        got = kernels.layer_norm_backward(a, c, mean, rstd, w, dx=a if target == "dy" else c)
+        assert all(torch.equal(p, q) for p, q in zip(got, (dx, dw, db))), target
+    y = x.clone()
+    assert torch.equal(kernels.layer_norm(y, w, b, out=y)[0], want)
+
+
+def test_partial_arguments(kernels):
+    x, dy = make((40, 300), F32, 1), make((40, 300), F32, 2)
+    w, b = weights(300, F32, 3)
+    full, mean, rstd = kernels.layer_norm(x, w, b)
+    y, none1, none2 = kernels.layer_norm(x, w, b, stats=False)
+    assert torch.equal(y, full) and none1 is None and none2 is None
+    check_forward(kernels, x, w, None)
+    check_forward(kernels, x, None, b)
+    check_forward(kernels, x, None, None, eps=0.0)
+    dx, dw, db = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+    only, n1, n2 = kernels.layer_norm_backward(dy, x, mean, rstd, w, wgrad=False)
+    assert torch.equal(only, dx) and n1 is None and n2 is None
+    # Sums without a weight, and sums in a type of their own.
+    _, dw1, db1 = check_backward(kernels, dy, x, None, stats=(mean, rstd), wgrad=True)
+    assert torch.equal(dw1, dw) and torch.equal(db1, db)
+    kind = torch.empty(300, device="cuda", dtype=BF16)
+    _, dw2, db2 = check_backward(kernels, dy, x, w, stats=(mean, rstd), dweight=kind)
+    assert dw2 is kind and db2.dtype == BF16 and torch.equal(dw2, dw.bfloat16())
+
+
+def test_no_rows(kernels):
+    x = torch.empty((0, 100), device="cuda")
+    w, b = weights(100, F32, 1)
+    y, mean, rstd = kernels.layer_norm(x, w, b)
+    assert y.shape == (0, 100) and mean.shape == rstd.shape == (0,)
+    dx, dw, db = kernels.layer_norm_backward(x, x, mean, rstd, w)
+    assert dx.shape == (0, 100) and bool((dw == 0).all()) and bool((db == 0).all())
+    y, _, _ = kernels.layer_norm(torch.empty((3, 0, 100), device="cuda"), w, b)
+    assert y.shape == (3, 0, 100)
+
+
+@pytest.mark.parametrize("cols", [8, 1001, 4096, 40000])
+def test_far_means_and_constant_rows(kernels, cols):
+    """Rows whose mean is far above their spread, constant rows, rows of zeros and rows of large values."""
+    x = make((8, cols), F32, 1)
+    x[0] += 1000.0
+    x[1] = 3.25
+    x[2] = 0.0
+    x[3] *= 1e15
+    x[4] *= 1e-15
+    w, b = weights(cols, F32, 3)
+    _, mean, rstd = check_forward(kernels, x, w, b)
+    assert bool((rstd[2] - EPS ** -0.5).abs() <= 4 * U * EPS ** -0.5)
+    check_backward(kernels, make((8, cols), F32, 2), x, w, stats=(mean, rstd))
+
+
+@pytest.mark.parametrize("cols", [16, 1001, 4096, 20000])
+def test_a_bad_row_stays_alone(kernels, cols):
+    """NaN and infinity spoil their own row, and the sums over rows; other rows keep their bits."""
+    x, dy = make((9, cols), F32, 1), make((9, cols), F32, 2)
+    w, b = weights(cols, F32, 3)
+    y, mean, rstd = kernels.layer_norm(x, w, b)
+    dx, dw, db = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+    bad = x.clone()
+    bad[4, cols // 2] = float("nan")
+    bad[6, 0] = float("inf")
+    y1, mean1, rstd1 = kernels.layer_norm(bad, w, b)
+    dx1, dw1, db1 = kernels.layer_norm_backward(dy, bad, mean1, rstd1, w)
+    good = [0, 1, 2, 3, 5, 7, 8]
+    for a, c in ((y, y1), (mean, mean1), (rstd, rstd1), (dx, dx1)):
+        assert torch.equal(a[good], c[good])
+    assert bool(y1[4].isnan().all()) and bool(y1[6].isnan().all()) and bool(dx1[4].isnan().all())
+    assert bool(dw1.isnan().all()) and torch.equal(db1, db)
+
+
+def test_same_bits_every_time(kernels):
+    for rows, cols in ((5000, 64), (700, 1001), (300, 4096), (40, 30000)):
+        x, dy = make((rows, cols), BF16, 1), make((rows, cols), BF16, 2)
+        w, b = weights(cols, F32, 3)
+        _, mean, rstd = kernels.layer_norm(x, w, b)
+        first = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(kernels.layer_norm_backward(dy, x, mean, rstd, w), first))
+
+
+@pytest.mark.parametrize("cols", [48, 1001])
+def test_differences(kernels, cols):
+    """dx, dweight and dbias against central differences of the forward kernel
+    along random directions: they differ by the roundings of both sides and by
+    what the difference itself is off, which 64 bits give."""
+    rows, h = 6, 1 / 64
+    x, w, b, c = make((rows, cols), F32, 1), *weights(cols, F32, 2), make((rows, cols), F32, 4)
+    _, mean, rstd = kernels.layer_norm(x, w, b)
+    grads = kernels.layer_norm_backward(c, x, mean, rstd, w)
+    ref = norm_back_ref(c, x, mean, rstd, w)
+    true = norm_back_ref(c, x, *norm_ref(x, w, b, EPS)[1:3], w)
+    for k, t in enumerate((x, w, b)):
+        d = make(tuple(t.shape), F32, 10 + k)
+        sides, exact, off = [], [], 0.0
+        for sign in (1, -1):
+            a = [x, w, b]
+            a[k] = t + sign * h * d
+            y = kernels.layer_norm(*a)[0]
+            want, *_, e_y = norm_ref(*a, EPS)
+            sides.append((y.double() * c).sum())
+            exact.append((want * c).sum())
+            off += float(((e_y + rounded(want.abs() + e_y, F32)) * c.abs()).sum()) / (2 * h)
+        moved = (a[k].double() - t) / (-h)  # the step that was taken, rounding included
+        got = (sides[0] - sides[1]) / (2 * h)
+        along = (true[k] * d).sum()
+        off += float((((exact[0] - exact[1]) / (2 * h)) - along).abs())
+        off += float(((ref[k] - true[k]).abs() * d.abs()).sum() + ((ref[3 + k] + rounded(ref[k].abs() + ref[3 + k], F32)) * d.abs()).sum())
+        assert abs(float((grads[k].double() * d).sum() - got)) <= off, k
+        assert moved.shape == d.shape
+
+
+def test_offsets_past_32_bits(kernels):
+    """Rows 2^31 + 8 elements apart."""
+    pitch, cols = (1 << 31) + 8, 1000
+    buf = torch.empty(2 * pitch + cols, device="cuda", dtype=F16)
+    x = buf.as_strided((3, cols), (pitch, 1))
+    x.copy_(make((3, cols), F16, 1))
+    w, b = weights(cols, F32, 2)
+    y = kernels.layer_norm(x, w, b, out=x)[0]
+    want = kernels.layer_norm(make((3, cols), F16, 1), w, b)[0]
+    assert torch.equal(y, want)
+    dy = make((3, cols), F16, 3)
+    x.copy_(make((3, cols), F16, 1))
+    got = check_backward(kernels, dy, x, w)
+    assert got[0].shape == (3, cols)
+
+
+def test_other_stream_and_capture(kernels):
+    """A side stream, and a captured pair of calls replayed on new inputs."""
+    x, dy = make((257, 768), BF16, 1), make((257, 768), BF16, 2)
+    w, b = weights(768, F32, 3)
+    want = kernels.layer_norm(x, w, b)
+    grads = kernels.layer_norm_backward(dy, x, *want[1:], w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = kernels.layer_norm(x, w, b, stream=side)
+    back = kernels.layer_norm_backward(dy, x, *got[1:], w, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip((*want, *grads), (*got, *back)))
+    sx, sdy = torch.zeros_like(x), torch.zeros_like(dy)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = kernels.layer_norm(sx, w, b)
+        g = kernels.layer_norm_backward(sdy, sx, *a[1:], w)
+    for seed in (1, 7):
+        sx.copy_(make((257, 768), BF16, seed))
+        sdy.copy_(make((257, 768), BF16, seed + 1))
+        graph.replay()
+        e = kernels.layer_norm(sx, w, b)
+        eg = kernels.layer_norm_backward(sdy, sx, *e[1:], w)
+        assert all(torch.equal(p, q) for p, q in zip((*a, *g), (*e, *eg)))
+
+
+def test_refusals(kernels):
+    err = spmd_mod("_lib").SpmdError
+    x, w = make((4, 32), F32, 1), make((32,), F32, 2)
+    _, mean, rstd = kernels.layer_norm(x)
+    for call, kind in (
+        (lambda: kernels.layer_norm(x.double()), TypeError),
+        (lambda: kernels.layer_norm(x.half(), dtype=BF16), TypeError),
+        (lambda: kernels.layer_norm(x.cpu()), ValueError),
+        (lambda: kernels.layer_norm(x, w.cpu()), ValueError),
+        (lambda: kernels.layer_norm(x, w[:16]), ValueError),
+        (lambda: kernels.layer_norm(x, make((64,), F32, 2)[::2]), ValueError),
+        (lambda: kernels.layer_norm(x, w, w.half()), TypeError),
+        (lambda: kernels.layer_norm(x, out=make((4, 16), F32, 1)), ValueError),
+        (lambda: kernels.layer_norm(x, dtype=F16, out=torch.empty_like(x)), TypeError),
+        (lambda: kernels.layer_norm(x, out=x[:1].expand(4, 32)), err),
+        (lambda: kernels.layer_norm(x, eps=-1.0), err),
+        (lambda: kernels.layer_norm(x, eps=float("nan")), err),
+        (lambda: kernels.layer_norm(torch.empty((4, 0), device="cuda")), err),
+        (lambda: kernels.layer_norm(torch.ones((), device="cuda")), ValueError),
+        (lambda: kernels.layer_norm(make((2, 3, 4, 8), F32, 1).transpose(0, 2)), ValueError),
+        (lambda: kernels.layer_norm_backward(x[:2], x, mean, rstd), ValueError),
+        (lambda: kernels.layer_norm_backward(x, x, mean[:2], rstd), ValueError),
+        (lambda: kernels.layer_norm_backward(x, x, mean.half(), rstd), TypeError),
+        (lambda: kernels.layer_norm_backward(x, x, mean, rstd, dx=x.half()), TypeError),
+        (lambda: kernels.layer_norm_backward(x, x, mean, rstd, w, ws=torch.empty(16, device="cuda")), err),
+        (lambda: kernels.layer_norm_backward(x, x, mean, rstd, w, wgrad=False, dbias=w), ValueError),
+    ):
+        with pytest.raises(kind):
+            call()
