@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPiece = 2048;  // elements a block takes at a time: 8 warps of one 8-bit state block each
+constexpr int kQuads = kPiece / kThreads / 4;
 constexpr float kTopCode = 448.0f, kLeastCode = 0x1p-9f, kLeastScale = 0x1p-120f;
 
 struct AdamHyper {
@@ -49,6 +50,7 @@ struct AdamTable {
   int64_t n[CAP];
   float decay[CAP];
   uint8_t copy_type[CAP];
+  uint8_t aligned[CAP];  // every address is a multiple of 4 elements (32-bit states) or 8 (8-bit)
   int count;
 };
 constexpr int kSmallCap = 32, kLargeCap = 384;
@@ -81,29 +83,76 @@ __device__ __forceinline__ float updated(float p, float m, float v, const AdamHy
   return fmaf(-c.step_size, m / fmaf(sqrtf(v), c.root_scale, h.eps), p * keep);
 }
 
+// One tensor's addresses and constants.
+template <class P, class G, class S>
+struct Tensor {
+  P *p;
+  const G *g;
+  S *m, *v;
+  void *copy;
+  int copy_type;
+  int64_t n;
+  float keep;  // 1 - lr decay
+  bool aligned;
+};
+template <class P, class G, class S, int CAP>
+__device__ __forceinline__ Tensor<P, G, S> tensor_at(const AdamTable<CAP> &t, int k, float lr) {
+  return {static_cast<P *>(t.p[k]), static_cast<const G *>(t.g[k]), static_cast<S *>(t.m[k]), static_cast<S *>(t.v[k]),
+          t.copy[k], t.copy_type[k], t.n[k], fmaf(-lr, t.decay[k], 1.0f), t.aligned[k] != 0};
+}
+
+// Every element is read and written once, so the step is bound by memory: 28
+// bytes per element with f32 parameters and states, 16-bit gradients and
+// copies.  A thread takes quads of four elements (16-byte loads of f32, all of
+// a piece's loads before the first use).
 template <class P, class G, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_32(const __grid_constant__ AdamTable<CAP> t) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_32(const __grid_constant__ AdamTable<CAP> t) {
   __shared__ Now sh;
   const AdamHyper &h = t.h;
   const Now c = constants(h, &sh);
   if (!isfinite(c.grad_scale)) return;
-  for (int64_t piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
-    const int k = tensor_of(t.first, t.count, piece);
+  const int64_t pieces = t.first[t.count];
+  int k = tensor_of(t.first, t.count, blockIdx.x);
+  for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+    while (piece >= t.first[k + 1]) ++k;
+    const Tensor<P, G, float> w = tensor_at<P, G, float>(t, k, c.lr);
     const int64_t lo = (piece - t.first[k]) * kPiece;
-    const int64_t hi = t.n[k] - lo < kPiece ? t.n[k] : lo + kPiece;
-    P *p = static_cast<P *>(t.p[k]);
-    const G *g = static_cast<const G *>(t.g[k]);
-    float *m = static_cast<float *>(t.m[k]), *v = static_cast<float *>(t.v[k]);
-    const float keep = fmaf(-c.lr, t.decay[k], 1.0f);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-      const float gi = to_f32(g[i]) * c.grad_scale;
-      const float mi = fmaf(h.beta1, m[i], h.rest1 * gi);
-      const float vi = fmaf(h.beta2, v[i], h.rest2 * gi * gi);
-      const float pi = updated(to_f32(p[i]), mi, vi, h, c, keep);
-      m[i] = mi;
-      v[i] = vi;
-      p[i] = from_f32<P>(pi);
-      if (t.copy[k]) store_from_f32(t.copy[k], t.copy_type[k], i, pi);
+    auto one = [&](float &p, float g, float &m, float &v) {
+      g *= c.grad_scale;
+      m = fmaf(h.beta1, m, h.rest1 * g);
+      v = fmaf(h.beta2, v, h.rest2 * g * g);
+      p = updated(p, m, v, h, c, w.keep);
+    };
+    if (w.aligned && lo + kPiece <= w.n) {
+      float p[kQuads][4], g[kQuads][4], m[kQuads][4], v[kQuads][4];
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const int64_t i = lo + 4 * (q * kThreads + (int)threadIdx.x);
+        load4(w.g + i, g[q]);
+        load4(w.m + i, m[q]);
+        load4(w.v + i, v[q]);
+        load4(w.p + i, p[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const int64_t i = lo + 4 * (q * kThreads + (int)threadIdx.x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) one(p[q][e], g[q][e], m[q][e], v[q][e]);
+        store4(w.m + i, m[q]);
+        store4(w.v + i, v[q]);
+        store4(w.p + i, p[q]);
+        if (w.copy) store_vec16<4>(w.copy, w.copy_type, i, p[q]);
+      }
+    } else {  // a tensor's last piece, and tensors at odd addresses
+      const int64_t hi = w.n - lo < kPiece ? w.n : lo + kPiece;
+      for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
+        float p = to_f32(w.p[i]), m = w.m[i], v = w.v[i];
+        one(p, to_f32(w.g[i]), m, v);
+        w.m[i] = m;
+        w.v[i] = v;
+        w.p[i] = from_f32<P>(p);
+        if (w.copy) store_from_f32(w.copy, w.copy_type, i, p);
+      }
     }
   }
 }
@@ -115,61 +164,103 @@ __device__ __forceinline__ float from_code(uint8_t c) {
 }
 __device__ __forceinline__ uint8_t to_code(float v) { return __nv_fp8_e4m3(v).__x; }
 
-// The largest of 32 lanes' non-negative values; NaN above all (its bits are).
-__device__ __forceinline__ float warp_top(float v) {
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+__device__ __forceinline__ float fmaxf_nan(float a, float b) { return a < b ? b : a; }  // a NaN `a` stays
+
+__device__ __forceinline__ void decode8(uint2 q, float v[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const unsigned two = ((k & 2) ? q.y : q.x) >> (16 * (k & 1));
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    v[2 * k] = f.x, v[2 * k + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint2 encode8(const float v[8]) {
+  unsigned w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * k], v[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
+// A warp takes a state block of 256 elements, eight consecutive ones a lane:
+// the block's largest magnitudes are one integer maximum over the warp each
+// (bits of non-negative floats order as the floats do, NaN above all).
 template <class P, class G, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_8(const __grid_constant__ AdamTable<CAP> t) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_8(const __grid_constant__ AdamTable<CAP> t) {
   __shared__ Now sh;
   const AdamHyper &h = t.h;
   const Now c = constants(h, &sh);
   if (!isfinite(c.grad_scale)) return;
   const int lane = threadIdx.x & 31;
-  for (int64_t piece = blockIdx.x; piece < t.first[t.count]; piece += gridDim.x) {
-    const int k = tensor_of(t.first, t.count, piece);
+  const int64_t pieces = t.first[t.count];
+  int k = tensor_of(t.first, t.count, blockIdx.x);
+  for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+    while (piece >= t.first[k + 1]) ++k;
+    const Tensor<P, G, uint8_t> w = tensor_at<P, G, uint8_t>(t, k, c.lr);
     const int64_t lo = (piece - t.first[k]) * kPiece + (threadIdx.x >> 5) * kStateBlock;
-    if (lo >= t.n[k]) continue;
+    if (lo >= w.n) continue;
     const int64_t b = lo / kStateBlock;
-    P *p = static_cast<P *>(t.p[k]);
-    const G *g = static_cast<const G *>(t.g[k]);
-    uint8_t *m = static_cast<uint8_t *>(t.m[k]), *v = static_cast<uint8_t *>(t.v[k]);
-    const float keep = fmaf(-c.lr, t.decay[k], 1.0f);
+    const int64_t i0 = lo + 8 * lane;
+    const bool whole = w.aligned && lo + kStateBlock <= w.n;  // the same for the whole warp
+    const int mine = (int)(w.n - i0 < 8 ? (w.n > i0 ? w.n - i0 : 0) : 8);
+    float p[8], g[8], m[8], r[8];
+    if (whole) {
+      load8(w.g + i0, g);
+      decode8(ld_u2(w.m + i0), m);
+      decode8(ld_u2(w.v + i0), r);
+      load8(w.p + i0, p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = e < mine;
+        p[e] = in ? to_f32(w.p[i0 + e]) : 0.0f;
+        g[e] = in ? to_f32(w.g[i0 + e]) : 0.0f;
+        m[e] = in ? from_code(w.m[i0 + e]) : 0.0f;
+        r[e] = in ? from_code(w.v[i0 + e]) : 0.0f;
+      }
+    }
+    // The scales go into the factors once per block (not their square, which
+    // would leave f32's range long before the root does).
     const float ms = t.ms[k][b], vs = t.vs[k][b];
-    float mi[8], ri[8], mtop = 0.0f, rtop = 0.0f;
+    const float keep1 = h.beta1 * ms, keep2 = h.beta2 * vs;
+    unsigned mtop = 0, rtop = 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int64_t i = lo + q * 32 + lane;
-      mi[q] = ri[q] = 0.0f;
-      if (i < t.n[k]) {
-        const float gi = to_f32(g[i]) * c.grad_scale;
-        const float r = from_code(v[i]) * vs;
-        mi[q] = fmaf(h.beta1, from_code(m[i]) * ms, h.rest1 * gi);
-        const float vi = fmaf(h.beta2, r * r, h.rest2 * gi * gi);
-        ri[q] = sqrtf(vi);
-        const float pi = updated(to_f32(p[i]), mi[q], vi, h, c, keep);
-        p[i] = from_f32<P>(pi);
-        if (t.copy[k]) store_from_f32(t.copy[k], t.copy_type[k], i, pi);
-      }
-      mtop = __uint_as_float(max(__float_as_uint(mtop), __float_as_uint(fabsf(mi[q]))));
-      rtop = __uint_as_float(max(__float_as_uint(rtop), __float_as_uint(ri[q])));
+    for (int e = 0; e < 8; ++e) {
+      g[e] *= c.grad_scale;
+      m[e] = fmaf(keep1, m[e], h.rest1 * g[e]);
+      r[e] = sqrtf(fmaf(keep2 * r[e], vs * r[e], h.rest2 * g[e] * g[e]));
+      // The quotient may be off by two units: it is rounded with the parameter.
+      p[e] = fmaf(-c.step_size, __fdividef(m[e], fmaf(r[e], c.root_scale, h.eps)), p[e] * w.keep);
+      mtop = max(mtop, __float_as_uint(fabsf(m[e])));
+      rtop = max(rtop, __float_as_uint(r[e]));
     }
-    const float mscale = warp_top(mtop) / kTopCode, rscale = warp_top(rtop) / kTopCode;
-    const float m1 = mscale < kLeastScale ? kLeastScale : mscale, r1 = rscale < kLeastScale ? kLeastScale : rscale;
-    __syncwarp();  // every lane has read the old scales
-    if (lane == 0) {
-      t.ms[k][b] = m1;
-      t.vs[k][b] = r1;
+    const float ms1 = fmaxf_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, mtop)) / kTopCode, kLeastScale);
+    const float vs1 = fmaxf_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, rtop)) / kTopCode, kLeastScale);
+    if (lane == 0) {  // every lane has read the old ones: the maxima came after
+      t.ms[k][b] = ms1;
+      t.vs[k][b] = vs1;
     }
+    const float mi = 1.0f / ms1, ri = 1.0f / vs1;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int64_t i = lo + q * 32 + lane;
-      if (i < t.n[k]) {
-        m[i] = to_code(mi[q] / m1);
-        const float u = ri[q] / r1;
-        v[i] = to_code(u > 0.0f && u < kLeastCode ? kLeastCode : u);
-      }
+    for (int e = 0; e < 8; ++e) {
+      m[e] *= mi;
+      r[e] *= ri;
+      r[e] = r[e] > 0.0f && r[e] < kLeastCode ? kLeastCode : r[e];
+    }
+    if (whole) {
+      *reinterpret_cast<uint2 *>(w.m + i0) = encode8(m);
+      *reinterpret_cast<uint2 *>(w.v + i0) = encode8(r);
+      store8(w.p + i0, p);
+      if (w.copy) store_vec16<8>(w.copy, w.copy_type, i0, p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < mine) {
+          w.m[i0 + e] = to_code(m[e]);
+          w.v[i0 + e] = to_code(r[e]);
+          w.p[i0 + e] = from_f32<P>(p[e]);
+          if (w.copy) store_from_f32(w.copy, w.copy_type, i0 + e, p[e]);
+        }
     }
   }
 }
@@ -201,7 +292,7 @@ cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, u
         for (int i = 0; i < t.count; ++i) {
           u.first[i] = t.first[i];
           u.p[i] = t.p[i], u.g[i] = t.g[i], u.m[i] = t.m[i], u.v[i] = t.v[i], u.ms[i] = t.ms[i], u.vs[i] = t.vs[i];
-          u.copy[i] = t.copy[i], u.n[i] = t.n[i], u.decay[i] = t.decay[i], u.copy_type[i] = t.copy_type[i];
+          u.copy[i] = t.copy[i], u.n[i] = t.n[i], u.decay[i] = t.decay[i], u.copy_type[i] = t.copy_type[i], u.aligned[i] = t.aligned[i];
         }
         e = launch<P, G, kSmallCap>(u, p.bits8, most, s);
       } else {
@@ -222,6 +313,9 @@ cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, u
     t.vs[i] = p.bits8 ? p.v_scales[k] : nullptr;
     t.copy[i] = p.copies ? p.copies[k] : nullptr;
     t.copy_type[i] = (uint8_t)(p.copies ? p.copy_types[k] : 0);
+    const unsigned unit = p.bits8 ? 8 : 4;  // elements
+    t.aligned[i] = (uintptr_t)t.p[i] % (unit * sizeof(P)) == 0 && (uintptr_t)t.g[i] % (unit * sizeof(G)) == 0 &&
+                   ((uintptr_t)t.m[i] | (uintptr_t)t.v[i]) % (p.bits8 ? 8 : 16) == 0 && (uintptr_t)t.copy[i] % (unit * 2) == 0;
     t.n[i] = p.sizes[k];
     t.decay[i] = (float)p.decay[k];
   }

@@ -49,6 +49,91 @@ __device__ __forceinline__ void store_from_f32(void *p, int type, int64_t i, flo
   else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// ---- vectors of elements, as f32 --------------------------------------------------
+// load4 / store4 want the address aligned to four elements, load8 / store8 to
+// eight.  Loads skip L1: every use here reads an element once.
+__device__ __forceinline__ float2 unpack(unsigned v, __half) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+__device__ __forceinline__ float2 unpack(unsigned v, __nv_bfloat16) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ unsigned pack(float a, float b, __half) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ unsigned pack(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const unsigned *>(&h);
+}
+
+__device__ __forceinline__ uint2 ld_u2(const void *p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_u4(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void load4(const float *p, float v[4]) {
+  const float4 q = ld_f4(p);
+  v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+}
+template <class T>
+__device__ __forceinline__ void load4(const T *p, float v[4]) {
+  const uint2 q = ld_u2(p);
+  const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{});
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+__device__ __forceinline__ void store4(float *p, const float v[4]) { st_f4(p, make_float4(v[0], v[1], v[2], v[3])); }
+template <class T>
+__device__ __forceinline__ void store4(T *p, const float v[4]) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack(v[0], v[1], T{}), pack(v[2], v[3], T{}));
+}
+__device__ __forceinline__ void load8(const float *p, float v[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
+}
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float v[8]) {
+  const uint4 q = ld_u4(p);
+  const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{}), c = unpack(q.z, T{}), d = unpack(q.w, T{});
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+}
+__device__ __forceinline__ void store8(float *p, const float v[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+template <class T>
+__device__ __forceinline__ void store8(T *p, const float v[8]) {
+  *reinterpret_cast<uint4 *>(p) = make_uint4(pack(v[0], v[1], T{}), pack(v[2], v[3], T{}), pack(v[4], v[5], T{}),
+                                             pack(v[6], v[7], T{}));
+}
+template <int W, class T>
+__device__ __forceinline__ void load_vec(const T *p, float *v) {
+  if constexpr (W == 8) load8(p, v);
+  else load4(p, v);
+}
+template <int W, class T>
+__device__ __forceinline__ void store_vec(T *p, const float *v) {
+  if constexpr (W == 8) store8(p, v);
+  else store4(p, v);
+}
+// Into a 16-bit tensor whose type is known at run time.
+template <int W>
+__device__ __forceinline__ void store_vec16(void *p, int type, int64_t i, const float *v) {
+  if (type == kF16) store_vec<W>(static_cast<__half *>(p) + i, v);
+  else store_vec<W>(static_cast<__nv_bfloat16 *>(p) + i, v);
+}
+
 __device__ __forceinline__ float warp_sum_f32(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
