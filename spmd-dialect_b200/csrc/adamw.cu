@@ -22,13 +22,16 @@ namespace spmdb200 {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPiece = 2048;  // elements a block takes at a time: 8 warps of one 8-bit state block each
+constexpr int kMostUnits = 8;  // state blocks a warp takes in a row; at most 32, a lane for each one's scales
+
 constexpr int kQuads = kPiece / kThreads / 4;
 constexpr float kTopCode = 448.0f, kLeastCode = 0x1p-9f, kLeastScale = 0x1p-120f;
 
 struct AdamHyper {
   float beta1, beta2, rest1, rest2;  // 1 - beta, taken in f64
+  float root_beta2, root_rest2;     // sqrt(beta2), sqrt(1 - beta2)
   float eps;
   float lr, step_size, root_scale;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) (host step and lr)
   double beta1_d, beta2_d;          // for a step number on the device
@@ -50,7 +53,7 @@ struct AdamTable {
   int64_t n[CAP];
   float decay[CAP];
   uint8_t copy_type[CAP];
-  uint8_t aligned[CAP];  // every address is a multiple of 4 elements (32-bit states) or 8 (8-bit)
+  uint8_t aligned[CAP];  // p, g and the copy at multiples of 4 elements (32-bit states) or 8 (8-bit), states of 16 bytes
   int count;
 };
 constexpr int kSmallCap = 32, kLargeCap = 384;
@@ -104,7 +107,9 @@ __device__ __forceinline__ Tensor<P, G, S> tensor_at(const AdamTable<CAP> &t, in
 // Every element is read and written once, so the step is bound by memory: 28
 // bytes per element with f32 parameters and states, 16-bit gradients and
 // copies.  A thread takes quads of four elements (16-byte loads of f32, all of
-// a piece's loads before the first use).
+// a piece's loads before the first use), a block one piece: 2^28 parameters in
+// 1096 us (6.86 TB/s), against 1277 with eight blocks an SM that loop, 1227
+// with pieces of twice the size, 1274 of half.
 template <class P, class G, int CAP>
 __global__ void __launch_bounds__(kThreads, 4) adamw_32(const __grid_constant__ AdamTable<CAP> t) {
   __shared__ Now sh;
@@ -164,7 +169,46 @@ __device__ __forceinline__ float from_code(uint8_t c) {
 }
 __device__ __forceinline__ uint8_t to_code(float v) { return __nv_fp8_e4m3(v).__x; }
 
-__device__ __forceinline__ float fmaxf_nan(float a, float b) { return a < b ? b : a; }  // a NaN `a` stays
+// Square root and reciprocal to within 2^-23 of the value: an 8-bit root and
+// the change of a parameter (a small part of it) are rounded far more coarsely,
+// and exact ones would cost as many instructions as the rest of the step.  The
+// root keeps subnormal arguments, whose roots are normal; the reciprocal's
+// argument is normal or zero.
+__device__ __forceinline__ float sqrt_near(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_near(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// To half a unit or so: one step of Newton's on the near one.
+__device__ __forceinline__ float rcp_full(float v) {
+  const float y = rcp_near(v);
+  return fmaf(fmaf(-v, y, 1.0f), y, y);
+}
+__device__ __forceinline__ float ld_f1(const float *p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+// Maxima that keep a NaN.
+__device__ __forceinline__ float top_of(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float at_least(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Over the warp, of non-negative values: their bits order as they do, NaN above all.
+__device__ __forceinline__ float warp_top(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
 
 __device__ __forceinline__ void decode8(uint2 q, float v[8]) {
 #pragma unroll
@@ -182,101 +226,206 @@ __device__ __forceinline__ uint2 encode8(const float v[8]) {
   return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
-// A warp takes a state block of 256 elements, eight consecutive ones a lane:
-// the block's largest magnitudes are one integer maximum over the warp each
-// (bits of non-negative floats order as the floats do, NaN above all).
+// The 8-bit step of eight elements a lane, one state block a warp; m and r come
+// as decoded codes and leave as codes' values, with the block's new scales.
+//   m = keep1 code + gain1 g,  v = o^2 + q^2 with o = keep2 code, q = gain2 g
+// (the factors beta1 ms, sqrt(beta2) vs, (1 - beta1) grad_scale and sqrt(1 -
+// beta2) grad_scale are taken once: no square of a scale, which would leave
+// f32's range long before the root does).
+struct Scales {
+  float m, v;
+};
+__device__ __forceinline__ Scales step8(float p[8], const float g[8], float m[8], float r[8], Scales old, const Now &c,
+                                        const AdamHyper &h, float keep, float gain1, float gain2) {
+  const float keep1 = h.beta1 * old.m, keep2 = h.root_beta2 * old.v;
+  const F2 k1{keep1, keep1}, k2{keep2, keep2}, g1{gain1, gain1}, g2{gain2, gain2}, root{c.root_scale, c.root_scale},
+      eps{h.eps, h.eps}, size{-c.step_size, -c.step_size}, kp{keep, keep};
+  float mtop = 0.0f, rtop = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const F2 ge{g[e], g[e + 1]};
+    const F2 me = fma2(k1, {m[e], m[e + 1]}, mul2(g1, ge));
+    const F2 o = mul2(k2, {r[e], r[e + 1]}), q = mul2(g2, ge);
+    const F2 v = fma2(o, o, mul2(q, q));
+    const F2 re{sqrt_near(v.x), sqrt_near(v.y)};
+    const F2 den = fma2(re, root, eps);
+    const F2 pe = fma2(mul2(size, me), {rcp_near(den.x), rcp_near(den.y)}, mul2(kp, {p[e], p[e + 1]}));
+    m[e] = me.x, m[e + 1] = me.y;
+    r[e] = re.x, r[e + 1] = re.y;
+    p[e] = pe.x, p[e + 1] = pe.y;
+    mtop = top_of(mtop, fabsf(me.x), fabsf(me.y));
+    rtop = top_of(rtop, re.x, re.y);
+  }
+  const Scales now{at_least(warp_top(mtop) * (1.0f / kTopCode), kLeastScale),
+                   at_least(warp_top(rtop) * (1.0f / kTopCode), kLeastScale)};
+  const float mi = rcp_full(now.m), ri = rcp_full(now.v);
+  const F2 mi2{mi, mi}, ri2{ri, ri};
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const F2 me = mul2(mi2, {m[e], m[e + 1]}), re = mul2(ri2, {r[e], r[e + 1]});
+    m[e] = me.x, m[e + 1] = me.y;
+    r[e] = re.x > 0.0f ? at_least(re.x, kLeastCode) : re.x;
+    r[e + 1] = re.y > 0.0f ? at_least(re.y, kLeastCode) : re.y;
+  }
+  return now;
+}
+
+// What a warp has of one state block in shared memory: eight elements a lane of
+// p and g in 16-byte chunks, and both states' codes.
+template <class P, class G>
+struct Stage8 {
+  static constexpr int kP = sizeof(P) / 2, kG = sizeof(G) / 2;
+  uint4 p[kP][32], g[kG][32], codes[32];  // codes: m in the first half, v in the second
+};
+constexpr int kStages8 = 2;
+
+template <class T, int N>
+__device__ __forceinline__ void fetch_chunks(uint4 (&slot)[N][32], const T *src, int lane) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) copy_async16(&slot[q][lane], reinterpret_cast<const uint4 *>(src) + q);
+}
+template <class T, int N>
+__device__ __forceinline__ void take_chunks(const uint4 (&slot)[N][32], int lane, float v[8]) {
+  if constexpr (N == 1) {
+    load8(reinterpret_cast<const T *>(&slot[0][lane]), v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 f = *reinterpret_cast<const float4 *>(&slot[q][lane]);
+      v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
+    }
+  }
+}
+
+// A warp takes state blocks of 256 elements, eight consecutive ones a lane: the
+// block's largest magnitudes are one integer maximum over the warp each.  10
+// bytes an element against some 30 instructions, so that instructions and the
+// wait for memory both count: a warp has `units` blocks of a tensor in a row,
+// one look-up for all of them, and the next on its way to shared memory while
+// one is computed.  A grid of all pieces hides a block's first wait behind
+// others (217 us for 2^27 bf16 parameters, 6.2 TB/s; 240 with three blocks an
+// SM that loop).  Two stages and 80 registers (three blocks an SM) measured
+// best: 238 looping, three stages 245, 64 registers and four blocks 245.
 template <class P, class G, int CAP>
-__global__ void __launch_bounds__(kThreads, 4) adamw_8(const __grid_constant__ AdamTable<CAP> t) {
+__global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ AdamTable<CAP> t, int units) {
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Now sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Stage8<P, G> *stages = reinterpret_cast<Stage8<P, G> *>(smem) + warp * kStages8;
   const AdamHyper &h = t.h;
   const Now c = constants(h, &sh);
   if (!isfinite(c.grad_scale)) return;
-  const int lane = threadIdx.x & 31;
+  const float gain1 = h.rest1 * c.grad_scale, gain2 = h.root_rest2 * c.grad_scale;
   const int64_t pieces = t.first[t.count];
   int k = tensor_of(t.first, t.count, blockIdx.x);
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
     while (piece >= t.first[k + 1]) ++k;
     const Tensor<P, G, uint8_t> w = tensor_at<P, G, uint8_t>(t, k, c.lr);
-    const int64_t lo = (piece - t.first[k]) * kPiece + (threadIdx.x >> 5) * kStateBlock;
+    const int64_t lo = ((piece - t.first[k]) * kWarps + warp) * units * kStateBlock;
     if (lo >= w.n) continue;
-    const int64_t b = lo / kStateBlock;
-    const int64_t i0 = lo + 8 * lane;
-    const bool whole = w.aligned && lo + kStateBlock <= w.n;  // the same for the whole warp
-    const int mine = (int)(w.n - i0 < 8 ? (w.n > i0 ? w.n - i0 : 0) : 8);
-    float p[8], g[8], m[8], r[8];
-    if (whole) {
-      load8(w.g + i0, g);
-      decode8(ld_u2(w.m + i0), m);
-      decode8(ld_u2(w.v + i0), r);
-      load8(w.p + i0, p);
-    } else {
+    float *ms = t.ms[k] + lo / kStateBlock, *vs = t.vs[k] + lo / kStateBlock;
+    const int64_t left = (w.n - lo) / kStateBlock;
+    const int whole = !w.aligned ? 0 : left < units ? (int)left : units;  // the same for the whole warp
+    int64_t i = lo + 8 * lane;
+    const P *fp = w.p + i;
+    const G *fg = w.g + i;
+    const uint8_t *fc = (lane < 16 ? w.m : w.v) + lo + 16 * (lane & 15);
+    int ahead = 0;  // blocks fetched
+    auto fetch = [&] {
+      if (ahead < whole) {
+        Stage8<P, G> &s = stages[ahead % kStages8];
+        fetch_chunks(s.g, fg, lane);
+        copy_async16(&s.codes[lane], fc);
+        fetch_chunks(s.p, fp, lane);
+        fp += kStateBlock, fg += kStateBlock, fc += kStateBlock;
+        ++ahead;
+      }
+      copy_commit();  // empty past the last block, so that the count of groups stays
+    };
+#pragma unroll
+    for (int u = 0; u < kStages8 - 1; ++u) fetch();
+    // Lane u holds block u's scales from the start: loaded a block ahead only,
+    // they were what the warp waited for (305 against 245 us).
+    const bool scaled = lane < units && lo + lane * kStateBlock < w.n;
+    Scales mine{scaled ? ms[lane] : 0.0f, scaled ? vs[lane] : 0.0f};
+    auto scales = [&](int u) { return Scales{__shfl_sync(0xffffffffu, mine.m, u), __shfl_sync(0xffffffffu, mine.v, u)}; };
+    int u = 0;
+    for (; u < whole; ++u, i += kStateBlock) {
+      fetch();
+      copy_wait<kStages8 - 1>();
+      __syncwarp();  // the other lanes' copies are there too
+      const Stage8<P, G> &s = stages[u % kStages8];
+      float p[8], g[8], m[8], r[8];
+      decode8(reinterpret_cast<const uint2 *>(s.codes)[lane], m);
+      decode8(reinterpret_cast<const uint2 *>(s.codes + 16)[lane], r);
+      take_chunks<G>(s.g, lane, g);
+      take_chunks<P>(s.p, lane, p);
+      __syncwarp();  // the stage may be filled again
+      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep, gain1, gain2);
+      if (lane == u) mine = now;
+      *reinterpret_cast<uint2 *>(w.m + i) = encode8(m);
+      *reinterpret_cast<uint2 *>(w.v + i) = encode8(r);
+      store8(w.p + i, p);
+      if (w.copy) store_vec16<8>(w.copy, w.copy_type, i, p);
+    }
+    // A tensor's last block, and tensors at odd addresses.
+    for (; u < units && lo + u * kStateBlock < w.n; ++u, i += kStateBlock) {
+      const int64_t rest = w.n - i;
+      float p[8], g[8], m[8], r[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool in = e < mine;
-        p[e] = in ? to_f32(w.p[i0 + e]) : 0.0f;
-        g[e] = in ? to_f32(w.g[i0 + e]) : 0.0f;
-        m[e] = in ? from_code(w.m[i0 + e]) : 0.0f;
-        r[e] = in ? from_code(w.v[i0 + e]) : 0.0f;
+        p[e] = e < rest ? to_f32(w.p[i + e]) : 0.0f;
+        g[e] = e < rest ? to_f32(w.g[i + e]) : 0.0f;
+        m[e] = e < rest ? from_code(w.m[i + e]) : 0.0f;
+        r[e] = e < rest ? from_code(w.v[i + e]) : 0.0f;
       }
-    }
-    // The scales go into the factors once per block (not their square, which
-    // would leave f32's range long before the root does).
-    const float ms = t.ms[k][b], vs = t.vs[k][b];
-    const float keep1 = h.beta1 * ms, keep2 = h.beta2 * vs;
-    unsigned mtop = 0, rtop = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      g[e] *= c.grad_scale;
-      m[e] = fmaf(keep1, m[e], h.rest1 * g[e]);
-      r[e] = sqrtf(fmaf(keep2 * r[e], vs * r[e], h.rest2 * g[e] * g[e]));
-      // The quotient may be off by two units: it is rounded with the parameter.
-      p[e] = fmaf(-c.step_size, __fdividef(m[e], fmaf(r[e], c.root_scale, h.eps)), p[e] * w.keep);
-      mtop = max(mtop, __float_as_uint(fabsf(m[e])));
-      rtop = max(rtop, __float_as_uint(r[e]));
-    }
-    const float ms1 = fmaxf_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, mtop)) / kTopCode, kLeastScale);
-    const float vs1 = fmaxf_nan(__uint_as_float(__reduce_max_sync(0xffffffffu, rtop)) / kTopCode, kLeastScale);
-    if (lane == 0) {  // every lane has read the old ones: the maxima came after
-      t.ms[k][b] = ms1;
-      t.vs[k][b] = vs1;
-    }
-    const float mi = 1.0f / ms1, ri = 1.0f / vs1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m[e] *= mi;
-      r[e] *= ri;
-      r[e] = r[e] > 0.0f && r[e] < kLeastCode ? kLeastCode : r[e];
-    }
-    if (whole) {
-      *reinterpret_cast<uint2 *>(w.m + i0) = encode8(m);
-      *reinterpret_cast<uint2 *>(w.v + i0) = encode8(r);
-      store8(w.p + i0, p);
-      if (w.copy) store_vec16<8>(w.copy, w.copy_type, i0, p);
-    } else {
+      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep, gain1, gain2);
+      if (lane == u) mine = now;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (e < mine) {
-          w.m[i0 + e] = to_code(m[e]);
-          w.v[i0 + e] = to_code(r[e]);
-          w.p[i0 + e] = from_f32<P>(p[e]);
-          if (w.copy) store_from_f32(w.copy, w.copy_type, i0 + e, p[e]);
+        if (e < rest) {
+          w.m[i + e] = to_code(m[e]);
+          w.v[i + e] = to_code(r[e]);
+          w.p[i + e] = from_f32<P>(p[e]);
+          if (w.copy) store_from_f32(w.copy, w.copy_type, i + e, p[e]);
         }
     }
+    if (scaled) {
+      ms[lane] = mine.m;
+      vs[lane] = mine.v;
+    }
   }
+  copy_wait<0>();
 }
 
 template <class P, class G, int CAP>
-cudaError_t launch(const AdamTable<CAP> &t, bool bits8, unsigned most, cudaStream_t s) {
+cudaError_t launch(AdamTable<CAP> &t, bool bits8, unsigned sms, cudaStream_t s) {
   const int64_t pieces = t.first[t.count];
-  const unsigned grid = (unsigned)(pieces < (int64_t)most ? pieces : (int64_t)most);
-  if (bits8) adamw_8<P, G, CAP><<<grid, kThreads, 0, s>>>(t);
-  else adamw_32<P, G, CAP><<<grid, kThreads, 0, s>>>(t);
+  if (!bits8) {
+    const int64_t most = INT32_MAX;
+    adamw_32<P, G, CAP><<<(unsigned)(pieces < most ? pieces : most), kThreads, 0, s>>>(t);
+    return cudaGetLastError();
+  }
+  // As many state blocks in a row per warp as leave every SM 32 pieces, up to
+  // kMostUnits (234 us at 4 for 2^27 parameters, 217 at 8, 16 and 32).
+  int units = 1;
+  while (units < kMostUnits && pieces >= (int64_t)units * 2 * 32 * sms) units *= 2;
+  int64_t at = 0;
+  for (int i = 0; i < t.count; ++i) {
+    t.first[i] = at;
+    at += (t.n[i] + units * kPiece - 1) / (units * kPiece);
+  }
+  t.first[t.count] = at;
+  constexpr int bytes = kWarps * kStages8 * (int)sizeof(Stage8<P, G>);
+  if (cudaError_t e = cudaFuncSetAttribute(adamw_8<P, G, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  const int64_t most = INT32_MAX;
+  adamw_8<P, G, CAP><<<(unsigned)(at < most ? at : most), kThreads, bytes, s>>>(t, units);
   return cudaGetLastError();
 }
 
 // Launches for the tensors of one type pair, kLargeCap of them at a time.
 template <class P, class G>
-cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, unsigned most, cudaStream_t s) {
+cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, unsigned sms, cudaStream_t s) {
   AdamTable<kLargeCap> t;
   t.h = h;
   t.count = 0;
@@ -294,9 +443,9 @@ cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, u
           u.p[i] = t.p[i], u.g[i] = t.g[i], u.m[i] = t.m[i], u.v[i] = t.v[i], u.ms[i] = t.ms[i], u.vs[i] = t.vs[i];
           u.copy[i] = t.copy[i], u.n[i] = t.n[i], u.decay[i] = t.decay[i], u.copy_type[i] = t.copy_type[i], u.aligned[i] = t.aligned[i];
         }
-        e = launch<P, G, kSmallCap>(u, p.bits8, most, s);
+        e = launch<P, G, kSmallCap>(u, p.bits8, sms, s);
       } else {
-        e = launch<P, G, kLargeCap>(t, p.bits8, most, s);
+        e = launch<P, G, kLargeCap>(t, p.bits8, sms, s);
       }
       if (e) return e;
       t.count = 0;
@@ -315,7 +464,7 @@ cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, u
     t.copy_type[i] = (uint8_t)(p.copies ? p.copy_types[k] : 0);
     const unsigned unit = p.bits8 ? 8 : 4;  // elements
     t.aligned[i] = (uintptr_t)t.p[i] % (unit * sizeof(P)) == 0 && (uintptr_t)t.g[i] % (unit * sizeof(G)) == 0 &&
-                   ((uintptr_t)t.m[i] | (uintptr_t)t.v[i]) % (p.bits8 ? 8 : 16) == 0 && (uintptr_t)t.copy[i] % (unit * 2) == 0;
+                   ((uintptr_t)t.m[i] | (uintptr_t)t.v[i]) % 16 == 0 && (uintptr_t)t.copy[i] % (unit * 2) == 0;
     t.n[i] = p.sizes[k];
     t.decay[i] = (float)p.decay[k];
   }
@@ -323,10 +472,10 @@ cudaError_t step_of(const AdamWProblem &p, int pt, int gt, const AdamHyper &h, u
 }
 
 template <class P>
-cudaError_t step_of_params(const AdamWProblem &p, int pt, const AdamHyper &h, unsigned most, cudaStream_t s) {
-  if (cudaError_t e = step_of<P, float>(p, pt, kF32, h, most, s)) return e;
-  if (cudaError_t e = step_of<P, __half>(p, pt, kF16, h, most, s)) return e;
-  return step_of<P, __nv_bfloat16>(p, pt, kBF16, h, most, s);
+cudaError_t step_of_params(const AdamWProblem &p, int pt, const AdamHyper &h, unsigned sms, cudaStream_t s) {
+  if (cudaError_t e = step_of<P, float>(p, pt, kF32, h, sms, s)) return e;
+  if (cudaError_t e = step_of<P, __half>(p, pt, kF16, h, sms, s)) return e;
+  return step_of<P, __nv_bfloat16>(p, pt, kBF16, h, sms, s);
 }
 
 }  // namespace
@@ -337,6 +486,7 @@ cudaError_t launch_adamw(const AdamWProblem &p, cudaStream_t s) {
   AdamHyper h{};
   h.beta1 = (float)p.beta1, h.beta2 = (float)p.beta2;
   h.rest1 = (float)(1.0 - p.beta1), h.rest2 = (float)(1.0 - p.beta2);
+  h.root_beta2 = (float)sqrt(p.beta2), h.root_rest2 = (float)sqrt(1.0 - p.beta2);
   h.eps = (float)p.eps;
   h.beta1_d = p.beta1, h.beta2_d = p.beta2;
   h.lr = (float)p.lr;
@@ -348,10 +498,10 @@ cudaError_t launch_adamw(const AdamWProblem &p, cudaStream_t s) {
   h.lr_dev = p.lr_dev;
   h.step_dev = p.step_dev;
   h.grad_scale = p.grad_scale;
-  const unsigned most = (unsigned)num_sms(dev) * 8;
-  if (cudaError_t e = step_of_params<float>(p, kF32, h, most, s)) return e;
-  if (cudaError_t e = step_of_params<__half>(p, kF16, h, most, s)) return e;
-  return step_of_params<__nv_bfloat16>(p, kBF16, h, most, s);
+  const unsigned sms = (unsigned)num_sms(dev);
+  if (cudaError_t e = step_of_params<float>(p, kF32, h, sms, s)) return e;
+  if (cudaError_t e = step_of_params<__half>(p, kF16, h, sms, s)) return e;
+  return step_of_params<__nv_bfloat16>(p, kBF16, h, sms, s);
 }
 
 }  // namespace spmdb200

@@ -101,12 +101,6 @@ __device__ __forceinline__ void load8(const float *p, float v[8]) {
                : "l"(p)
                : "memory");
 }
-template <class T>
-__device__ __forceinline__ void load8(const T *p, float v[8]) {
-  const uint4 q = ld_u4(p);
-  const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{}), c = unpack(q.z, T{}), d = unpack(q.w, T{});
-  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
-}
 __device__ __forceinline__ void store8(float *p, const float v[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
                "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
@@ -117,11 +111,44 @@ __device__ __forceinline__ void store8(T *p, const float v[8]) {
   *reinterpret_cast<uint4 *>(p) = make_uint4(pack(v[0], v[1], T{}), pack(v[2], v[3], T{}), pack(v[4], v[5], T{}),
                                              pack(v[6], v[7], T{}));
 }
-template <int W, class T>
-__device__ __forceinline__ void load_vec(const T *p, float *v) {
-  if constexpr (W == 8) load8(p, v);
-  else load4(p, v);
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float v[8]) {  // any address space
+  const uint4 q = *reinterpret_cast<const uint4 *>(p);
+  const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{}), c = unpack(q.z, T{}), d = unpack(q.w, T{});
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
 }
+
+// ---- asynchronous 16-byte copies to shared memory --------------------------------------
+__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Two f32 operations in one instruction, each rounded as the single one.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 template <int W, class T>
 __device__ __forceinline__ void store_vec(T *p, const float *v) {
   if constexpr (W == 8) store8(p, v);

@@ -7,7 +7,6 @@ All compute happens in libspmdb200.so; nothing here computes anything.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from array import array
 
@@ -221,38 +220,53 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _FLOATS = frozenset(_TYPES)
 _E4M3 = torch.float8_e4m3fn
 STATE_BLOCK = 256  # elements that share one scale of an 8-bit optimizer state
+_get_device, _is_contiguous, _data_ptr, _numel = (getattr(torch.Tensor, n) for n in (
+    "get_device", "is_contiguous", "data_ptr", "numel"))
+
+
+def _elsewhere(dev: int, stream) -> bool:
+    """Whether a call has to enter a stream or device first (_at)."""
+    if dev < 0:
+        raise ValueError("device entries take CUDA tensors")
+    return stream is not None or dev != torch._C._cuda_getDevice()
 
 
 def _at(dev: int, stream):
-    """Context in which launches and allocations belong to `stream` (or to the
-    current stream of device `dev`)."""
-    if dev < 0:
-        raise ValueError("device entries take CUDA tensors")
-    if stream is not None:
-        if stream.device_index != dev:
-            raise ValueError(f"the stream belongs to cuda:{stream.device_index}, the tensors to cuda:{dev}")
-        return torch.cuda.stream(stream)
-    return contextlib.nullcontext() if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    """Context in which launches and allocations belong to `stream`, or to the
+    current stream of device `dev`."""
+    if stream is None:
+        return torch.cuda.device(dev)
+    if stream.device_index != dev:
+        raise ValueError(f"the stream belongs to cuda:{stream.device_index}, the tensors to cuda:{dev}")
+    return torch.cuda.stream(stream)
 
 
-def _ptr(vals: array | None) -> int | None:
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _ptr(a: array | None) -> int | None:
     """Address of a host array, which the caller keeps until the call is over."""
-    return None if vals is None else vals.buffer_info()[0]
+    return None if a is None else a.buffer_info()[0]
 
 
 def _norm_operand(name: str, t: torch.Tensor, shape, dev: int, dtype=None) -> None:
     if t.get_device() != dev:
         raise ValueError(f"layer_norm: {name} is not on x's device")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype or t.dtype not in _TYPES:
+    if (t.dtype != dtype) if dtype is not None else (t.dtype not in _TYPES):
         raise TypeError(f"layer_norm: {name} has dtype {t.dtype}")
+
+
+def _norm_vector(name: str, t: torch.Tensor, shape, dev: int, dtype=None) -> None:
+    _norm_operand(name, t, shape, dev, dtype)
+    if not t.is_contiguous():
+        raise ValueError(f"layer_norm: {name} must be contiguous")
 
 
 def _norm_rows(name: str, t: torch.Tensor) -> torch.Tensor:
     """A view of rank 1-3 (leading dimensions merged where the rank is higher)."""
-    if t.dim() < 1:
-        raise ValueError(f"layer_norm: {name} needs a dimension to normalise over")
     if t.dim() <= 3:
         return t
     try:
@@ -261,15 +275,11 @@ def _norm_rows(name: str, t: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"layer_norm: the leading dimensions of {name} do not merge into rows") from None
 
 
-def _norm_weight(name: str, t: torch.Tensor, cols: int, dev: int) -> None:
-    _norm_operand(name, t, (cols,), dev)
-    if not t.is_contiguous():
-        raise ValueError(f"layer_norm: {name} must be contiguous")
-
-
-def _same_or_f32(a: torch.dtype, b: torch.dtype) -> None:
-    if a != b and a != torch.float32 and b != torch.float32:
-        raise TypeError(f"layer_norm: {a} and {b}: equal, or one of them float32")
+def _norm_types(x: torch.Tensor, y: torch.dtype) -> None:
+    if x.dtype not in _TYPES or y not in _TYPES:
+        raise TypeError(f"layer_norm: dtypes {x.dtype}, {y}")
+    if x.dtype != y and x.dtype != torch.float32 and y != torch.float32:
+        raise TypeError(f"layer_norm: {x.dtype} and {y}: equal, or one of them float32")
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -280,34 +290,36 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x's; one of the two may be float32) and may be x itself.  mean and rstd
     (float32, x's leading shape) are what layer_norm_backward takes; stats=False
     leaves them out (None)."""
-    if x.dtype not in _TYPES:
-        raise TypeError(f"layer_norm: unsupported dtype {x.dtype}")
     dev = x.get_device()
-    with _at(dev, stream):
-        if x.dim() < 1:
-            raise ValueError("layer_norm: x needs a dimension to normalise over")
-        lead, cols = x.shape[:-1], x.shape[-1]
-        if out is None:
-            out = torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
-        _norm_operand("out", out, x.shape, dev, dtype)
-        _same_or_f32(x.dtype, out.dtype)
-        wtype = 0
-        for name, t in (("weight", weight), ("bias", bias)):
-            if t is not None:
-                _norm_weight(name, t, cols, dev)
-                wtype = _TYPES[t.dtype]
-        if weight is not None and bias is not None and weight.dtype != bias.dtype:
-            raise TypeError("layer_norm: weight and bias must have one dtype")
-        mean = rstd = None
-        if stats:
-            mean = torch.empty(lead, dtype=torch.float32, device=x.device)
-            rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
-        xv, ov = _norm_rows("x", x), _norm_rows("out", out)
-        sizes, xs, os_ = array("q", xv.shape), array("q", xv.stride()), array("q", ov.stride())
-        call("spmdb200_layer_norm", xv.dim(), _ptr(sizes), xv.data_ptr(), _TYPES[x.dtype], _ptr(xs), ov.data_ptr(),
-             _TYPES[out.dtype], _ptr(os_), None if weight is None else weight.data_ptr(),
-             None if bias is None else bias.data_ptr(), wtype, eps, None if mean is None else mean.data_ptr(),
-             None if rstd is None else rstd.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    if _elsewhere(dev, stream):
+        with _at(dev, stream):
+            return layer_norm(x, weight, bias, eps, dtype, out, stats)
+    shape = x.shape
+    if not shape:
+        raise ValueError("layer_norm: x needs a dimension to normalise over")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
+    else:
+        _norm_operand("out", out, shape, dev, dtype)
+    _norm_types(x, out.dtype)
+    w = b = m = r = mean = rstd = None
+    wtype = 0
+    if weight is not None:
+        _norm_vector("weight", weight, shape[-1:], dev)
+        w, wtype = weight.data_ptr(), _TYPES[weight.dtype]
+    if bias is not None:
+        _norm_vector("bias", bias, shape[-1:], dev, None if weight is None else weight.dtype)
+        b, wtype = bias.data_ptr(), _TYPES[bias.dtype]
+    if stats:
+        mean = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        m, r = mean.data_ptr(), rstd.data_ptr()
+    xv, ov = _norm_rows("x", x), _norm_rows("out", out)
+    rank = xv.dim()
+    dims = array("q", (*xv.shape, *xv.stride(), *ov.stride()))
+    at = _ptr(dims)
+    call("spmdb200_layer_norm", rank, at, xv.data_ptr(), _TYPES[x.dtype], at + 8 * rank, ov.data_ptr(),
+         _TYPES[out.dtype], at + 16 * rank, w, b, wtype, eps, m, r, _raw_stream(dev))
     return out, mean, rstd
 
 
@@ -325,62 +337,65 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     dx has x's dtype and may be dy or x itself; dweight and dbias have weight's
     dtype (float32 without a weight) unless tensors are given.  wgrad=False
     leaves both out (None), the default without a weight."""
-    if x.dtype not in _TYPES:
-        raise TypeError(f"layer_norm: unsupported dtype {x.dtype}")
     dev = x.get_device()
-    with _at(dev, stream):
-        if x.dim() < 1:
-            raise ValueError("layer_norm: x needs a dimension to normalise over")
-        lead, cols = x.shape[:-1], x.shape[-1]
-        _norm_operand("dy", dy, x.shape, dev)
-        _same_or_f32(x.dtype, dy.dtype)
-        for name, t in (("mean", mean), ("rstd", rstd)):
-            _norm_operand(name, t, lead, dev, torch.float32)
-            if not t.is_contiguous():
-                raise ValueError(f"layer_norm: {name} must be contiguous")
-        if weight is not None:
-            _norm_weight("weight", weight, cols, dev)
-        if wgrad is None:
-            wgrad = weight is not None or dweight is not None or dbias is not None
-        if wgrad:
-            given = dweight if dweight is not None else dbias
-            kind = given.dtype if given is not None else weight.dtype if weight is not None else torch.float32
-            dweight = torch.empty(cols, dtype=kind, device=x.device) if dweight is None else dweight
-            dbias = torch.empty(cols, dtype=kind, device=x.device) if dbias is None else dbias
-            _norm_weight("dweight", dweight, cols, dev)
-            _norm_weight("dbias", dbias, cols, dev)
-            if dweight.dtype != dbias.dtype:
-                raise TypeError("layer_norm: dweight and dbias must have one dtype")
-        elif dweight is not None or dbias is not None:
-            raise ValueError("layer_norm: dweight or dbias given with wgrad=False")
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if dx is None else dx
-        _norm_operand("dx", dx, x.shape, dev, x.dtype)
-        gv, xv, dv = _norm_rows("dy", dy), _norm_rows("x", x), _norm_rows("dx", dx)
-        rows = mean.numel()
-        if ws is None:
-            ws = layer_norm_workspace(rows, cols, x.device)
-        elif ws.get_device() != dev or not ws.is_contiguous():
-            raise ValueError("layer_norm: ws is a contiguous tensor on x's device")
-        sizes = array("q", xv.shape)
-        gs, xs, ds = array("q", gv.stride()), array("q", xv.stride()), array("q", dv.stride())
-        call("spmdb200_layer_norm_backward", xv.dim(), _ptr(sizes), gv.data_ptr(), _TYPES[dy.dtype], _ptr(gs),
-             xv.data_ptr(), _TYPES[x.dtype], _ptr(xs), mean.data_ptr(), rstd.data_ptr(),
-             None if weight is None else weight.data_ptr(), 0 if weight is None else _TYPES[weight.dtype],
-             dv.data_ptr(), _ptr(ds), None if not wgrad else dweight.data_ptr(),
-             None if not wgrad else dbias.data_ptr(), 0 if not wgrad else _TYPES[dweight.dtype], ws.data_ptr(),
-             ws.numel() * ws.element_size(), torch.cuda.current_stream().cuda_stream)
+    if _elsewhere(dev, stream):
+        with _at(dev, stream):
+            return layer_norm_backward(dy, x, mean, rstd, weight, wgrad, dx, dweight, dbias, ws)
+    shape = x.shape
+    if not shape:
+        raise ValueError("layer_norm: x needs a dimension to normalise over")
+    _norm_operand("dy", dy, shape, dev)
+    _norm_types(x, dy.dtype)
+    _norm_vector("mean", mean, shape[:-1], dev, torch.float32)
+    _norm_vector("rstd", rstd, shape[:-1], dev, torch.float32)
+    w = dw = db = None
+    wtype = dtype = 0
+    if weight is not None:
+        _norm_vector("weight", weight, shape[-1:], dev)
+        w, wtype = weight.data_ptr(), _TYPES[weight.dtype]
+    if wgrad is None:
+        wgrad = weight is not None or dweight is not None or dbias is not None
+    if wgrad:
+        given = dweight if dweight is not None else dbias if dbias is not None else weight
+        kind = torch.float32 if given is None else given.dtype
+        dweight = torch.empty(shape[-1:], dtype=kind, device=x.device) if dweight is None else dweight
+        dbias = torch.empty(shape[-1:], dtype=kind, device=x.device) if dbias is None else dbias
+        _norm_vector("dweight", dweight, shape[-1:], dev)
+        _norm_vector("dbias", dbias, shape[-1:], dev, dweight.dtype)
+        dw, db, dtype = dweight.data_ptr(), dbias.data_ptr(), _TYPES[dweight.dtype]
+    elif dweight is not None or dbias is not None:
+        raise ValueError("layer_norm: dweight or dbias given with wgrad=False")
+    if dx is None:
+        dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    else:
+        _norm_operand("dx", dx, shape, dev, x.dtype)
+    gv, xv, dv = _norm_rows("dy", dy), _norm_rows("x", x), _norm_rows("dx", dx)
+    if ws is None:
+        ws = layer_norm_workspace(mean.numel(), shape[-1], x.device)
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError("layer_norm: ws is a contiguous tensor on x's device")
+    rank = xv.dim()
+    dims = array("q", (*xv.shape, *gv.stride(), *xv.stride(), *dv.stride()))
+    at = _ptr(dims)
+    call("spmdb200_layer_norm_backward", rank, at, gv.data_ptr(), _TYPES[dy.dtype], at + 8 * rank, xv.data_ptr(),
+         _TYPES[x.dtype], at + 16 * rank, mean.data_ptr(), rstd.data_ptr(), w, wtype, dv.data_ptr(), at + 24 * rank, dw,
+         db, dtype, ws.data_ptr(), ws.nbytes, _raw_stream(dev))
     return dx, dweight, dbias
 
 
-def _listed(what: str, tensors, dev: int, dtypes) -> list:
+def _listed(what: str, tensors: list, dev: int, dtypes) -> array:
     """Addresses of a list of contiguous tensors of `dtypes` on device `dev`."""
-    if any(d != dev for d in map(torch.Tensor.get_device, tensors)):
+    if not {dev}.issuperset(map(_get_device, tensors)):
         raise ValueError(f"{what}: every tensor must be on one CUDA device")
-    if not all(map(torch.Tensor.is_contiguous, tensors)):
+    if not all(map(_is_contiguous, tensors)):
         raise ValueError(f"{what}: every tensor must be contiguous")
     if not dtypes.issuperset([t.dtype for t in tensors]):
-        raise TypeError(f"{what}: dtypes {sorted(str(t.dtype) for t in tensors if t.dtype not in dtypes)}")
-    return list(map(torch.Tensor.data_ptr, tensors))
+        raise TypeError(f"{what}: dtypes {sorted({str(t.dtype) for t in tensors} - {str(d) for d in dtypes})}")
+    return array("Q", map(_data_ptr, tensors))
+
+
+def _types(tensors: list) -> array:
+    return array("i", [_TYPES[t.dtype] for t in tensors])
 
 
 def grad_norm(grads, max_norm: float | None = None, ws: torch.Tensor | None = None, stream=None):
@@ -390,19 +405,19 @@ def grad_norm(grads, max_norm: float | None = None, ws: torch.Tensor | None = No
     scale as its grad_scale, with no read by the host in between."""
     grads = list(grads)
     dev = grads[0].get_device() if grads else torch.cuda.current_device()
-    with _at(dev, stream):
-        ptrs = array("Q", _listed("grad_norm", grads, dev, _FLOATS))
-        sizes, types = array("q", map(torch.Tensor.numel, grads)), array("i", [_TYPES[t.dtype] for t in grads])
-        if ws is None:
-            ws = torch.empty(int(lib().spmdb200_grad_norm_workspace_bytes(len(grads))), dtype=torch.uint8,
-                             device=f"cuda:{dev}")
-        elif ws.get_device() != dev or not ws.is_contiguous():
-            raise ValueError("grad_norm: ws is a contiguous tensor on the gradients' device")
-        norm = torch.empty(1, dtype=torch.float32, device=ws.device)
-        scale = None if max_norm is None else torch.empty(1, dtype=torch.float32, device=ws.device)
-        call("spmdb200_grad_norm", len(grads), _ptr(ptrs), _ptr(sizes), _ptr(types),
-             0.0 if max_norm is None else max_norm, norm.data_ptr(), None if scale is None else scale.data_ptr(),
-             ws.data_ptr(), ws.numel() * ws.element_size(), torch.cuda.current_stream().cuda_stream)
+    if _elsewhere(dev, stream):
+        with _at(dev, stream):
+            return grad_norm(grads, max_norm, ws)
+    ptrs, sizes, types = _listed("grad_norm", grads, dev, _FLOATS), array("q", map(_numel, grads)), _types(grads)
+    if ws is None:
+        ws = torch.empty(int(lib().spmdb200_grad_norm_workspace_bytes(len(grads))), dtype=torch.uint8,
+                         device=f"cuda:{dev}")
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError("grad_norm: ws is a contiguous tensor on the gradients' device")
+    norm = torch.empty(1, dtype=torch.float32, device=ws.device)
+    scale = None if max_norm is None else torch.empty_like(norm)
+    call("spmdb200_grad_norm", len(grads), _ptr(ptrs), _ptr(sizes), _ptr(types), 0.0 if max_norm is None else max_norm,
+         norm.data_ptr(), None if scale is None else scale.data_ptr(), ws.data_ptr(), ws.nbytes, _raw_stream(dev))
     return norm, scale
 
 
@@ -411,7 +426,7 @@ def adamw_state(params, bits: int = 32) -> dict:
     (float32, or float8_e4m3fn codes for bits=8) and for bits=8 their scales."""
     if bits not in (8, 32):
         raise ValueError("adamw: states have 8 or 32 bits")
-    kind = torch.float32 if bits == 32 else _E4M3
+    params, kind = list(params), torch.float32 if bits == 32 else _E4M3
     names = ["exp_avg", "exp_avg_sq"]
     state = {n: [torch.zeros(p.shape, dtype=kind, device=p.device) for p in params] for n in names}
     if bits == 8:
@@ -433,55 +448,60 @@ def adamw(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), e
     """One AdamW step over lists of contiguous tensors, in place; returns params.
 
     params and grads are float32, float16 or bfloat16, independently.  States
-    are float32, or float8_e4m3fn with their `*_scales` (adamw_state makes
-    either).  copies: per parameter a float16 / bfloat16 tensor that receives
-    the new value too, or None.  weight_decay: a number, or one per parameter.
-    step (from 1) and lr are numbers, or one-element device tensors (int64,
-    float32) that a captured step reads anew at each replay.  grad_scale
-    multiplies every gradient; when it is NaN or infinite nothing is changed."""
+    hold as many elements as their parameter: float32, or float8_e4m3fn with
+    their `*_scales` (adamw_state makes either).  copies: per parameter a
+    float16 / bfloat16 tensor that receives the new value too, or None.
+    weight_decay: a number, or one per parameter.  step (from 1) and lr are
+    numbers, or one-element device tensors (int64, float32) that a captured
+    step reads anew at each replay.  grad_scale multiplies every gradient; when
+    it is NaN or infinite nothing is changed."""
     params, grads, exp_avg, exp_avg_sq = list(params), list(grads), list(exp_avg), list(exp_avg_sq)
     n = len(params)
     if not n:
+        if grads or exp_avg or exp_avg_sq:
+            raise ValueError("adamw: no parameters for the tensors given")
         return params
-    bits = 8 if exp_avg_scales is not None or exp_avg_sq_scales is not None else 32
-    lists = [("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)]
-    shapes = [p.shape for p in params]
-    for name, ts in lists:
-        if [t.shape for t in ts] != shapes:
-            raise ValueError(f"adamw: {name} must have the parameters' shapes")
     dev = params[0].get_device()
-    state_type = {torch.float32} if bits == 32 else {_E4M3}
-    with _at(dev, stream):
-        arrays = [array("Q", _listed("adamw: params", params, dev, _FLOATS)),
-                  array("Q", _listed("adamw: grads", grads, dev, _FLOATS)),
-                  array("Q", _listed("adamw: exp_avg", exp_avg, dev, state_type)),
-                  array("Q", _listed("adamw: exp_avg_sq", exp_avg_sq, dev, state_type))]
-        p_types, g_types = (array("i", [_TYPES[t.dtype] for t in ts]) for ts in (params, grads))
-        sizes = array("q", map(torch.Tensor.numel, params))
-        scale_lists = [None, None]
-        if bits == 8:
-            for k, ts in enumerate((exp_avg_scales, exp_avg_sq_scales)):
-                ts = list(ts) if ts is not None else []
-                if [t.numel() for t in ts] != [-(-m // STATE_BLOCK) for m in sizes]:
-                    raise ValueError(f"adamw: 8-bit states need one scale per {STATE_BLOCK} elements of each parameter")
-                scale_lists[k] = array("Q", _listed("adamw: scales", ts, dev, {torch.float32}))
-        copy_ptrs = copy_types = None
-        if copies is not None:
-            copies = list(copies)
-            if len(copies) != n or any(c is not None and c.shape != s for c, s in zip(copies, shapes)):
-                raise ValueError("adamw: copies must have the parameters' shapes")
-            there = [c for c in copies if c is not None]
-            ptrs = iter(_listed("adamw: copies", there, dev, {torch.float16, torch.bfloat16}))
-            copy_ptrs = array("Q", [0 if c is None else next(ptrs) for c in copies])
-            copy_types = array("i", [0 if c is None else _TYPES[c.dtype] for c in copies])
-        decay = array("d", weight_decay) if hasattr(weight_decay, "__len__") else array("d", [weight_decay]) * n
-        if len(decay) != n:
-            raise ValueError("adamw: weight_decay is a number or one per parameter")
-        lr_dev = _scalar("lr", lr, dev, torch.float32) if isinstance(lr, torch.Tensor) else None
-        step_dev = _scalar("step", step, dev, torch.int64) if isinstance(step, torch.Tensor) else None
-        factor = None if grad_scale is None else _scalar("grad_scale", grad_scale, dev, torch.float32)
-        call("spmdb200_adamw", n, _ptr(arrays[0]), _ptr(p_types), _ptr(arrays[1]), _ptr(g_types), _ptr(sizes),
-             _ptr(arrays[2]), _ptr(arrays[3]), bits, _ptr(scale_lists[0]), _ptr(scale_lists[1]), _ptr(copy_ptrs),
-             _ptr(copy_types), _ptr(decay), 0.0 if lr_dev else lr, lr_dev, betas[0], betas[1], eps, 1 if step_dev else step, step_dev, factor,
-             torch.cuda.current_stream().cuda_stream)
+    if _elsewhere(dev, stream):
+        with _at(dev, stream):
+            return adamw(params, grads, exp_avg, exp_avg_sq, step=step, lr=lr, betas=betas, eps=eps,
+                         weight_decay=weight_decay, exp_avg_scales=exp_avg_scales, exp_avg_sq_scales=exp_avg_sq_scales,
+                         copies=copies, grad_scale=grad_scale)
+    shapes, sizes = [p.shape for p in params], array("q", map(_numel, params))
+    if [g.shape for g in grads] != shapes:
+        raise ValueError("adamw: grads must have the parameters' shapes")
+    if array("q", map(_numel, exp_avg)) != sizes or array("q", map(_numel, exp_avg_sq)) != sizes:
+        raise ValueError("adamw: exp_avg and exp_avg_sq must have the parameters' sizes")
+    bits = 8 if exp_avg_scales is not None or exp_avg_sq_scales is not None else 32
+    kind = {torch.float32} if bits == 32 else {_E4M3}
+    p, g = _listed("adamw: params", params, dev, _FLOATS), _listed("adamw: grads", grads, dev, _FLOATS)
+    m, v = _listed("adamw: exp_avg", exp_avg, dev, kind), _listed("adamw: exp_avg_sq", exp_avg_sq, dev, kind)
+    p_types, g_types = _types(params), _types(grads)
+    m_scales = v_scales = c = c_types = None
+    if bits == 8:
+        blocks = array("q", [-(-k // STATE_BLOCK) for k in sizes])
+        lists = [list(ts) if ts is not None else [] for ts in (exp_avg_scales, exp_avg_sq_scales)]
+        if any(array("q", map(_numel, ts)) != blocks for ts in lists):
+            raise ValueError(f"adamw: 8-bit states need one scale per {STATE_BLOCK} elements of each parameter")
+        m_scales, v_scales = (_listed("adamw: scales", ts, dev, {torch.float32}) for ts in lists)
+    if copies is not None:
+        copies = list(copies)
+        if len(copies) != n or any(t is not None and t.shape != s for t, s in zip(copies, shapes)):
+            raise ValueError("adamw: copies must have the parameters' shapes")
+        ptrs = iter(_listed("adamw: copies", [t for t in copies if t is not None], dev, {torch.float16, torch.bfloat16}))
+        c = array("Q", [0 if t is None else next(ptrs) for t in copies])
+        c_types = array("i", [0 if t is None else _TYPES[t.dtype] for t in copies])
+    decay = array("d", weight_decay) if hasattr(weight_decay, "__len__") else array("d", [weight_decay]) * n
+    if len(decay) != n:
+        raise ValueError("adamw: weight_decay is a number or one per parameter")
+    lr_dev = step_dev = factor = None
+    if isinstance(lr, torch.Tensor):
+        lr, lr_dev = 0.0, _scalar("lr", lr, dev, torch.float32)
+    if isinstance(step, torch.Tensor):
+        step, step_dev = 1, _scalar("step", step, dev, torch.int64)
+    if grad_scale is not None:
+        factor = _scalar("grad_scale", grad_scale, dev, torch.float32)
+    call("spmdb200_adamw", n, _ptr(p), _ptr(p_types), _ptr(g), _ptr(g_types), _ptr(sizes), _ptr(m), _ptr(v), bits,
+         _ptr(m_scales), _ptr(v_scales), _ptr(c), _ptr(c_types), _ptr(decay), lr, lr_dev, betas[0], betas[1], eps, step,
+         step_dev, factor, _raw_stream(dev))
     return params
