@@ -282,12 +282,12 @@ constexpr int kStages8 = 2;
 template <class T, int N>
 __device__ __forceinline__ void fetch_chunks(uint4 (&slot)[N][32], const T *src, int lane) {
 #pragma unroll
-  for (int q = 0; q < N; ++q) copy_async16(&slot[q][lane], reinterpret_cast<const uint4 *>(src) + q);
+  for (int q = 0; q < N; ++q) copy_async<16>(&slot[q][lane], reinterpret_cast<const uint4 *>(src) + q);
 }
 template <class T, int N>
 __device__ __forceinline__ void take_chunks(const uint4 (&slot)[N][32], int lane, float v[8]) {
   if constexpr (N == 1) {
-    load8(reinterpret_cast<const T *>(&slot[0][lane]), v);
+    unpack8<T>(slot[0][lane], v);
   } else {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ A
       if (ahead < whole) {
         Stage8<P, G> &s = stages[ahead % kStages8];
         fetch_chunks(s.g, fg, lane);
-        copy_async16(&s.codes[lane], fc);
+        copy_async<16>(&s.codes[lane], fc);
         fetch_chunks(s.p, fp, lane);
         fp += kStateBlock, fg += kStateBlock, fc += kStateBlock;
         ++ahead;

@@ -112,15 +112,43 @@ __device__ __forceinline__ void store8(T *p, const float v[8]) {
                                              pack(v[6], v[7], T{}));
 }
 template <class T>
-__device__ __forceinline__ void load8(const T *p, float v[8]) {  // any address space
-  const uint4 q = *reinterpret_cast<const uint4 *>(p);
+__device__ __forceinline__ void unpack8(uint4 q, float v[8]) {
   const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{}), c = unpack(q.z, T{}), d = unpack(q.w, T{});
   v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
 }
+template <class T>
+__device__ __forceinline__ void load8(const T *p, float v[8]) {
+  unpack8<T>(ld_u4(p), v);
+}
+// W elements of a global tensor.
+template <int W, class T>
+__device__ __forceinline__ void load_vec(const T *p, float *v) {
+  if constexpr (W == 8) load8(p, v);
+  else load4(p, v);
+}
+// W elements that a thread has put into shared memory itself.
+template <int W, class T>
+__device__ __forceinline__ void take_vec(const unsigned char *slot, float *v) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4 *>(slot);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else if constexpr (W == 8) {
+    unpack8<T>(*reinterpret_cast<const uint4 *>(slot), v);
+  } else {
+    const uint2 q = *reinterpret_cast<const uint2 *>(slot);
+    const float2 a = unpack(q.x, T{}), b = unpack(q.y, T{});
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+  }
+}
 
-// ---- asynchronous 16-byte copies to shared memory --------------------------------------
-__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// ---- asynchronous copies to shared memory -----------------------------------------------
+// 32 lanes that copy one address each cost 32 turns: one lane does it for all.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *dst, const void *src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -153,6 +181,22 @@ template <int W, class T>
 __device__ __forceinline__ void store_vec(T *p, const float *v) {
   if constexpr (W == 8) store8(p, v);
   else store4(p, v);
+}
+// Of a tensor whose type is known at run time, kept in the caches (weights).
+template <int W>
+__device__ __forceinline__ void load_kept(const void *p, int type, int64_t i, float *v) {
+#pragma unroll
+  for (int e = 0; e < W; e += 4) {
+    if (type == kF32) {
+      const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + e);
+      v[e] = f.x, v[e + 1] = f.y, v[e + 2] = f.z, v[e + 3] = f.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i + e);
+      const float2 a = type == kF16 ? unpack(q.x, __half{}) : unpack(q.x, __nv_bfloat16{});
+      const float2 b = type == kF16 ? unpack(q.y, __half{}) : unpack(q.y, __nv_bfloat16{});
+      v[e] = a.x, v[e + 1] = a.y, v[e + 2] = b.x, v[e + 3] = b.y;
+    }
+  }
 }
 // Into a 16-bit tensor whose type is known at run time.
 template <int W>

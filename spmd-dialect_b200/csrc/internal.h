@@ -170,7 +170,7 @@ struct StencilNdProblem {
 };
 cudaError_t launch_stencil_nd(const StencilNdProblem &p, int promote, cudaStream_t s);
 
-// ---- layer norm (layer_norm.cu) -----------------------------------------------------
+// ---- layer norm (layer_norm.cu, layer_norm_backward.cu) -----------------------------------------------------
 // One struct for both directions: y is the output going forward and dy going
 // back; mean and rstd are written going forward (where not null) and read
 // going back.  rows, cols as checked by the entry (cols >= 1).

@@ -1,0 +1,303 @@
+// layer_norm_backward.cu -- gradients of the layer norm.
+//
+// With xh = (x - mean) rstd, a = dy w, c1 = sum a / N, c2 = sum a xh / N
+//   dx = rstd (a - c1 - xh c2),  dw = sum over rows of dy xh,  db = sum over rows of dy.
+// Sums are held in f32; dx, dw and db are rounded once to their type.  Bound by
+// memory: x and dy are read once, dx is written.  The sums over rows have a
+// fixed order: a block adds up its rows in registers and writes one partial
+// row, a second kernel adds up the partial rows.
+#include "layer_norm.cuh"
+
+namespace spmdb200 {
+
+namespace {
+
+constexpr int kMost = 16;        // elements of a row in a thread: two sums are held for each too
+constexpr int kWideLanes = 512;  // threads of a block for rows past kThreads * kMost columns
+constexpr int kMaxParts = 444;   // three blocks per SM
+constexpr int kColWidth = 32, kColDepth = 32;
+constexpr int64_t kHeld = (int64_t)kWideLanes * kMost;  // columns that a block holds
+
+// What the kernels are given.
+template <class TX, class TY>
+struct Back {
+  const TY *dy;
+  Rows gr;
+  const TX *x;
+  Rows xr;
+  const float *mean, *rstd;
+  const void *w;
+  int wtype;
+  TX *dx;  // may be null
+  Rows dr;
+  float *part;  // column sums, or null
+  int64_t rows, cols;
+};
+
+// Rows that a block's lanes hold: a block goes through rows with stride and
+// keeps the column sums of its rows in registers; at the end its groups of lanes
+// are added up in order.
+template <class TX, class TY, int W, int NV, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back<TX, TY> p, int lanes) {
+  extern __shared__ float sums[];  // [rows of partial sums][lanes * NV * W]
+  __shared__ float sh[2][2][32];
+  const int lane = threadIdx.x & (lanes - 1), groups = blockDim.x / lanes, group = threadIdx.x / lanes;
+  const int cols = (int)p.cols;
+  const float inv_n = 1.0f / (float)cols;
+  float w[NV][W], sw[NV][W], sb[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, VEC>(p.w, p.wtype, 0, cols, k, lane, lanes, 1.0f, w[k]);
+#pragma unroll
+    for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t r = (int64_t)blockIdx.x * groups; r < p.rows; r += (int64_t)gridDim.x * groups, turn ^= 1) {
+    const int64_t i = r + group;
+    const int n = i < p.rows ? cols : 0;
+    const float mean = n ? p.mean[i] : 0.0f, rstd = n ? p.rstd[i] : 0.0f;
+    float g[NV][W], x[NV][W];
+    load_row<W, NV, VEC>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
+    load_row<W, NV, VEC>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float xh = (x[k][e] - mean) * rstd, a = g[k][e] * w[k][e];
+        sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
+        sb[k][e] += g[k][e];
+        s1 += a;
+        s2 = fmaf(a, xh, s2);
+        g[k][e] = a;
+        x[k][e] = xh;
+      }
+    if (!p.dx) continue;
+    const float c1 = row_sum(s1, lanes, sh[turn][0]) * inv_n, c2 = row_sum(s2, lanes, sh[turn][1]) * inv_n;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
+    if (n) store_row<W, NV, VEC>(p.dx + row_offset(p.dr, i), p.dr.sc, n, lane, lanes, g);
+  }
+  if (!p.part) return;
+  // Groups of one warp first, by shuffles, then the block's over shared memory.
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      for (int o = lanes; o < 32; o <<= 1) {
+        sw[k][e] += __shfl_xor_sync(0xffffffffu, sw[k][e], o);
+        sb[k][e] += __shfl_xor_sync(0xffffffffu, sb[k][e], o);
+      }
+  const int wide = lanes * NV * W, stack = lanes < 32 ? blockDim.x >> 5 : groups;
+  const int at = lanes < 32 ? threadIdx.x >> 5 : group;
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+    if ((threadIdx.x & 31) < lanes || lanes >= 32) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          sums[at * wide + column<W, VEC>(k, e, lane, lanes)] = which ? sb[k][e] : sw[k][e];
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < wide && j < cols; j += blockDim.x) {
+      float s = 0.0f;
+      for (int q = 0; q < stack; ++q) s += sums[q * wide + j];
+      p.part[(2 * (int64_t)blockIdx.x + which) * cols + j] = s;
+    }
+  }
+}
+
+// Longer rows, first pass: the two sums of each run of kRun columns of a row.
+constexpr int kRun = kThreads * kMost;
+
+template <class TX, class TY, int W, bool VEC>
+__global__ void __launch_bounds__(kThreads) ln_row_sums(const __grid_constant__ Back<TX, TY> p, float2 *run_sums, int64_t runs) {
+  constexpr int NV = kMost / W;
+  __shared__ float sh[2][2][32];
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < p.rows * runs; item += gridDim.x, turn ^= 1) {
+    const int64_t i = item / runs, first = (item - i * runs) * kRun;
+    const int n = p.cols - first < kRun ? (int)(p.cols - first) : kRun;
+    const float mean = p.mean[i], rstd = p.rstd[i];
+    float g[NV][W], x[NV][W];
+    load_row<W, NV, VEC>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
+    load_row<W, NV, VEC>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float w[W];
+      load_weight<W, VEC>(p.w, p.wtype, first, n, k, threadIdx.x, kThreads, 1.0f, w);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float a = g[k][e] * w[e];
+        s1 += a;
+        s2 = fmaf(a, (x[k][e] - mean) * rstd, s2);
+      }
+    }
+    s1 = row_sum(s1, kThreads, sh[turn][0]);
+    s2 = row_sum(s2, kThreads, sh[turn][1]);
+    if (threadIdx.x == 0) run_sums[item] = make_float2(s1, s2);
+  }
+}
+
+// Second pass: block (run, part) takes kRun columns of the part's rows, writes
+// dx and keeps the column sums.  x and dy come from L2 where they fit there.
+template <class TX, class TY, int W, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+ln_row_grads(const __grid_constant__ Back<TX, TY> p, const float2 *run_sums, int64_t runs, int parts) {
+  constexpr int NV = kMost / W;
+  const int64_t run = blockIdx.x % runs, part = blockIdx.x / runs, first = run * kRun;
+  const int n = p.cols - first < kRun ? (int)(p.cols - first) : kRun;
+  const float inv_n = 1.0f / (float)p.cols;
+  float w[NV][W], sw[NV][W], sb[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, VEC>(p.w, p.wtype, first, n, k, threadIdx.x, kThreads, 1.0f, w[k]);
+#pragma unroll
+    for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
+  }
+  for (int64_t i = part; i < p.rows; i += parts) {
+    const float mean = p.mean[i], rstd = p.rstd[i];
+    float g[NV][W], x[NV][W];
+    load_row<W, NV, VEC>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
+    load_row<W, NV, VEC>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
+    float c1 = 0.0f, c2 = 0.0f;
+    if (p.dx) {  // every warp adds up the row's runs for itself, in one order
+      for (int64_t q = threadIdx.x & 31; q < runs; q += 32) {
+        const float2 s = run_sums[i * runs + q];
+        c1 += s.x;
+        c2 += s.y;
+      }
+      c1 = warp_sum_f32(c1) * inv_n;
+      c2 = warp_sum_f32(c2) * inv_n;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float xh = (x[k][e] - mean) * rstd;
+        sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
+        sb[k][e] += g[k][e];
+        g[k][e] = (g[k][e] * w[k][e] - c1 - xh * c2) * rstd;
+      }
+    if (p.dx) store_row<W, NV, VEC>(p.dx + row_offset(p.dr, i) + first * p.dr.sc, p.dr.sc, n, threadIdx.x, kThreads, g);
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int c = column<W, VEC>(k, e, threadIdx.x, kThreads);
+      if (c < n) {
+        p.part[2 * part * p.cols + first + c] = sw[k][e];
+        p.part[(2 * part + 1) * p.cols + first + c] = sb[k][e];
+      }
+    }
+}
+
+// dw and db from the partial rows (part p: dw at row 2p, db at row 2p + 1).
+__global__ void __launch_bounds__(kColWidth *kColDepth)
+ln_finish(const float *__restrict__ part, int parts, int64_t cols, void *dw, void *db, int type) {
+  __shared__ float sh[2][kColDepth][kColWidth];
+  const int tx = threadIdx.x & (kColWidth - 1), ty = threadIdx.x / kColWidth;
+  const int64_t j = (int64_t)blockIdx.x * kColWidth + tx;
+  float sw = 0.0f, sb = 0.0f;
+  if (j < cols)
+#pragma unroll 4
+    for (int p = ty; p < parts; p += kColDepth) {
+      sw += part[(2 * (int64_t)p) * cols + j];
+      sb += part[(2 * (int64_t)p + 1) * cols + j];
+    }
+  sh[0][ty][tx] = sw;
+  sh[1][ty][tx] = sb;
+  __syncthreads();
+  if (ty < 2 && j < cols) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kColDepth; ++k) s += sh[ty][k][tx];
+    void *out = ty == 0 ? dw : db;
+    if (out) store_from_f32(out, type, j, s);
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------
+// Partial rows of the column sums for rows that a block holds, and for longer
+// ones: there, few parts of few rows each, so that blocks fill the GPU.
+int held_parts(int64_t rows, int groups) {
+  const int64_t p = (rows + groups - 1) / groups;
+  return (int)(p < 1 ? 1 : p < kMaxParts ? p : kMaxParts);
+}
+int64_t long_runs(int64_t cols) { return (cols + kRun - 1) / kRun; }
+int long_parts(int64_t rows, int64_t cols) {
+  const int64_t most = (4 * kMaxParts + long_runs(cols) - 1) / long_runs(cols);
+  const int64_t p = rows < most ? rows : most;
+  return (int)(p < 1 ? 1 : p);
+}
+size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+template <class TX, class TY, int NV, bool VEC, int MAXT>
+cudaError_t backward_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>;
+  const int threads = lanes < kThreads ? kThreads : lanes, groups = threads / lanes;
+  *parts = held_parts(b.rows, groups);
+  const size_t bytes = b.part ? (size_t)(lanes < 32 ? threads / 32 : groups) * lanes * NV * W * sizeof(float) : 0;
+  ln_backward<TX, TY, W, NV, VEC, MAXT><<<*parts, threads, bytes, s>>>(b, lanes);
+  return cudaGetLastError();
+}
+
+template <class TX, class TY, bool VEC>
+cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>;
+  if (b.cols > kHeld) {
+    const int64_t runs = long_runs(b.cols);
+    *parts = long_parts(b.rows, b.cols);
+    float2 *run_sums = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)*parts * 2 * b.cols * sizeof(float)));
+    if (b.dx) {
+      ln_row_sums<TX, TY, W, VEC><<<grid_for(b.rows * runs), kThreads, 0, s>>>(b, run_sums, runs);
+      if (cudaError_t e = cudaGetLastError()) return e;
+    }
+    ln_row_grads<TX, TY, W, VEC><<<grid_for(runs * *parts), kThreads, 0, s>>>(b, run_sums, runs, *parts);
+    return cudaGetLastError();
+  }
+  if (b.cols > kThreads * kMost) return backward_rows<TX, TY, kMost / W, VEC, kWideLanes>(b, kWideLanes, parts, s);
+  const int lanes = row_lanes(b.rows, b.cols, W, kMost);
+  switch (row_vectors(b.cols, lanes, W)) {
+    case 1: return backward_rows<TX, TY, 1, VEC, kThreads>(b, lanes, parts, s);
+    case 2: return backward_rows<TX, TY, 2, VEC, kThreads>(b, lanes, parts, s);
+    default: return backward_rows<TX, TY, kMost / W, VEC, kThreads>(b, lanes, parts, s);
+  }
+}
+
+template <class TX, class TY>
+cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>;
+  const bool vec = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) && vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) &&
+                   vec_weight(p.w) && (!p.dx || vec_rows(p.dx, p.dr, p.rows, sizeof(TX), W));
+  const Back<TX, TY> b{static_cast<const TY *>(p.y), p.yr, static_cast<const TX *>(p.x), p.xr, p.mean, p.rstd, p.w, p.wtype,
+                       static_cast<TX *>(p.dx), p.dr, p.dw || p.db ? static_cast<float *>(p.ws) : nullptr, p.rows, p.cols};
+  int parts = 0;
+  if (p.rows > 0) {
+    if (cudaError_t e = vec ? backward_of<TX, TY, true>(b, p.ws, &parts, s) : backward_of<TX, TY, false>(b, p.ws, &parts, s)) return e;
+  }
+  if (!b.part) return cudaSuccess;
+  const int64_t tiles = (p.cols + kColWidth - 1) / kColWidth;
+  ln_finish<<<grid_for(tiles), kColWidth * kColDepth, 0, s>>>(b.part, parts, p.cols, p.dw, p.db, p.dwtype);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
+  if (cols <= kHeld) return (size_t)held_parts(rows, 1) * 2 * (size_t)cols * sizeof(float);
+  return round16((size_t)long_parts(rows, cols) * 2 * (size_t)cols * sizeof(float)) +
+         (size_t)rows * (size_t)long_runs(cols) * sizeof(float2);
+}
+
+cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s) {
+  return by_types(p.xtype, p.ytype, [&](auto tx, auto ty) { return backward<decltype(tx), decltype(ty)>(p, s); });
+}
+
+}  // namespace spmdb200
