@@ -150,6 +150,14 @@ __device__ __forceinline__ void copy_async(void *dst, const void *src) {
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
 }
+// The first `bytes` of a copy come from memory, the rest are zero.
+template <int BYTES>
+__device__ __forceinline__ void copy_async_part(void *dst, const void *src, int bytes) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void copy_wait() {

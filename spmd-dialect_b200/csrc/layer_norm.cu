@@ -4,8 +4,8 @@
 //   xh = (x - mean) rstd,  y = xh w + b
 // Sums are held in f32; x, w and b are widened exactly, y is rounded once to
 // its type.  A few operations an element: bound by memory.  A row's elements
-// stay in registers, so that the variance is taken around the mean from the
-// same read.
+// stay on the SM, so that the variance is taken around the mean from the same
+// read.
 #include <cooperative_groups.h>
 
 #include "layer_norm.cuh"
@@ -33,6 +33,104 @@ __device__ __forceinline__ float whole_sum(float v, int lanes, float *sh, float 
     v = warp_sum_f32(lane < (int)cluster.num_blocks() ? *cluster.map_shared_rank(mine, lane) : 0.0f);
   }
   return v;
+}
+
+// Streamed rows (layer_norm.cuh): weight and bias are loaded once a thread.  A
+// group of lanes takes R rows at a time: the two reductions of a row are a long
+// chain of waits, and a second row fills them.
+constexpr int kStages = 3;
+constexpr int kStreamMost = 16;  // elements of a row in a thread
+
+template <class TX, class TY, int W, int NV, int R, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
+ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
+                  const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int lanes) {
+  constexpr int kBytes = W * sizeof(TX), kPitch = MAXT * kBytes;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float sh[2][R][32];
+  const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
+  const float inv_n = 1.0f / (float)cols;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int64_t i = (int64_t)blockIdx.x * groups + group;
+  RowAt ahead = row_at(xr, i), at = row_at(yr, i);
+  int64_t next = i;  // the row to copy next
+  const int shift = i < rows ? (int)((uintptr_t)(x + ahead.offset) / sizeof(TX) % W) : 0;
+  unsigned char *const slots = smem + threadIdx.x * kBytes;
+  int stage_in = 0, stage = 0;
+  auto fetch = [&] {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (next < rows) stream_row<W, NV>(slots + (stage_in * R + q) * (NV * kPitch), kPitch, x + ahead.offset, cols, lane, lanes, shift);
+      next += step;
+      next_row(xr, ahead);
+    }
+    copy_commit();  // empty past the last row, so that the count of groups stays
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+  };
+#pragma unroll
+  for (int q = 0; q < kStages - 1; ++q) fetch();
+  float wv[NV][W], bv[NV][W];
+  stream_weight<W, NV>(w, wtype, cols, lane, lanes, shift, 1.0f, wv);
+  stream_weight<W, NV>(b, wtype, cols, lane, lanes, shift, 0.0f, bv);
+  for (int64_t block_row = i - group; block_row < rows; block_row += R * step) {
+    fetch();
+    copy_wait<kStages - 1>();
+    float v[R][NV][W], s[R], mean[R], rstd[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      s[q] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        take_vec<W, TX>(slots + ((stage * R + q) * NV + k) * kPitch, v[q][k]);
+        if (!whole<W>(k, cols, lane, lanes, shift)) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const int c = shifted<W>(k, e, lane, lanes, shift);
+            if (c < 0 || c >= cols) v[q][k][e] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) s[q] += v[q][k][e];
+      }
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    row_sums<R>(s, lanes, sh[0]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = s[q] * inv_n;
+      s[q] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const bool all = whole<W>(k, cols, lane, lanes, shift);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          v[q][k][e] -= mean[q];
+          const int c = shifted<W>(k, e, lane, lanes, shift);
+          if (all || (c >= 0 && c < cols)) s[q] = fmaf(v[q][k][e], v[q][k][e], s[q]);
+        }
+      }
+    }
+    row_sums<R>(s, lanes, sh[1]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      rstd[q] = 1.0f / sqrtf(s[q] * inv_n + eps);
+      if (i < rows) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) v[q][k][e] = fmaf(v[q][k][e] * rstd[q], wv[k][e], bv[k][e]);
+          stream_store<W>(y + at.offset, k, cols, lane, lanes, shift, v[q][k]);
+        }
+        if (lane == 0) {
+          if (mean_out) mean_out[i] = mean[q];
+          if (rstd_out) rstd_out[i] = rstd[q];
+        }
+      }
+      i += step;
+      next_row(yr, at);
+    }
+  }
+  copy_wait<0>();
 }
 
 template <class TX, class TY, int W, int NV, bool VEC, int MAXT, bool CLUSTER>
@@ -201,6 +299,33 @@ cudaError_t forward_rows(const LayerNormProblem &p, int lanes, int cluster, cuda
                             static_cast<TY *>(p.y), p.yr, p.w, p.b, p.wtype, p.rows, p.cols, p.eps, p.mean, p.rstd, lanes);
 }
 
+template <class TX, class TY, int NV, int R, int MAXT>
+cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int grid, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, bytes = kStages * R * NV * MAXT * W * (int)sizeof(TX);
+  auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  const int64_t step = (int64_t)grid * (MAXT / lanes);
+  kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, step), static_cast<TY *>(p.y),
+                                   row_walk(p.yr, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
+  return cudaGetLastError();
+}
+
+// Streamed rows: as many blocks as are resident, or one for each block of rows
+// where those are fewer (then one row at a time).
+template <class TX, class TY>
+cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, NV = kStreamMost / W;
+  if (p.cols + spare > kThreads * kStreamMost)
+    return stream_rows<TX, TY, NV, 1, 2 * kThreads>(p, 2 * kThreads, stream_grid(p.rows, 1, device_sms(), W), s);
+  const int lanes = row_lanes(p.rows, p.cols, W, kStreamMost, spare), groups = kThreads / lanes;
+  const int nv = row_vectors(p.cols + spare, lanes, W), most = (nv * W > 8 ? 2 : 3) * device_sms();
+  const int grid = stream_grid(p.rows, groups, most, W);
+  if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads>(p, lanes, grid, s);
+  if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads>(p, lanes, grid, s);
+  if (p.rows <= (int64_t)most * groups) return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, grid, s);
+  return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, grid, s);
+}
+
 template <class TX, class TY, bool VEC>
 cudaError_t forward_of(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>;
@@ -215,18 +340,25 @@ cudaError_t forward_of(const LayerNormProblem &p, cudaStream_t s) {
     return forward_rows<TX, TY, kWideMost / W, VEC, kWideLanes, true>(p, kWideLanes, cluster, s);
   }
   if (p.cols > kHeld) return forward_rows<TX, TY, kWideMost / W, VEC, kWideLanes, false>(p, kWideLanes, 1, s);
-  const int lanes = row_lanes(p.rows, p.cols, W, kMost);
+  if constexpr (VEC) {  // what is left of shorter rows: weights at odd addresses
+    return forward_rows<TX, TY, kMost / W, true, kThreads, false>(p, kThreads, 1, s);
+  }
+  const int lanes = row_lanes(p.rows, p.cols, W, kMost, 0);
   switch (row_vectors(p.cols, lanes, W)) {
-    case 1: return forward_rows<TX, TY, 1, VEC, kThreads, false>(p, lanes, 1, s);
-    case 2: return forward_rows<TX, TY, 2, VEC, kThreads, false>(p, lanes, 1, s);
-    case 4: return forward_rows<TX, TY, 4, VEC, kThreads, false>(p, lanes, 1, s);
-    default: return forward_rows<TX, TY, kMost / W, VEC, kThreads, false>(p, lanes, 1, s);
+    case 1: return forward_rows<TX, TY, 1, false, kThreads, false>(p, lanes, 1, s);
+    case 2: return forward_rows<TX, TY, 2, false, kThreads, false>(p, lanes, 1, s);
+    case 4: return forward_rows<TX, TY, 4, false, kThreads, false>(p, lanes, 1, s);
+    default: return forward_rows<TX, TY, kMost / W, false, kThreads, false>(p, lanes, 1, s);
   }
 }
 
 template <class TX, class TY>
 cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>;
+  const int spare = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) ? 0 : W - 1;
+  if (p.cols + spare <= 2 * kThreads * kStreamMost && p.xr.sc == 1 && p.yr.sc == 1 &&
+      same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
+    return forward_streamed<TX, TY>(p, spare, s);
   const bool vec = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) && vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) &&
                    vec_weight(p.w) && vec_weight(p.b);
   return vec ? forward_of<TX, TY, true>(p, s) : forward_of<TX, TY, false>(p, s);

@@ -1,10 +1,18 @@
 // layer_norm.cuh -- what the two directions of the layer norm share.
 //
 // A row is taken by `lanes` threads (a power of two), each with NV vectors of W
-// elements.  W is what 16 bytes of the wider type hold.  VEC: rows at vector
-// alignment, thread t's vectors t, t + lanes, ...; otherwise (any strides and
-// addresses) single elements t, t + lanes, ...  Columns are 32-bit numbers: a
-// block holds at most a few thousand, longer rows are cut into runs.
+// elements; W is what 16 bytes of the wider type hold.  Three layouts:
+// - Streamed rows (up to a few thousand columns, last dimension contiguous): a
+//   block goes through rows with stride, the next rows on their way to shared
+//   memory while one is computed.  Thread t copies and reads the aligned vectors
+//   t, t + lanes, ... that cover the row.  A row may start `shift` elements into
+//   its first vector (odd lengths, odd addresses): the stride of rows is a
+//   multiple of W, so that a thread's rows all have one shift, and its columns,
+//   with their weights and sums in registers, are the same in all of them.
+// - VEC: rows at vector alignment, thread t's vectors t, t + lanes, ...
+// - Any strides and addresses: single elements t, t + lanes, ...
+// Columns are 32-bit numbers: a block holds at most a few thousand, longer rows
+// are cut into runs.
 #pragma once
 
 #include "dtypes.cuh"
@@ -32,6 +40,26 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *sh) {
   if (lane == 0) sh[warp] = v;
   __syncthreads();
   return warp_sum_f32(lane < warps ? sh[(warp & ~(warps - 1)) + lane] : 0.0f);
+}
+
+// R sums at once; `sh` holds 32 floats for each.
+template <int R>
+__device__ __forceinline__ void row_sums(float (&v)[R], int lanes, float (*sh)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = lanes >> 5;
+  for (int o = lanes < 32 ? lanes >> 1 : 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+  if (lanes <= 32) return;
+  if (lane == 0)
+#pragma unroll
+    for (int q = 0; q < R; ++q) sh[q][warp] = v[q];
+  __syncthreads();
+  const int first = warp & ~(warps - 1);
+#pragma unroll
+  for (int q = 0; q < R; ++q) v[q] = sh[q][first + (lane & (warps - 1))];
+  for (int o = warps >> 1; o > 0; o >>= 1)
+#pragma unroll
+    for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
 }
 
 // Which column element e of a thread's vector k is.
@@ -89,6 +117,96 @@ __device__ __forceinline__ void load_weight(const void *p, int type, int64_t fir
   }
 }
 
+// ---- streamed rows ------------------------------------------------------------------
+// A view's row offset as a block goes through rows: `step` rows on, i1 (the row
+// within n1) and the offset grow by constants, with a correction past n1.
+struct RowWalk {
+  int64_t n1, s0, s1;
+  int64_t i1_step, step, wrap;
+};
+inline RowWalk row_walk(const Rows &r, int64_t step) {
+  const int64_t a = step / r.n1, b = step - a * r.n1;
+  return {r.n1, r.s0, r.s1, b, a * r.s0 + b * r.s1, r.s0 - r.n1 * r.s1};
+}
+struct RowAt {
+  int64_t i1, offset;
+};
+__device__ __forceinline__ RowAt row_at(const RowWalk &w, int64_t i) {
+  const int64_t a = i < w.n1 ? 0 : i / w.n1, b = i - a * w.n1;
+  return {b, a * w.s0 + b * w.s1};
+}
+__device__ __forceinline__ void next_row(const RowWalk &w, RowAt &r) {
+  r.i1 += w.i1_step;
+  r.offset += w.step;
+  if (r.i1 >= w.n1) {
+    r.i1 -= w.n1;
+    r.offset += w.wrap;
+  }
+}
+
+// Column of element e of vector k of a thread whose rows have `shift`.
+template <int W>
+__device__ __forceinline__ int shifted(int k, int e, int lane, int lanes, int shift) {
+  return (k * lanes + lane) * W + e - shift;
+}
+// Starts the copies of a row's vectors into a thread's slots, `pitch` bytes apart.
+// Of a vector that holds the row's end only the row's elements are read; one
+// that holds its start is read from the vector's start (in the same aligned 16
+// bytes, so in the same allocation).
+template <int W, int NV, class T>
+__device__ __forceinline__ void stream_row(unsigned char *slot, int pitch, const T *row, int cols, int lane, int lanes, int shift) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = shifted<W>(k, 0, lane, lanes, shift), left = cols - c;
+    if (left >= W) copy_async<W * sizeof(T)>(slot + k * pitch, row + c);
+    else if (left > 0) copy_async_part<W * sizeof(T)>(slot + k * pitch, row + c, left * (int)sizeof(T));
+  }
+}
+// Whether all of vector k's elements are in the row.
+template <int W>
+__device__ __forceinline__ bool whole(int k, int cols, int lane, int lanes, int shift) {
+  const int c = shifted<W>(k, 0, lane, lanes, shift);
+  return c >= 0 && c + W <= cols;
+}
+// Weight or bias of a thread's columns; `rest` without one and past the row's ends.
+template <int W, int NV>
+__device__ __forceinline__ void stream_weight(const void *p, int type, int cols, int lane, int lanes, int shift, float rest,
+                                              float (&v)[NV][W]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (p && shift == 0 && (uintptr_t)p % 16 == 0 && whole<W>(k, cols, lane, lanes, 0)) {
+      load_kept<W>(p, type, shifted<W>(k, 0, lane, lanes, 0), v[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int c = shifted<W>(k, e, lane, lanes, shift);
+        v[k][e] = p && c >= 0 && c < cols ? load_as_f32(p, type, c) : rest;
+      }
+    }
+  }
+}
+template <int W, class T>
+__device__ __forceinline__ void stream_store(T *row, int k, int cols, int lane, int lanes, int shift, const float (&v)[W]) {
+  const int c = shifted<W>(k, 0, lane, lanes, shift);
+  if (c >= 0 && c + W <= cols) {
+    store_vec<W>(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (c + e >= 0 && c + e < cols) row[c + e] = from_f32<T>(v[e]);
+  }
+}
+
+// Rows of views that start equally far into a vector, all of them or a period
+// of w rows: where an element lies modulo w.
+inline bool same_shift(const void *p, const Rows &r, int p_size, const void *q, const Rows &t, int q_size, int64_t rows, int w) {
+  const uint64_t uw = (uint64_t)w;
+  return ((uintptr_t)p / p_size - (uintptr_t)q / q_size) % uw == 0 &&
+         (rows < 2 || ((uint64_t)(r.s1 - t.s1) % uw == 0 && (rows <= r.n1 && rows <= t.n1)) ||
+          ((uint64_t)r.s1 % uw == 0 && (uint64_t)t.s1 % uw == 0 && (rows <= r.n1 || (uint64_t)r.s0 % uw == 0) &&
+           (rows <= t.n1 || (uint64_t)t.s0 % uw == 0)));
+}
+
 inline int device_sms() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess ? num_sms(dev) : 148;
@@ -103,11 +221,13 @@ inline bool vec_rows(const void *p, const Rows &r, int64_t rows, int size, int w
 }
 inline bool vec_weight(const void *p) { return (uintptr_t)p % 16 == 0; }
 
-// Lanes of a row: as few as hold it at `most` elements each, which leaves a
-// thread several loads in flight; more, down to one vector each, where that
-// leaves the GPU unfilled (a few rows: latency counts).
-inline int row_lanes(int64_t rows, int64_t cols, int w, int most) {
+// Lanes of a row: as few as hold it at `most` elements each (`spare` of them
+// for a start within a vector), which leaves a thread several loads in flight;
+// more, down to one vector each, where that leaves the GPU unfilled (a few rows:
+// latency counts).
+inline int row_lanes(int64_t rows, int64_t cols, int w, int most, int spare) {
   int lanes = 1;
+  cols += spare;
   while (lanes < kThreads && (int64_t)lanes * most < cols) lanes *= 2;
   const int64_t fill = (int64_t)device_sms() * 1024;
   while (lanes < kThreads && (int64_t)lanes * w < cols && rows * lanes < fill) lanes *= 2;
@@ -117,6 +237,15 @@ inline int row_vectors(int64_t cols, int lanes, int w) {
   int nv = 1;
   while ((int64_t)lanes * nv * w < cols) nv *= 2;
   return nv;
+}
+
+// Blocks of streamed rows: a row each, at most `most`, and where they come
+// around again a stride of rows that is a multiple of w.
+inline int stream_grid(int64_t rows, int64_t groups, int most, int w) {
+  const int64_t blocks = (rows + groups - 1) / groups;
+  if (blocks <= most) return (int)blocks;
+  while (most * groups % w != 0) --most;
+  return most;
 }
 
 // The type pairs (x, y): equal, or one of the two f32.

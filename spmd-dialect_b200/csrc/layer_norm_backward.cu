@@ -34,12 +34,38 @@ struct Back {
   int64_t rows, cols;
 };
 
-// Rows that a block's lanes hold: a block goes through rows with stride and
-// keeps the column sums of its rows in registers; at the end its groups of lanes
-// are added up in order.
-template <class TX, class TY, int W, int NV, bool VEC, int MAXT>
+// At the end of a block: its groups' column sums, added up in order, into partial
+// row blockIdx.x.  col(k, e) is a thread's column (groups may differ in theirs,
+// by their shifts); `sums` holds a row for each group.
+template <int W, int NV, class Column>
+__device__ __forceinline__ void reduce_columns(const float (&sw)[NV][W], const float (&sb)[NV][W], int lanes, int cols,
+                                               float *sums, float *part, Column col) {
+  const int groups = blockDim.x / lanes;
+  float *mine = sums + (int)(threadIdx.x / lanes) * cols;
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int c = col(k, e);
+        if (c >= 0 && c < cols) mine[c] = which ? sb[k][e] : sw[k][e];
+      }
+    __syncthreads();
+    for (int j = threadIdx.x; j < cols; j += blockDim.x) {
+      float s = 0.0f;
+#pragma unroll 8
+      for (int q = 0; q < groups; ++q) s += sums[q * cols + j];
+      part[(2 * (int64_t)blockIdx.x + which) * cols + j] = s;
+    }
+  }
+}
+
+// Rows that a block's lanes hold, any strides: a block goes through rows with
+// stride and keeps the column sums of its rows in registers.
+template <class TX, class TY, int W, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back<TX, TY> p, int lanes) {
-  extern __shared__ float sums[];  // [rows of partial sums][lanes * NV * W]
+  extern __shared__ __align__(16) float sums[];
   __shared__ float sh[2][2][32];
   const int lane = threadIdx.x & (lanes - 1), groups = blockDim.x / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols;
@@ -47,7 +73,7 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
   float w[NV][W], sw[NV][W], sb[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    load_weight<W, VEC>(p.w, p.wtype, 0, cols, k, lane, lanes, 1.0f, w[k]);
+    load_weight<W, false>(p.w, p.wtype, 0, cols, k, lane, lanes, 1.0f, w[k]);
 #pragma unroll
     for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
   }
@@ -57,9 +83,9 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     const int n = i < p.rows ? cols : 0;
     const float mean = n ? p.mean[i] : 0.0f, rstd = n ? p.rstd[i] : 0.0f;
     float g[NV][W], x[NV][W];
-    load_row<W, NV, VEC>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
-    load_row<W, NV, VEC>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
-    float s1 = 0.0f, s2 = 0.0f;
+    load_row<W, NV, false>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
+    load_row<W, NV, false>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
+    float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -67,47 +93,122 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
         const float xh = (x[k][e] - mean) * rstd, a = g[k][e] * w[k][e];
         sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
         sb[k][e] += g[k][e];
-        s1 += a;
-        s2 = fmaf(a, xh, s2);
+        s[0] += a;
+        s[1] = fmaf(a, xh, s[1]);
         g[k][e] = a;
         x[k][e] = xh;
       }
     if (!p.dx) continue;
-    const float c1 = row_sum(s1, lanes, sh[turn][0]) * inv_n, c2 = row_sum(s2, lanes, sh[turn][1]) * inv_n;
+    row_sums<2>(s, lanes, sh[turn]);
+    const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
-    if (n) store_row<W, NV, VEC>(p.dx + row_offset(p.dr, i), p.dr.sc, n, lane, lanes, g);
+    if (n) store_row<W, NV, false>(p.dx + row_offset(p.dr, i), p.dr.sc, n, lane, lanes, g);
   }
-  if (!p.part) return;
-  // Groups of one warp first, by shuffles, then the block's over shared memory.
+  if (p.part)
+    reduce_columns<W, NV>(sw, sb, lanes, cols, sums, p.part, [&](int k, int e) { return column<W, false>(k, e, lane, lanes); });
+}
+
+// Streamed rows (layer_norm.cuh): x and dy of the next rows are on their way
+// while one is computed, its mean and rstd with them.
+constexpr int kStages = 3;
+
+template <class TX, class TY, int W, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3)
+ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
+                   const __grid_constant__ RowWalk dr, int lanes) {
+  constexpr int kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * MAXT * (kXBytes + kGBytes);
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float sh[2][2][32];
+  __shared__ float2 stats[kStages][MAXT];  // a group's row, or a warp's where the group is wider
+  const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
+  const int cols = (int)p.cols, mine = lanes <= 32 ? group : threadIdx.x >> 5;
+  const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
+  const float inv_n = 1.0f / (float)cols;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  int64_t i = (int64_t)blockIdx.x * groups + group;
+  RowAt x_ahead = row_at(xr, i), g_ahead = row_at(gr, i), at = row_at(dr, i);
+  int64_t next = i;
+  const int shift = i < p.rows ? (int)((uintptr_t)(p.x + x_ahead.offset) / sizeof(TX) % W) : 0;
+  unsigned char *const x_slots = smem + threadIdx.x * kXBytes, *const g_slots = smem + NV * MAXT * kXBytes + threadIdx.x * kGBytes;
+  int stage_in = 0, stage = 0;
+  auto fetch = [&] {
+    if (next < p.rows) {
+      stream_row<W, NV>(x_slots + stage_in * kStage, MAXT * kXBytes, p.x + x_ahead.offset, cols, lane, lanes, shift);
+      stream_row<W, NV>(g_slots + stage_in * kStage, MAXT * kGBytes, p.dy + g_ahead.offset, cols, lane, lanes, shift);
+      if (first) {
+        copy_async<4>(&stats[stage_in][mine].x, p.mean + next);
+        copy_async<4>(&stats[stage_in][mine].y, p.rstd + next);
+      }
+    }
+    copy_commit();  // empty past the last row, so that the count of groups stays
+    next += step;
+    next_row(xr, x_ahead);
+    next_row(gr, g_ahead);
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+  };
+#pragma unroll
+  for (int q = 0; q < kStages - 1; ++q) fetch();
+  float w[NV][W], sw[NV][W], sb[NV][W];
+  stream_weight<W, NV>(p.w, p.wtype, cols, lane, lanes, shift, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int e = 0; e < W; ++e)
-      for (int o = lanes; o < 32; o <<= 1) {
-        sw[k][e] += __shfl_xor_sync(0xffffffffu, sw[k][e], o);
-        sb[k][e] += __shfl_xor_sync(0xffffffffu, sb[k][e], o);
+    for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
+  int turn = 0;
+  for (int64_t block_row = i - group; block_row < p.rows; block_row += step, i += step, turn ^= 1) {
+    fetch();
+    copy_wait<kStages - 1>();
+    __syncwarp();  // the first lane's copies are there too
+    const bool live = i < p.rows;
+    const float2 stat = stats[stage][mine];
+    float g[NV][W], x[NV][W], s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      take_vec<W, TX>(x_slots + stage * kStage + k * (MAXT * kXBytes), x[k]);
+      take_vec<W, TY>(g_slots + stage * kStage + k * (MAXT * kGBytes), g[k]);
+      if (!live || !whole<W>(k, cols, lane, lanes, shift)) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const int c = shifted<W>(k, e, lane, lanes, shift);
+          if (!live || c < 0 || c >= cols) g[k][e] = x[k][e] = 0.0f;
+        }
       }
-  const int wide = lanes * NV * W, stack = lanes < 32 ? blockDim.x >> 5 : groups;
-  const int at = lanes < 32 ? threadIdx.x >> 5 : group;
-  for (int which = 0; which < 2; ++which) {
-    __syncthreads();
-    if ((threadIdx.x & 31) < lanes || lanes >= 32) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          sums[at * wide + column<W, VEC>(k, e, lane, lanes)] = which ? sb[k][e] : sw[k][e];
     }
-    __syncthreads();
-    for (int j = threadIdx.x; j < wide && j < cols; j += blockDim.x) {
-      float s = 0.0f;
-      for (int q = 0; q < stack; ++q) s += sums[q * wide + j];
-      p.part[(2 * (int64_t)blockIdx.x + which) * cols + j] = s;
+    const float mean = live ? stat.x : 0.0f, rstd = live ? stat.y : 0.0f;
+    __syncwarp();  // every lane has its statistics: the slot may be filled again
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {  // an element past the row's ends has g = 0: it adds nothing to any sum
+        const float xh = (x[k][e] - mean) * rstd, a = g[k][e] * w[k][e];
+        sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
+        sb[k][e] += g[k][e];
+        s[0] += a;
+        s[1] = fmaf(a, xh, s[1]);
+        g[k][e] = a;
+        x[k][e] = xh;
+      }
+    if (!p.dx) continue;
+    row_sums<2>(s, lanes, sh[turn]);
+    const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
+        stream_store<W>(p.dx + at.offset, k, cols, lane, lanes, shift, g[k]);
+      }
     }
+    next_row(dr, at);
   }
+  copy_wait<0>();
+  if (p.part)
+    reduce_columns<W, NV>(sw, sb, lanes, cols, reinterpret_cast<float *>(smem), p.part,
+                          [&](int k, int e) { return shifted<W>(k, e, lane, lanes, shift); });
 }
 
 // Longer rows, first pass: the two sums of each run of kRun columns of a row.
@@ -238,49 +339,72 @@ int long_parts(int64_t rows, int64_t cols) {
 }
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-template <class TX, class TY, int NV, bool VEC, int MAXT>
+template <class TX, class TY, int NV, int MAXT>
 cudaError_t backward_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
-  const int threads = lanes < kThreads ? kThreads : lanes, groups = threads / lanes;
-  *parts = held_parts(b.rows, groups);
-  const size_t bytes = b.part ? (size_t)(lanes < 32 ? threads / 32 : groups) * lanes * NV * W * sizeof(float) : 0;
-  ln_backward<TX, TY, W, NV, VEC, MAXT><<<*parts, threads, bytes, s>>>(b, lanes);
+  *parts = held_parts(b.rows, MAXT / lanes);
+  ln_backward<TX, TY, kWidth<TX, TY>, NV, MAXT><<<*parts, MAXT, b.part ? MAXT / lanes * b.cols * sizeof(float) : 0, s>>>(b, lanes);
+  return cudaGetLastError();
+}
+
+template <class TX, class TY, int NV, int MAXT>
+cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, staged = kStages * NV * MAXT * W * (int)(sizeof(TX) + sizeof(TY));
+  const int sums = b.part ? (int)(MAXT / lanes * b.cols * sizeof(float)) : 0, bytes = staged > sums ? staged : sums;
+  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  const int64_t groups = MAXT / lanes;
+  const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
+  *parts = stream_grid(b.rows, groups, most < kMaxParts ? most : kMaxParts, W);
+  const int64_t step = *parts * groups;
+  kernel<<<*parts, MAXT, bytes, s>>>(b, row_walk(b.gr, step), row_walk(b.xr, step), row_walk(b.dr, step), lanes);
   return cudaGetLastError();
 }
 
 template <class TX, class TY, bool VEC>
-cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
+cudaError_t backward_long(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>;
-  if (b.cols > kHeld) {
-    const int64_t runs = long_runs(b.cols);
-    *parts = long_parts(b.rows, b.cols);
-    float2 *run_sums = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)*parts * 2 * b.cols * sizeof(float)));
-    if (b.dx) {
-      ln_row_sums<TX, TY, W, VEC><<<grid_for(b.rows * runs), kThreads, 0, s>>>(b, run_sums, runs);
-      if (cudaError_t e = cudaGetLastError()) return e;
-    }
-    ln_row_grads<TX, TY, W, VEC><<<grid_for(runs * *parts), kThreads, 0, s>>>(b, run_sums, runs, *parts);
-    return cudaGetLastError();
+  const int64_t runs = long_runs(b.cols);
+  *parts = long_parts(b.rows, b.cols);
+  float2 *run_sums = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)*parts * 2 * b.cols * sizeof(float)));
+  if (b.dx) {
+    ln_row_sums<TX, TY, W, VEC><<<grid_for(b.rows * runs), kThreads, 0, s>>>(b, run_sums, runs);
+    if (cudaError_t e = cudaGetLastError()) return e;
   }
-  if (b.cols > kThreads * kMost) return backward_rows<TX, TY, kMost / W, VEC, kWideLanes>(b, kWideLanes, parts, s);
-  const int lanes = row_lanes(b.rows, b.cols, W, kMost);
-  switch (row_vectors(b.cols, lanes, W)) {
-    case 1: return backward_rows<TX, TY, 1, VEC, kThreads>(b, lanes, parts, s);
-    case 2: return backward_rows<TX, TY, 2, VEC, kThreads>(b, lanes, parts, s);
-    default: return backward_rows<TX, TY, kMost / W, VEC, kThreads>(b, lanes, parts, s);
+  ln_row_grads<TX, TY, W, VEC><<<grid_for(runs * *parts), kThreads, 0, s>>>(b, run_sums, runs, *parts);
+  return cudaGetLastError();
+}
+
+template <class TX, class TY>
+cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, NV = kMost / W;
+  const bool even = vec_rows(b.x, b.xr, b.rows, sizeof(TX), W) && vec_rows(b.dy, b.gr, b.rows, sizeof(TY), W) &&
+                    (!b.dx || vec_rows(b.dx, b.dr, b.rows, sizeof(TX), W));
+  const int spare = even ? 0 : W - 1;
+  if (b.cols > kHeld - spare)
+    return even && vec_weight(b.w) ? backward_long<TX, TY, true>(b, ws, parts, s) : backward_long<TX, TY, false>(b, ws, parts, s);
+  const bool wide = b.cols + spare > kThreads * kMost;
+  const int lanes = wide ? kWideLanes : row_lanes(b.rows, b.cols, W, kMost, spare), nv = row_vectors(b.cols + spare, lanes, W);
+  if (b.xr.sc == 1 && b.gr.sc == 1 && (!b.dx || b.dr.sc == 1) &&
+      same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
+      (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W))) {
+    if (wide) return stream_rows<TX, TY, NV, kWideLanes>(b, lanes, parts, s);
+    if (nv == 1) return stream_rows<TX, TY, 1, kThreads>(b, lanes, parts, s);
+    if (nv < NV) return stream_rows<TX, TY, 2, kThreads>(b, lanes, parts, s);
+    return stream_rows<TX, TY, NV, kThreads>(b, lanes, parts, s);
   }
+  if (wide) return backward_rows<TX, TY, NV, kWideLanes>(b, lanes, parts, s);
+  if (nv == 1) return backward_rows<TX, TY, 1, kThreads>(b, lanes, parts, s);
+  if (nv < NV) return backward_rows<TX, TY, 2, kThreads>(b, lanes, parts, s);
+  return backward_rows<TX, TY, NV, kThreads>(b, lanes, parts, s);
 }
 
 template <class TX, class TY>
 cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
-  const bool vec = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) && vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) &&
-                   vec_weight(p.w) && (!p.dx || vec_rows(p.dx, p.dr, p.rows, sizeof(TX), W));
   const Back<TX, TY> b{static_cast<const TY *>(p.y), p.yr, static_cast<const TX *>(p.x), p.xr, p.mean, p.rstd, p.w, p.wtype,
                        static_cast<TX *>(p.dx), p.dr, p.dw || p.db ? static_cast<float *>(p.ws) : nullptr, p.rows, p.cols};
   int parts = 0;
   if (p.rows > 0) {
-    if (cudaError_t e = vec ? backward_of<TX, TY, true>(b, p.ws, &parts, s) : backward_of<TX, TY, false>(b, p.ws, &parts, s)) return e;
+    if (cudaError_t e = backward_of<TX, TY>(b, p.ws, &parts, s)) return e;
   }
   if (!b.part) return cudaSuccess;
   const int64_t tiles = (p.cols + kColWidth - 1) / kColWidth;
@@ -291,9 +415,12 @@ cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
 }  // namespace
 
 size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
-  if (cols <= kHeld) return (size_t)held_parts(rows, 1) * 2 * (size_t)cols * sizeof(float);
-  return round16((size_t)long_parts(rows, cols) * 2 * (size_t)cols * sizeof(float)) +
-         (size_t)rows * (size_t)long_runs(cols) * sizeof(float2);
+  // Rows a few columns short of what a block holds may take either way, as their addresses have it.
+  const size_t held = cols <= kHeld ? (size_t)held_parts(rows, 1) * 2 * (size_t)cols * sizeof(float) : 0;
+  if (cols <= kHeld - 7) return held;
+  const size_t cut = round16((size_t)long_parts(rows, cols) * 2 * (size_t)cols * sizeof(float)) +
+                     (size_t)rows * (size_t)long_runs(cols) * sizeof(float2);
+  return held > cut ? held : cut;
 }
 
 cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s) {
