@@ -7,6 +7,8 @@ linked with the static CUDA runtime into libspmdb200.so (no link-time
 dependency on libcuda, so the library also loads on machines without a GPU
 driver).  refabi.cu -- the kernels with the reference's PTX entry names -- is
 compiled to spmdb200_kernels.cubin for cuModuleLoadData callers.
+tensor_lists.cpp -- the reader of lists of torch tensors -- becomes the Python
+module _tensor_lists.so, against the installed torch's headers.
 libspmdb200_checked.so is the same library with the general kernels
 (forall_map.cu, stencil_nd.cu) compiled with -DSPMDB200_CHECKED.  ptxas
 register / spill reports go to _build/ptxas.log.
@@ -19,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -31,6 +34,7 @@ LIB = PKG / "libspmdb200.so"
 CHECKED_LIB = PKG / "libspmdb200_checked.so"
 CHECKED_UNITS = ("forall_map.cu", "stencil_nd.cu")
 CUBIN = PKG / "spmdb200_kernels.cubin"
+LISTS = PKG / "_tensor_lists.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -65,6 +69,18 @@ def _run(cmd: list[str]) -> str:
     return r.stdout + r.stderr
 
 
+def build_lists() -> None:
+    """_tensor_lists.so: plain C++ against torch's and Python's headers."""
+    import torch
+    from torch.utils import cpp_extension
+    libs = cpp_extension.library_paths()
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"])],
+          str(CSRC / "tensor_lists.cpp"), "-o", str(LISTS), *[f"-L{p}" for p in libs], *[f"-Wl,-rpath,{p}" for p in libs],
+          "-ltorch_python", "-ltorch_cpu", "-lc10"])
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, checked: bool = True) -> Path:
     BUILD.mkdir(exist_ok=True)
     cc = nvcc()
@@ -75,11 +91,14 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, c
     logs: dict[str, str] = {}
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as ex:
         futs = {ex.submit(_run, [cc, *NVCC_FLAGS, "-c", str(u), "-o", str(o)]): u for u, o in todo}
+        lists = ex.submit(build_lists) if force or _stale(LISTS, [CSRC / "tensor_lists.cpp", *INCLUDE.glob("*.h")]) else None
         cubin_src = CSRC / "refabi.cu"
         if force or _stale(CUBIN, [cubin_src] + deps):
             futs[ex.submit(_run, [cc, *NVCC_FLAGS, "-cubin", str(cubin_src), "-o", str(CUBIN)])] = cubin_src
         for f in cf.as_completed(futs):
             logs[futs[f].name] = f.result()
+        if lists is not None:
+            lists.result()
     if force or todo or _stale(LIB, objs):
         _run([cc, "-shared", *ARCH, "-cudart", "static", "-Xcompiler", "-fPIC", "-o", str(LIB),
               *map(str, objs), "-lpthread", "-ldl", "-lrt"])

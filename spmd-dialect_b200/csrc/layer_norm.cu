@@ -36,8 +36,8 @@ __device__ __forceinline__ float whole_sum(float v, int lanes, float *sh, float 
 }
 
 // Streamed rows (layer_norm.cuh): weight and bias are loaded once a thread.  A
-// group of lanes takes R rows at a time: the two reductions of a row are a long
-// chain of waits, and a second row fills them.
+// group of lanes takes R rows at a time, one or two: the two reductions of a row
+// are a long chain of waits, and a second row fills them.
 constexpr int kStages = 3;
 constexpr int kStreamMost = 16;  // elements of a row in a thread
 
@@ -45,89 +45,107 @@ template <class TX, class TY, int W, int NV, int R, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
 ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
                   const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int lanes) {
-  constexpr int kBytes = W * sizeof(TX), kPitch = MAXT * kBytes;
+  constexpr int kBytes = W * sizeof(TX), kPitch = MAXT * kBytes, kStage = R * NV * kPitch;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float sh[2][R][32];
+  __shared__ __align__(16) F2 sh[2][32];
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
   const float inv_n = 1.0f / (float)cols;
   const int64_t step = (int64_t)gridDim.x * groups;
   int64_t i = (int64_t)blockIdx.x * groups + group;
-  RowAt ahead = row_at(xr, i), at = row_at(yr, i);
-  int64_t next = i;  // the row to copy next
-  const int shift = i < rows ? (int)((uintptr_t)(x + ahead.offset) / sizeof(TX) % W) : 0;
+  const int mine = row_count(i, rows, step), turns = row_count(i - group, rows, step);
+  const TX *from = x + (mine ? row_offset(xr.r, i) : 0);
+  const int shift = (int)((uintptr_t)from / sizeof(TX) % W);
+  TY *to = y + (mine ? row_offset(yr.r, i) : 0) + lane * W - shift;
+  from += lane * W - shift;
+  const Held have = held<W, NV>(cols, lane, lanes, shift);
+  int bytes[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TX));
   unsigned char *const slots = smem + threadIdx.x * kBytes;
-  int stage_in = 0, stage = 0;
+#pragma unroll
+  for (int q = 0; q < kStages * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), bytes);
+  int stage_in = 0, stage = 0, fetched = 0;  // stages as offsets
   auto fetch = [&] {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      if (next < rows) stream_row<W, NV>(slots + (stage_in * R + q) * (NV * kPitch), kPitch, x + ahead.offset, cols, lane, lanes, shift);
-      next += step;
-      next_row(xr, ahead);
+      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, bytes);
+      ++fetched;
+      from = next_row(from, x + lane * W - shift, xr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
-    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
   for (int q = 0; q < kStages - 1; ++q) fetch();
   float wv[NV][W], bv[NV][W];
   stream_weight<W, NV>(w, wtype, cols, lane, lanes, shift, 1.0f, wv);
   stream_weight<W, NV>(b, wtype, cols, lane, lanes, shift, 0.0f, bv);
-  for (int64_t block_row = i - group; block_row < rows; block_row += R * step) {
+  // R sums of a row each, as a pair.
+  auto sums = [&](const F2 (&t)[R], F2 *space) {
+    if constexpr (R == 2) return row_sum2({t[0].x + t[0].y, t[1].x + t[1].y}, lanes, space);
+    else return both(row_sum(t[0].x + t[0].y, lanes, &space->x));
+  };
+  for (int turn = 0; turn < turns; turn += R) {
     fetch();
     copy_wait<kStages - 1>();
-    float v[R][NV][W], s[R], mean[R], rstd[R];
+    F2 v[R][NV][W / 2], t[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      s[q] = 0.0f;
+      unsigned char *const slot = slots + stage + q * (NV * kPitch);
+      if (have.front) clear_front<TX>(slot, shift);
+      t[q] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        take_vec<W, TX>(slots + ((stage * R + q) * NV + k) * kPitch, v[q][k]);
-        if (!whole<W>(k, cols, lane, lanes, shift)) {
+        take_pairs<W, TX>(slot + k * kPitch, v[q][k]);
 #pragma unroll
-          for (int e = 0; e < W; ++e) {
-            const int c = shifted<W>(k, e, lane, lanes, shift);
-            if (c < 0 || c >= cols) v[q][k][e] = 0.0f;
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < W; ++e) s[q] += v[q][k][e];
+        for (int e = 0; e < W / 2; ++e) t[q] = add2(t[q], v[q][k][e]);
       }
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    row_sums<R>(s, lanes, sh[0]);
+    stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
+    const F2 mean2 = mul2(sums(t, sh[0]), both(inv_n));
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      mean[q] = s[q] * inv_n;
-      s[q] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const bool all = whole<W>(k, cols, lane, lanes, shift);
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          v[q][k][e] -= mean[q];
-          const int c = shifted<W>(k, e, lane, lanes, shift);
-          if (all || (c >= 0 && c < cols)) s[q] = fmaf(v[q][k][e], v[q][k][e], s[q]);
-        }
-      }
-    }
-    row_sums<R>(s, lanes, sh[1]);
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      rstd[q] = 1.0f / sqrtf(s[q] * inv_n + eps);
-      if (i < rows) {
+      const float mean = q ? mean2.y : mean2.x;
+      t[q] = {0.0f, 0.0f};
+      if (have.edges) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
+          const unsigned in = inside<W>(k, cols, lane, lanes, shift);
 #pragma unroll
-          for (int e = 0; e < W; ++e) v[q][k][e] = fmaf(v[q][k][e] * rstd[q], wv[k][e], bv[k][e]);
-          stream_store<W>(y + at.offset, k, cols, lane, lanes, shift, v[q][k]);
+          for (int e = 0; e < W / 2; ++e) {  // elements outside the row stay zero
+            v[q][k][e] = add2(v[q][k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
+            t[q] = fma2(v[q][k][e], v[q][k][e], t[q]);
+          }
         }
-        if (lane == 0) {
-          if (mean_out) mean_out[i] = mean[q];
-          if (rstd_out) rstd_out[i] = rstd[q];
+      } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const F2 off = both(have.whole >> k & 1 ? -mean : 0.0f);
+#pragma unroll
+          for (int e = 0; e < W / 2; ++e) {
+            v[q][k][e] = add2(v[q][k][e], off);
+            t[q] = fma2(v[q][k][e], v[q][k][e], t[q]);
+          }
         }
       }
-      i += step;
-      next_row(yr, at);
+    }
+    const F2 var2 = mul2(sums(t, sh[1]), both(inv_n));
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const float rstd = 1.0f / sqrtf((q ? var2.y : var2.x) + eps);
+      if (turn + q < mine) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int e = 0; e < W / 2; ++e)
+            v[q][k][e] = fma2(mul2(v[q][k][e], both(rstd)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
+        stream_store<W, NV>(to, have, cols, lane, lanes, shift, v[q]);
+        if (lane == 0) {
+          if (mean_out) mean_out[i + (turn + q) * step] = q ? mean2.y : mean2.x;
+          if (rstd_out) rstd_out[i + (turn + q) * step] = rstd;
+        }
+      }
+      to = next_row(to, y + lane * W - shift, yr, i + (turn + q + 1) * step);
     }
   }
   copy_wait<0>();
@@ -305,8 +323,8 @@ cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int grid, cudaStre
   auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
   const int64_t step = (int64_t)grid * (MAXT / lanes);
-  kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, step), static_cast<TY *>(p.y),
-                                   row_walk(p.yr, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
+  kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, step), static_cast<TY *>(p.y),
+                                   row_walk(p.yr, p.rows, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
   return cudaGetLastError();
 }
 

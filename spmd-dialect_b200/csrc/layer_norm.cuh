@@ -42,24 +42,32 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *sh) {
   return warp_sum_f32(lane < warps ? sh[(warp & ~(warps - 1)) + lane] : 0.0f);
 }
 
-// R sums at once; `sh` holds 32 floats for each.
-template <int R>
-__device__ __forceinline__ void row_sums(float (&v)[R], int lanes, float (*sh)[32]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = lanes >> 5;
-  for (int o = lanes < 32 ? lanes >> 1 : 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
-  if (lanes <= 32) return;
-  if (lane == 0)
-#pragma unroll
-    for (int q = 0; q < R; ++q) sh[q][warp] = v[q];
+// Two such sums at once, for rows of one block; `sh` as above, of pairs.  The
+// first exchange gives either half of the lanes one of the two to go on with.
+__device__ __forceinline__ F2 row_sum2(F2 v, int lanes, F2 *sh) {
+  const int lane = threadIdx.x & 31;
+  if (lanes == 1) return v;
+  int o = lanes < 32 ? lanes >> 1 : 16;
+  const int half = o;
+  const bool upper = lane & half;
+  float s = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, o);
+  for (o >>= 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lanes <= 32) {
+    const float t = __shfl_xor_sync(0xffffffffu, s, half);
+    return upper ? F2{t, s} : F2{s, t};
+  }
+  const int warp = threadIdx.x >> 5, warps = lanes >> 5;
+  if ((lane & 15) == 0) (upper ? sh[warp].y : sh[warp].x) = s;
   __syncthreads();
-  const int first = warp & ~(warps - 1);
+  const float4 *two = reinterpret_cast<const float4 *>(sh + (warp & ~(warps - 1)));
+  F2 t{0.0f, 0.0f};
 #pragma unroll
-  for (int q = 0; q < R; ++q) v[q] = sh[q][first + (lane & (warps - 1))];
-  for (int o = warps >> 1; o > 0; o >>= 1)
-#pragma unroll
-    for (int q = 0; q < R; ++q) v[q] += __shfl_xor_sync(0xffffffffu, v[q], o);
+  for (int q = 0; q < 8; ++q)
+    if (q < warps / 2) {
+      const float4 f = two[q];
+      t = add2(t, add2({f.x, f.y}, {f.z, f.w}));
+    }
+  return t;
 }
 
 // Which column element e of a thread's vector k is.
@@ -118,30 +126,21 @@ __device__ __forceinline__ void load_weight(const void *p, int type, int64_t fir
 }
 
 // ---- streamed rows ------------------------------------------------------------------
-// A view's row offset as a block goes through rows: `step` rows on, i1 (the row
-// within n1) and the offset grow by constants, with a correction past n1.
+// A view as a block goes through its rows: `step` elements from one to the next,
+// or, where the rows are not at one stride (wraps), each row's own offset.
 struct RowWalk {
-  int64_t n1, s0, s1;
-  int64_t i1_step, step, wrap;
+  Rows r;
+  int64_t step;
+  bool wraps;
 };
-inline RowWalk row_walk(const Rows &r, int64_t step) {
-  const int64_t a = step / r.n1, b = step - a * r.n1;
-  return {r.n1, r.s0, r.s1, b, a * r.s0 + b * r.s1, r.s0 - r.n1 * r.s1};
+inline RowWalk row_walk(const Rows &r, int64_t rows, int64_t step) { return {r, step * r.s1, rows > r.n1}; }
+template <class T>
+__device__ __forceinline__ T *next_row(T *row, T *view, const RowWalk &w, int64_t i) {
+  return w.wraps ? view + row_offset(w.r, i) : row + w.step;
 }
-struct RowAt {
-  int64_t i1, offset;
-};
-__device__ __forceinline__ RowAt row_at(const RowWalk &w, int64_t i) {
-  const int64_t a = i < w.n1 ? 0 : i / w.n1, b = i - a * w.n1;
-  return {b, a * w.s0 + b * w.s1};
-}
-__device__ __forceinline__ void next_row(const RowWalk &w, RowAt &r) {
-  r.i1 += w.i1_step;
-  r.offset += w.step;
-  if (r.i1 >= w.n1) {
-    r.i1 -= w.n1;
-    r.offset += w.wrap;
-  }
+// Rows i, i + step, ... below `rows`.
+__device__ __forceinline__ int row_count(int64_t i, int64_t rows, int64_t step) {
+  return i < rows ? (int)((rows - i + step - 1) / step) : 0;
 }
 
 // Column of element e of vector k of a thread whose rows have `shift`.
@@ -149,24 +148,77 @@ template <int W>
 __device__ __forceinline__ int shifted(int k, int e, int lane, int lanes, int shift) {
   return (k * lanes + lane) * W + e - shift;
 }
-// Starts the copies of a row's vectors into a thread's slots, `pitch` bytes apart.
-// Of a vector that holds the row's end only the row's elements are read; one
-// that holds its start is read from the vector's start (in the same aligned 16
-// bytes, so in the same allocation).
-template <int W, int NV, class T>
-__device__ __forceinline__ void stream_row(unsigned char *slot, int pitch, const T *row, int cols, int lane, int lanes, int shift) {
+// Bytes of vector k that a row has (from the vector's start: one that holds the
+// row's start is read from there, in the same aligned 16 bytes, so in the same
+// allocation; of one that holds its end only the row's are read).
+template <int W>
+__device__ __forceinline__ int vector_bytes(int k, int cols, int lane, int lanes, int shift, int size) {
+  const int left = cols - shifted<W>(k, 0, lane, lanes, shift);
+  return (left < 0 ? 0 : left < W ? left : W) * size;
+}
+// Starts the copies of a row's vectors into a thread's slots, `PITCH` bytes apart;
+// what a vector past the row's end does not have of it becomes zero.  Slots of
+// vectors that have nothing of it are zero from the start.
+template <int W, int NV, int PITCH, class T>
+__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, const int (&bytes)[NV]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (bytes[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, bytes[k]);
+}
+template <int W, int NV, int PITCH, class T>
+__device__ __forceinline__ void clear_row(unsigned char *slot, const int (&bytes)[NV]) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (!bytes[k]) {
+#pragma unroll
+      for (int q = 0; q < W * (int)sizeof(T); q += 8) *reinterpret_cast<uint2 *>(slot + k * PITCH + q) = make_uint2(0, 0);
+    }
+}
+// Bit e: whether element e of vector k is in the row.
+template <int W>
+__device__ __forceinline__ unsigned inside(int k, int cols, int lane, int lanes, int shift) {
+  unsigned m = 0;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    const int c = shifted<W>(k, e, lane, lanes, shift);
+    if (c >= 0 && c < cols) m |= 1u << e;
+  }
+  return m;
+}
+// What of its vectors a thread has in a row: bit k of `whole`, all of vector k.
+// `edges`: whether a lane of the warp has one that is there in part (the row's
+// start or end); `front`: this one has the start, `shift` elements of another row
+// before it.
+struct Held {
+  unsigned whole;
+  bool edges, front;
+};
+template <int W, int NV>
+__device__ __forceinline__ Held held(int cols, int lane, int lanes, int shift) {
+  Held h{0, false, lane == 0 && shift > 0};
+  bool part = false;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = shifted<W>(k, 0, lane, lanes, shift), left = cols - c;
-    if (left >= W) copy_async<W * sizeof(T)>(slot + k * pitch, row + c);
-    else if (left > 0) copy_async_part<W * sizeof(T)>(slot + k * pitch, row + c, left * (int)sizeof(T));
+    const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+    if (in == (1u << W) - 1) h.whole |= 1u << k;
+    else part |= in != 0;
   }
+  h.edges = __any_sync(0xffffffffu, part);
+  return h;
 }
-// Whether all of vector k's elements are in the row.
-template <int W>
-__device__ __forceinline__ bool whole(int k, int cols, int lane, int lanes, int shift) {
-  const int c = shifted<W>(k, 0, lane, lanes, shift);
-  return c >= 0 && c + W <= cols;
+// A vector out of a thread's slot as pairs.  What of another row is before this
+// one's start is made zero first, so that sums need no tests.
+template <int W, class T>
+__device__ __forceinline__ void take_pairs(const unsigned char *slot, F2 (&v)[W / 2]) {
+  float f[W];
+  take_vec<W, T>(slot, f);
+#pragma unroll
+  for (int e = 0; e < W / 2; ++e) v[e] = {f[2 * e], f[2 * e + 1]};
+}
+template <class T>
+__device__ __forceinline__ void clear_front(unsigned char *slot, int shift) {
+#pragma unroll 1
+  for (int e = 0; e < shift; ++e) reinterpret_cast<T *>(slot)[e] = from_f32<T>(0.0f);
 }
 // Weight or bias of a thread's columns; `rest` without one and past the row's ends.
 template <int W, int NV>
@@ -174,7 +226,7 @@ __device__ __forceinline__ void stream_weight(const void *p, int type, int cols,
                                               float (&v)[NV][W]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    if (p && shift == 0 && (uintptr_t)p % 16 == 0 && whole<W>(k, cols, lane, lanes, 0)) {
+    if (p && shift == 0 && (uintptr_t)p % 16 == 0 && shifted<W>(k, W, lane, lanes, 0) <= cols) {
       load_kept<W>(p, type, shifted<W>(k, 0, lane, lanes, 0), v[k]);
     } else {
 #pragma unroll
@@ -185,15 +237,27 @@ __device__ __forceinline__ void stream_weight(const void *p, int type, int cols,
     }
   }
 }
-template <int W, class T>
-__device__ __forceinline__ void stream_store(T *row, int k, int cols, int lane, int lanes, int shift, const float (&v)[W]) {
-  const int c = shifted<W>(k, 0, lane, lanes, shift);
-  if (c >= 0 && c + W <= cols) {
-    store_vec<W>(row + c, v);
-  } else {
+// A row's vectors to memory: whole ones at once, the others element by element.
+template <int W, int NV, class T>
+__device__ __forceinline__ void stream_store(T *vector, const Held &have, int cols, int lane, int lanes, int shift,
+                                             const F2 (&v)[NV][W / 2]) {
 #pragma unroll
-    for (int e = 0; e < W; ++e)
-      if (c + e >= 0 && c + e < cols) row[c + e] = from_f32<T>(v[e]);
+  for (int k = 0; k < NV; ++k)
+    if (have.whole >> k & 1) {
+      float f[W];
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) f[2 * e] = v[k][e].x, f[2 * e + 1] = v[k][e].y;
+      store_vec<W>(vector + k * lanes * W, f);
+    }
+  if (have.edges) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (!(have.whole >> k & 1)) {
+        const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (in >> e & 1) vector[k * lanes * W + e] = from_f32<T>(e & 1 ? v[k][e / 2].y : v[k][e / 2].x);
+      }
   }
 }
 

@@ -66,7 +66,7 @@ __device__ __forceinline__ void reduce_columns(const float (&sw)[NV][W], const f
 template <class TX, class TY, int W, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back<TX, TY> p, int lanes) {
   extern __shared__ __align__(16) float sums[];
-  __shared__ float sh[2][2][32];
+  __shared__ __align__(16) F2 sh[2][32];
   const int lane = threadIdx.x & (lanes - 1), groups = blockDim.x / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols;
   const float inv_n = 1.0f / (float)cols;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     float g[NV][W], x[NV][W];
     load_row<W, NV, false>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
     load_row<W, NV, false>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
-    float s[2] = {0.0f, 0.0f};
+    F2 s{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -93,14 +93,14 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
         const float xh = (x[k][e] - mean) * rstd, a = g[k][e] * w[k][e];
         sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
         sb[k][e] += g[k][e];
-        s[0] += a;
-        s[1] = fmaf(a, xh, s[1]);
+        s.x += a;
+        s.y = fmaf(a, xh, s.y);
         g[k][e] = a;
         x[k][e] = xh;
       }
     if (!p.dx) continue;
-    row_sums<2>(s, lanes, sh[turn]);
-    const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
+    s = row_sum2(s, lanes, sh[turn]);
+    const float c1 = s.x * inv_n, c2 = s.y * inv_n;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -121,94 +121,113 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
                    const __grid_constant__ RowWalk dr, int lanes) {
   constexpr int kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * MAXT * (kXBytes + kGBytes);
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float sh[2][2][32];
+  __shared__ __align__(16) F2 sh[2][32];
   __shared__ float2 stats[kStages][MAXT];  // a group's row, or a warp's where the group is wider
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
-  const int cols = (int)p.cols, mine = lanes <= 32 ? group : threadIdx.x >> 5;
+  const int cols = (int)p.cols, slot = lanes <= 32 ? group : threadIdx.x >> 5;
   const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
   const float inv_n = 1.0f / (float)cols;
-  const int64_t step = (int64_t)gridDim.x * groups;
-  int64_t i = (int64_t)blockIdx.x * groups + group;
-  RowAt x_ahead = row_at(xr, i), g_ahead = row_at(gr, i), at = row_at(dr, i);
-  int64_t next = i;
-  const int shift = i < p.rows ? (int)((uintptr_t)(p.x + x_ahead.offset) / sizeof(TX) % W) : 0;
+  const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
+  const int mine = row_count(i, p.rows, step), turns = row_count(i - group, p.rows, step);
+  const TX *x_from = p.x + (mine ? row_offset(xr.r, i) : 0);
+  const int shift = (int)((uintptr_t)x_from / sizeof(TX) % W);
+  const int64_t start = lane * W - shift;  // of the thread's first vector in a row
+  const TY *g_from = p.dy + (mine ? row_offset(gr.r, i) : 0) + start;
+  TX *to = p.dx + (mine && p.dx ? row_offset(dr.r, i) : 0) + start;
+  x_from += start;
+  const Held have = held<W, NV>(cols, lane, lanes, shift);
+  int x_bytes[NV], g_bytes[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    x_bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TX));
+    g_bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TY));
+  }
   unsigned char *const x_slots = smem + threadIdx.x * kXBytes, *const g_slots = smem + NV * MAXT * kXBytes + threadIdx.x * kGBytes;
-  int stage_in = 0, stage = 0;
+#pragma unroll
+  for (int q = 0; q < kStages; ++q) {
+    clear_row<W, NV, MAXT * kXBytes, TX>(x_slots + q * kStage, x_bytes);
+    clear_row<W, NV, MAXT * kGBytes, TY>(g_slots + q * kStage, g_bytes);
+  }
+  int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
-    if (next < p.rows) {
-      stream_row<W, NV>(x_slots + stage_in * kStage, MAXT * kXBytes, p.x + x_ahead.offset, cols, lane, lanes, shift);
-      stream_row<W, NV>(g_slots + stage_in * kStage, MAXT * kGBytes, p.dy + g_ahead.offset, cols, lane, lanes, shift);
+    if (fetched < mine) {
+      stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage, x_from, lanes, x_bytes);
+      stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage, g_from, lanes, g_bytes);
       if (first) {
-        copy_async<4>(&stats[stage_in][mine].x, p.mean + next);
-        copy_async<4>(&stats[stage_in][mine].y, p.rstd + next);
+        copy_async<4>(&stats[stage_in][slot].x, p.mean + (i + fetched * step));
+        copy_async<4>(&stats[stage_in][slot].y, p.rstd + (i + fetched * step));
       }
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
-    next += step;
-    next_row(xr, x_ahead);
-    next_row(gr, g_ahead);
+    ++fetched;
+    x_from = next_row(x_from, p.x + start, xr, i + fetched * step);
+    g_from = next_row(g_from, p.dy + start, gr, i + fetched * step);
     stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
   };
 #pragma unroll
   for (int q = 0; q < kStages - 1; ++q) fetch();
-  float w[NV][W], sw[NV][W], sb[NV][W];
+  float w[NV][W];
+  F2 sw[NV][W / 2], sb[NV][W / 2];
   stream_weight<W, NV>(p.w, p.wtype, cols, lane, lanes, shift, 1.0f, w);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
-  int turn = 0;
-  for (int64_t block_row = i - group; block_row < p.rows; block_row += step, i += step, turn ^= 1) {
+    for (int e = 0; e < W / 2; ++e) sw[k][e] = sb[k][e] = {0.0f, 0.0f};
+  for (int turn = 0; turn < turns; ++turn) {
     fetch();
     copy_wait<kStages - 1>();
     __syncwarp();  // the first lane's copies are there too
-    const bool live = i < p.rows;
-    const float2 stat = stats[stage][mine];
-    float g[NV][W], x[NV][W], s[2] = {0.0f, 0.0f};
+    const bool live = turn < mine;
+    const float2 stat = stats[stage][slot];
+    F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f}, g[NV][W / 2], x[NV][W / 2];
+    if (live) {
+      // An element outside the row has g = 0 and a finite x, and adds nothing to any sum.
+      unsigned char *const xs = x_slots + stage * kStage, *const gs = g_slots + stage * kStage;
+      if (have.front) {
+        clear_front<TX>(xs, shift);
+        clear_front<TY>(gs, shift);
+      }
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      take_vec<W, TX>(x_slots + stage * kStage + k * (MAXT * kXBytes), x[k]);
-      take_vec<W, TY>(g_slots + stage * kStage + k * (MAXT * kGBytes), g[k]);
-      if (!live || !whole<W>(k, cols, lane, lanes, shift)) {
+      for (int k = 0; k < NV; ++k) {
+        take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x[k]);
+        take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g[k]);
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const int c = shifted<W>(k, e, lane, lanes, shift);
-          if (!live || c < 0 || c >= cols) g[k][e] = x[k][e] = 0.0f;
+        for (int e = 0; e < W / 2; ++e) {
+          x[k][e] = mul2(add2(x[k][e], both(-stat.x)), both(stat.y));
+          sw[k][e] = fma2(g[k][e], x[k][e], sw[k][e]);
+          sb[k][e] = add2(g[k][e], sb[k][e]);
+          g[k][e] = mul2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]});
+          s1 = add2(s1, g[k][e]);
+          s2 = fma2(g[k][e], x[k][e], s2);
         }
       }
     }
-    const float mean = live ? stat.x : 0.0f, rstd = live ? stat.y : 0.0f;
     __syncwarp();  // every lane has its statistics: the slot may be filled again
     stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (!p.dx) continue;
+    const F2 c = mul2(row_sum2({s1.x + s1.y, s2.x + s2.y}, lanes, sh[turn & 1]), both(-inv_n));
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) g[k][e] = mul2(fma2(x[k][e], both(c.y), add2(g[k][e], both(c.x))), both(stat.y));
+      stream_store<W, NV>(to, have, cols, lane, lanes, shift, g);
+    }
+    to = next_row(to, p.dx + start, dr, i + (turn + 1) * step);
+  }
+  copy_wait<0>();
+  if (p.part) {
+    float tw[NV][W], tb[NV][W];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < W; ++e) {  // an element past the row's ends has g = 0: it adds nothing to any sum
-        const float xh = (x[k][e] - mean) * rstd, a = g[k][e] * w[k][e];
-        sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
-        sb[k][e] += g[k][e];
-        s[0] += a;
-        s[1] = fmaf(a, xh, s[1]);
-        g[k][e] = a;
-        x[k][e] = xh;
+      for (int e = 0; e < W; ++e) {
+        tw[k][e] = e & 1 ? sw[k][e / 2].y : sw[k][e / 2].x;
+        tb[k][e] = e & 1 ? sb[k][e / 2].y : sb[k][e / 2].x;
       }
-    if (!p.dx) continue;
-    row_sums<2>(s, lanes, sh[turn]);
-    const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
-    if (live) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-#pragma unroll
-        for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
-        stream_store<W>(p.dx + at.offset, k, cols, lane, lanes, shift, g[k]);
-      }
-    }
-    next_row(dr, at);
-  }
-  copy_wait<0>();
-  if (p.part)
-    reduce_columns<W, NV>(sw, sb, lanes, cols, reinterpret_cast<float *>(smem), p.part,
+    reduce_columns<W, NV>(tw, tb, lanes, cols, reinterpret_cast<float *>(smem), p.part,
                           [&](int k, int e) { return shifted<W>(k, e, lane, lanes, shift); });
+  }
 }
 
 // Longer rows, first pass: the two sums of each run of kRun columns of a row.
@@ -356,7 +375,7 @@ cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream
   const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
   *parts = stream_grid(b.rows, groups, most < kMaxParts ? most : kMaxParts, W);
   const int64_t step = *parts * groups;
-  kernel<<<*parts, MAXT, bytes, s>>>(b, row_walk(b.gr, step), row_walk(b.xr, step), row_walk(b.dr, step), lanes);
+  kernel<<<*parts, MAXT, bytes, s>>>(b, row_walk(b.gr, b.rows, step), row_walk(b.xr, b.rows, step), row_walk(b.dr, b.rows, step), lanes);
   return cudaGetLastError();
 }
 

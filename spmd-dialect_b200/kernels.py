@@ -13,6 +13,7 @@ from array import array
 import torch
 
 from ._lib import c_i, c_p, call, lib
+from ._tensor_lists import read as _read_list
 from .forall_program import insn as map_insn  # noqa: F401  (re-exported)
 
 _DTYPES = {torch.float32: "f32", torch.int32: "i32", torch.uint8: "u8", torch.float64: "f64"}
@@ -217,11 +218,8 @@ def jacobi3d(u: torch.Tensor, v: torch.Tensor, sweeps: int, res_every: int = 0, 
 # not) and on its current stream unless `stream` says otherwise, and read or
 # write no autograd state: gradients are what the *_backward entry returns.
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_FLOATS = frozenset(_TYPES)
 _E4M3 = torch.float8_e4m3fn
 STATE_BLOCK = 256  # elements that share one scale of an 8-bit optimizer state
-_get_device, _is_contiguous, _data_ptr, _numel = (getattr(torch.Tensor, n) for n in (
-    "get_device", "is_contiguous", "data_ptr", "numel"))
 
 
 def _elsewhere(dev: int, stream) -> bool:
@@ -245,9 +243,9 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _ptr(a: array | None) -> int | None:
+def _ptr(a: array) -> int:
     """Address of a host array, which the caller keeps until the call is over."""
-    return None if a is None else a.buffer_info()[0]
+    return a.buffer_info()[0]
 
 
 def _norm_operand(name: str, t: torch.Tensor, shape, dev: int, dtype=None) -> None:
@@ -383,19 +381,13 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     return dx, dweight, dbias
 
 
-def _listed(what: str, tensors: list, dev: int, dtypes) -> array:
-    """Addresses of a list of contiguous tensors of `dtypes` on device `dev`."""
-    if not {dev}.issuperset(map(_get_device, tensors)):
-        raise ValueError(f"{what}: every tensor must be on one CUDA device")
-    if not all(map(_is_contiguous, tensors)):
-        raise ValueError(f"{what}: every tensor must be contiguous")
-    if not dtypes.issuperset([t.dtype for t in tensors]):
-        raise TypeError(f"{what}: dtypes {sorted({str(t.dtype) for t in tensors} - {str(d) for d in dtypes})}")
-    return array("Q", map(_data_ptr, tensors))
+def _kinds(*dtypes: torch.dtype) -> int:
+    """Allowed dtypes of a list, as _tensor_lists.read takes them."""
+    return sum(1 << (3 if d == _E4M3 else _TYPES[d]) for d in dtypes)
 
 
-def _types(tensors: list) -> array:
-    return array("i", [_TYPES[t.dtype] for t in tensors])
+_ANY_FLOAT, _ONLY_F32, _ONLY_E4M3 = _kinds(*_TYPES), _kinds(torch.float32), _kinds(_E4M3)
+_COPIES = _kinds(torch.float16, torch.bfloat16) | 256  # an entry may be None
 
 
 def grad_norm(grads, max_norm: float | None = None, ws: torch.Tensor | None = None, stream=None):
@@ -408,16 +400,15 @@ def grad_norm(grads, max_norm: float | None = None, ws: torch.Tensor | None = No
     if _elsewhere(dev, stream):
         with _at(dev, stream):
             return grad_norm(grads, max_norm, ws)
-    ptrs, sizes, types = _listed("grad_norm", grads, dev, _FLOATS), array("q", map(_numel, grads)), _types(grads)
+    ptrs, sizes, types = _read_list("grad_norm", grads, dev, _ANY_FLOAT, None)
     if ws is None:
-        ws = torch.empty(int(lib().spmdb200_grad_norm_workspace_bytes(len(grads))), dtype=torch.uint8,
-                         device=f"cuda:{dev}")
+        ws = torch.empty(lib().spmdb200_grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8, device=f"cuda:{dev}")
     elif ws.get_device() != dev or not ws.is_contiguous():
         raise ValueError("grad_norm: ws is a contiguous tensor on the gradients' device")
     norm = torch.empty(1, dtype=torch.float32, device=ws.device)
     scale = None if max_norm is None else torch.empty_like(norm)
-    call("spmdb200_grad_norm", len(grads), _ptr(ptrs), _ptr(sizes), _ptr(types), 0.0 if max_norm is None else max_norm,
-         norm.data_ptr(), None if scale is None else scale.data_ptr(), ws.data_ptr(), ws.nbytes, _raw_stream(dev))
+    call("spmdb200_grad_norm", len(grads), ptrs, sizes, types, 0.0 if max_norm is None else max_norm, norm.data_ptr(),
+         None if scale is None else scale.data_ptr(), ws.data_ptr(), ws.nbytes, _raw_stream(dev))
     return norm, scale
 
 
@@ -467,30 +458,24 @@ def adamw(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), e
             return adamw(params, grads, exp_avg, exp_avg_sq, step=step, lr=lr, betas=betas, eps=eps,
                          weight_decay=weight_decay, exp_avg_scales=exp_avg_scales, exp_avg_sq_scales=exp_avg_sq_scales,
                          copies=copies, grad_scale=grad_scale)
-    shapes, sizes = [p.shape for p in params], array("q", map(_numel, params))
-    if [g.shape for g in grads] != shapes:
-        raise ValueError("adamw: grads must have the parameters' shapes")
-    if array("q", map(_numel, exp_avg)) != sizes or array("q", map(_numel, exp_avg_sq)) != sizes:
-        raise ValueError("adamw: exp_avg and exp_avg_sq must have the parameters' sizes")
     bits = 8 if exp_avg_scales is not None or exp_avg_sq_scales is not None else 32
-    kind = {torch.float32} if bits == 32 else {_E4M3}
-    p, g = _listed("adamw: params", params, dev, _FLOATS), _listed("adamw: grads", grads, dev, _FLOATS)
-    m, v = _listed("adamw: exp_avg", exp_avg, dev, kind), _listed("adamw: exp_avg_sq", exp_avg_sq, dev, kind)
-    p_types, g_types = _types(params), _types(grads)
+    state = _ONLY_F32 if bits == 32 else _ONLY_E4M3
+    p, sizes, p_types = _read_list("adamw: params", params, dev, _ANY_FLOAT, None)
+    g, _, g_types = _read_list("adamw: grads", grads, dev, _ANY_FLOAT, params)
+    (m, m_sizes, _), (v, v_sizes, _) = (_read_list("adamw: " + name, ts, dev, state, None) for name, ts in (
+        ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)))
+    if m_sizes != sizes or v_sizes != sizes:
+        raise ValueError("adamw: exp_avg and exp_avg_sq must have the parameters' sizes")
     m_scales = v_scales = c = c_types = None
     if bits == 8:
-        blocks = array("q", [-(-k // STATE_BLOCK) for k in sizes])
-        lists = [list(ts) if ts is not None else [] for ts in (exp_avg_scales, exp_avg_sq_scales)]
-        if any(array("q", map(_numel, ts)) != blocks for ts in lists):
+        blocks = array("q", [-(-k // STATE_BLOCK) for k in array("q", sizes)]).tobytes()
+        (m_scales, m_blocks, _), (v_scales, v_blocks, _) = (
+            _read_list("adamw: scales", [] if ts is None else list(ts), dev, _ONLY_F32, None)
+            for ts in (exp_avg_scales, exp_avg_sq_scales))
+        if m_blocks != blocks or v_blocks != blocks:
             raise ValueError(f"adamw: 8-bit states need one scale per {STATE_BLOCK} elements of each parameter")
-        m_scales, v_scales = (_listed("adamw: scales", ts, dev, {torch.float32}) for ts in lists)
     if copies is not None:
-        copies = list(copies)
-        if len(copies) != n or any(t is not None and t.shape != s for t, s in zip(copies, shapes)):
-            raise ValueError("adamw: copies must have the parameters' shapes")
-        ptrs = iter(_listed("adamw: copies", [t for t in copies if t is not None], dev, {torch.float16, torch.bfloat16}))
-        c = array("Q", [0 if t is None else next(ptrs) for t in copies])
-        c_types = array("i", [0 if t is None else _TYPES[t.dtype] for t in copies])
+        c, _, c_types = _read_list("adamw: copies", list(copies), dev, _COPIES, params)
     decay = array("d", weight_decay) if hasattr(weight_decay, "__len__") else array("d", [weight_decay]) * n
     if len(decay) != n:
         raise ValueError("adamw: weight_decay is a number or one per parameter")
@@ -501,7 +486,6 @@ def adamw(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), e
         step, step_dev = 1, _scalar("step", step, dev, torch.int64)
     if grad_scale is not None:
         factor = _scalar("grad_scale", grad_scale, dev, torch.float32)
-    call("spmdb200_adamw", n, _ptr(p), _ptr(p_types), _ptr(g), _ptr(g_types), _ptr(sizes), _ptr(m), _ptr(v), bits,
-         _ptr(m_scales), _ptr(v_scales), _ptr(c), _ptr(c_types), _ptr(decay), lr, lr_dev, betas[0], betas[1], eps, step,
-         step_dev, factor, _raw_stream(dev))
+    call("spmdb200_adamw", n, p, p_types, g, g_types, sizes, m, v, bits, m_scales, v_scales, c, c_types, _ptr(decay), lr,
+         lr_dev, betas[0], betas[1], eps, step, step_dev, factor, _raw_stream(dev))
     return params
