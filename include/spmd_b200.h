@@ -499,10 +499,14 @@ int spmdb200_jacobi3d(float *U_base, float *U_aligned, int64_t U_offset,
  * elements of w_type, unit stride; either may be NULL (1 and 0).  mean and
  * rstd (device f32, one per row in row order) may be NULL.  x_type and y_type
  * are equal, or one of them is SPMDB200_F32.  Sums are f32; y is rounded once.
- * y may be x (same view); other overlaps are undefined. */
+ * y may be x (same view); other overlaps are undefined.  ws: device memory of at
+ * least spmdb200_layer_norm_forward_workspace_bytes(rows, N) bytes, 16-byte
+ * aligned, contents irrelevant; 0 bytes (NULL) for rows of up to 8185 elements.
+ * Calls that share ws must not overlap on the GPU. */
+size_t spmdb200_layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols);
 int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_type, const int64_t *x_strides,
                         void *y, int y_type, const int64_t *y_strides, const void *weight, const void *bias,
-                        int w_type, float eps, float *mean, float *rstd, void *stream);
+                        int w_type, float eps, float *mean, float *rstd, void *ws, size_t ws_bytes, void *stream);
 
 /* Gradients of spmdb200_layer_norm.  dy has y's shape and type, mean and rstd
  * are what the forward entry wrote.  With xh = (x - mean) rstd and a = dy *

@@ -93,7 +93,8 @@ _SIGS = {
     "spmdb200_fill_jacobi3d_input": (ctypes.c_int, [c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i, ctypes.c_uint64, c_p]),
     # training-step operators
     "spmdb200_layer_norm": (ctypes.c_int, [ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, c_p,
-                                           ctypes.c_int, c_f, c_p, c_p, c_p]),
+                                           ctypes.c_int, c_f, c_p, c_p, c_p, c_sz, c_p]),
+    "spmdb200_layer_norm_forward_workspace_bytes": (c_sz, [c_i, c_i]),
     "spmdb200_layer_norm_workspace_bytes": (c_sz, [c_i, c_i]),
     "spmdb200_layer_norm_backward": (ctypes.c_int, [ctypes.c_int, c_p, c_p, ctypes.c_int, c_p, c_p, ctypes.c_int, c_p,
                                                     c_p, c_p, c_p, ctypes.c_int, c_p, c_p, c_p, c_p, ctypes.c_int,

@@ -1002,13 +1002,16 @@ void hierarchical_sum(float *A_base, float *A, int64_t A_off, int64_t A_size, in
 }
 
 // ------------------------------------------------------- training-step operators
+size_t spmdb200_layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows < 0 || cols < 1 ? 0 : layer_norm_forward_workspace_bytes(rows, cols);
+}
 size_t spmdb200_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   return rows < 0 || cols < 1 ? 0 : layer_norm_workspace_bytes(rows, cols);
 }
 
 int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_type, const int64_t *x_strides, void *y,
                         int y_type, const int64_t *y_strides, const void *weight, const void *bias, int w_type,
-                        float eps, float *mean, float *rstd, void *stream) {
+                        float eps, float *mean, float *rstd, void *ws, size_t ws_bytes, void *stream) {
   LayerNormProblem p{};
   CHECK(norm_shape(rank, sizes, x_type, y_type, &p));
   if (!(eps >= 0.0f)) return fail(SPMDB200_ERR_INVALID_ARG, "eps must be >= 0");
@@ -1022,7 +1025,10 @@ int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_typ
   CHECK(check_aligned("rstd", rstd, SPMDB200_F32));
   p.x = x, p.xtype = x_type, p.y = y, p.ytype = y_type;
   p.w = weight, p.b = bias, p.wtype = w_type;
-  p.eps = eps, p.mean = mean, p.rstd = rstd;
+  p.eps = eps, p.mean = mean, p.rstd = rstd, p.ws = ws;
+  if (const size_t need = layer_norm_forward_workspace_bytes(p.rows, p.cols))
+    if (!ws || ((uintptr_t)ws & 15u) != 0 || ws_bytes < need)
+      return fail(SPMDB200_ERR_WORKSPACE, "workspace must be >= %zu bytes and 16-byte aligned", need);
   CHECK(have_device());
   CUDA_TRY(launch_layer_norm(p, (cudaStream_t)stream));
   return ok();

@@ -16,30 +16,17 @@ namespace spmdb200 {
 
 namespace {
 
-constexpr int kMost = 32;          // elements of a row in a thread of a block of kThreads
-constexpr int kWideLanes = 1024;   // longer rows: blocks of so many threads,
-constexpr int kWideMost = 16;      // with so many elements each (64 registers a thread)
-constexpr int kCluster = 8;        // still longer ones: blocks that share a row
-constexpr int64_t kHeld = (int64_t)kThreads * kMost, kWideHeld = (int64_t)kWideLanes * kWideMost;
-
-template <bool CLUSTER>
-__device__ __forceinline__ float whole_sum(float v, int lanes, float *sh, float *mine) {
-  v = row_sum(v, lanes, sh);
-  if constexpr (CLUSTER) {
-    cg::cluster_group cluster = cg::this_cluster();
-    if (threadIdx.x == 0) *mine = v;
-    cluster.sync();
-    const int lane = threadIdx.x & 31;
-    v = warp_sum_f32(lane < (int)cluster.num_blocks() ? *cluster.map_shared_rank(mine, lane) : 0.0f);
-  }
-  return v;
-}
+constexpr int kMost = 16;         // elements of a row in a thread
+constexpr int kHalfLanes = 512;   // threads of a block for rows past kThreads * kMost columns
+constexpr int kLongLanes = 1024;  // threads of a block for long rows of any strides,
+constexpr int kCluster = 8;       // and at most so many of them share a row
+constexpr int64_t kHeld = (int64_t)kThreads * kMost, kHalfHeld = (int64_t)kHalfLanes * kMost;
+constexpr int64_t kLongRun = (int64_t)kLongLanes * kMost;
 
 // Streamed rows (layer_norm.cuh): weight and bias are loaded once a thread.  A
 // group of lanes takes R rows at a time, one or two: the two reductions of a row
 // are a long chain of waits, and a second row fills them.
 constexpr int kStages = 3;
-constexpr int kStreamMost = 16;  // elements of a row in a thread
 
 template <class TX, class TY, int W, int NV, int R, int MAXT>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
@@ -50,25 +37,24 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   __shared__ __align__(16) F2 sh[2][32];
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
   const float inv_n = 1.0f / (float)cols;
-  const int64_t step = (int64_t)gridDim.x * groups;
-  int64_t i = (int64_t)blockIdx.x * groups + group;
+  const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
   const int mine = row_count(i, rows, step), turns = row_count(i - group, rows, step);
   const TX *from = x + (mine ? row_offset(xr.r, i) : 0);
   const int shift = (int)((uintptr_t)from / sizeof(TX) % W);
   TY *to = y + (mine ? row_offset(yr.r, i) : 0) + lane * W - shift;
   from += lane * W - shift;
   const Held have = held<W, NV>(cols, lane, lanes, shift);
-  int bytes[NV];
+  int left[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TX));
+  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
   unsigned char *const slots = smem + threadIdx.x * kBytes;
 #pragma unroll
-  for (int q = 0; q < kStages * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), bytes);
+  for (int q = 0; q < kStages * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), left);
   int stage_in = 0, stage = 0, fetched = 0;  // stages as offsets
   auto fetch = [&] {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, bytes);
+      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, left);
       ++fetched;
       from = next_row(from, x + lane * W - shift, xr, i + fetched * step);
     }
@@ -78,12 +64,15 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 #pragma unroll
   for (int q = 0; q < kStages - 1; ++q) fetch();
   float wv[NV][W], bv[NV][W];
-  stream_weight<W, NV>(w, wtype, cols, lane, lanes, shift, 1.0f, wv);
-  stream_weight<W, NV>(b, wtype, cols, lane, lanes, shift, 0.0f, bv);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, true>(w, wtype, 0, 0, cols, k, lane, lanes, shift, 1.0f, wv[k]);
+    load_weight<W, true>(b, wtype, 0, 0, cols, k, lane, lanes, shift, 0.0f, bv[k]);
+  }
   // R sums of a row each, as a pair.
-  auto sums = [&](const F2 (&t)[R], F2 *space) {
-    if constexpr (R == 2) return row_sum2({t[0].x + t[0].y, t[1].x + t[1].y}, lanes, space);
-    else return both(row_sum(t[0].x + t[0].y, lanes, &space->x));
+  auto sums = [&](const F2 (&t)[R], int space) {
+    if constexpr (R == 2) return row_sum2({t[0].x + t[0].y, t[1].x + t[1].y}, lanes, sh[space]);
+    else return both(row_sum(t[0].x + t[0].y, lanes, &sh[space]->x));
   };
   for (int turn = 0; turn < turns; turn += R) {
     fetch();
@@ -102,7 +91,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
       }
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
-    const F2 mean2 = mul2(sums(t, sh[0]), both(inv_n));
+    const F2 mean2 = mul2(sums(t, 0), both(inv_n));
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const float mean = q ? mean2.y : mean2.x;
@@ -129,7 +118,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
         }
       }
     }
-    const F2 var2 = mul2(sums(t, sh[1]), both(inv_n));
+    const F2 var2 = mul2(sums(t, 1), both(inv_n));
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const float rstd = 1.0f / sqrtf((q ? var2.y : var2.x) + eps);
@@ -151,64 +140,51 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   copy_wait<0>();
 }
 
-template <class TX, class TY, int W, int NV, bool VEC, int MAXT, bool CLUSTER>
-__global__ void __launch_bounds__(MAXT, MAXT == kThreads ? 3 : 1)
-ln_forward(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, int wtype, int64_t rows, int64_t all_cols,
-           float eps, float *mean_out, float *rstd_out, int lanes) {
+// Rows of any strides.  Rows past the last take part in the barriers, with no
+// columns.
+template <class TX, class TY, int W, int NV>
+__global__ void __launch_bounds__(kThreads, 3)
+ln_forward(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, int wtype, int64_t rows, int cols, float eps,
+           float *mean_out, float *rstd_out, int lanes) {
   __shared__ float sh[2][32];
-  __shared__ float mine[2];
-  const int lane = threadIdx.x & (lanes - 1);
-  const float inv_n = 1.0f / (float)all_cols;
-  int64_t first = 0, i = (int64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes,
-          step = (int64_t)gridDim.x * (blockDim.x / lanes);
-  int cols = (int)all_cols;
-  if constexpr (CLUSTER) {  // each block of a cluster has an equal run of the row's columns
-    first = (int64_t)cg::this_cluster().block_rank() * (lanes * NV * W);
-    const int64_t left = all_cols - first;
-    cols = left < 0 ? 0 : left < lanes * NV * W ? (int)left : lanes * NV * W;
-    i = blockIdx.x / cg::this_cluster().num_blocks(), step = gridDim.x / cg::this_cluster().num_blocks();
-  }
-  // Rows past the last take part in the barriers, with no columns.
-  for (int64_t block_row = CLUSTER ? i : i - threadIdx.x / lanes; block_row < rows; block_row += step, i += step) {
+  const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes;
+  const float inv_n = 1.0f / (float)cols;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / lanes);
+  for (int64_t i = (int64_t)blockIdx.x * (kThreads / lanes) + group; i - group < rows; i += step) {
     const int n = i < rows ? cols : 0;
     float v[NV][W], s = 0.0f;
-    load_row<W, NV, VEC>(x + (n ? row_offset(xr, i) + first * xr.sc : 0), xr.sc, n, lane, lanes, 0.0f, v);
+    load_row<W, NV, false>(x + (n ? row_offset(xr, i) : 0), xr.sc, 0, n, lane, lanes, 0, 0.0f, v);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < W; ++e) s += v[k][e];
-    const float mean = whole_sum<CLUSTER>(s, lanes, sh[0], &mine[0]) * inv_n;
+    const float mean = row_sum(s, lanes, sh[0]) * inv_n;
     s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool whole = VEC && column<W, VEC>(k, W - 1, lane, lanes) < n;
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         v[k][e] -= mean;
-        if (whole || column<W, VEC>(k, e, lane, lanes) < n) s = fmaf(v[k][e], v[k][e], s);
+        if (column<W, false>(k, e, lane, lanes, 0) < n) s = fmaf(v[k][e], v[k][e], s);
       }
-    }
-    const float rstd = 1.0f / sqrtf(whole_sum<CLUSTER>(s, lanes, sh[1], &mine[1]) * inv_n + eps);
+    const float rstd = 1.0f / sqrtf(row_sum(s, lanes, sh[1]) * inv_n + eps);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float wv[W], bv[W];
-      load_weight<W, VEC>(w, wtype, first, n, k, lane, lanes, 1.0f, wv);
-      load_weight<W, VEC>(b, wtype, first, n, k, lane, lanes, 0.0f, bv);
+      load_weight<W, false>(w, wtype, 0, 0, n, k, lane, lanes, 0, 1.0f, wv);
+      load_weight<W, false>(b, wtype, 0, 0, n, k, lane, lanes, 0, 0.0f, bv);
 #pragma unroll
       for (int e = 0; e < W; ++e) v[k][e] = fmaf(v[k][e] * rstd, wv[e], bv[e]);
     }
-    store_row<W, NV, VEC>(y + (n ? row_offset(yr, i) + first * yr.sc : 0), yr.sc, n, lane, lanes, v);
-    if (lane == 0 && n && first == 0) {
+    store_row<W, NV, false>(y + (n ? row_offset(yr, i) : 0), yr.sc, 0, n, lane, lanes, 0, v);
+    if (lane == 0 && n) {
       if (mean_out) mean_out[i] = mean;
       if (rstd_out) rstd_out[i] = rstd;
     }
-    if constexpr (CLUSTER) cg::this_cluster().sync();  // the others have read `mine`
   }
 }
 
-// Rows longer than a cluster holds: the same cluster reads them twice, the
-// second time from L2.  A thread's elements are taken kWideMost at a time; two
-// sets' count, mean and sum of squares around it join into those of both.
+// Two sets' count, mean and sum of squares around it join into those of both.
 struct Moments {
   float n, mean, m2;
 };
@@ -218,73 +194,235 @@ __device__ __forceinline__ Moments join(Moments a, Moments b) {
   const float d = b.mean - a.mean, share = b.n / n;
   return {n, fmaf(d, share, a.mean), a.m2 + b.m2 + d * d * a.n * share};
 }
-template <class TX, class TY, int W, bool VEC>
-__global__ void __launch_bounds__(kWideLanes)
+__device__ __forceinline__ Moments join_warp(Moments a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = join(a, {__shfl_xor_sync(0xffffffffu, a.n, o), __shfl_xor_sync(0xffffffffu, a.mean, o),
+                 __shfl_xor_sync(0xffffffffu, a.m2, o)});
+  return {__shfl_sync(0xffffffffu, a.n, 0), __shfl_sync(0xffffffffu, a.mean, 0), __shfl_sync(0xffffffffu, a.m2, 0)};
+}
+
+// Longer rows, first pass: moments of each warp's share of a run.
+constexpr int kCutStages = 4;
+
+template <class TX, int W>
+__global__ void __launch_bounds__(kThreads, 4)
+ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const __grid_constant__ Cut cut, float4 *shares) {
+  constexpr int NV = kCutMost / W, kBytes = W * sizeof(TX), kPitch = kThreads * kBytes, kStage = NV * kPitch;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const CutPlace at = cut_place(cut);
+  if (at.rows == 0) return;
+  const int lane = threadIdx.x;
+  const TX *from = x + row_offset(xr.r, at.i);
+  const int64_t first = at.run * kRun;
+  const int start = (int)((uintptr_t)from / sizeof(TX) % W);
+  // The run's columns, relative to `first`: from `low` (0 or the run before's end) to `high`.
+  const int low = at.run == 0 ? 0 : -start, high = cols - first < kRun - start ? (int)(cols - first) : kRun - start;
+  // As a row of its own that starts `shift` elements into its first vector.
+  const int shift = at.run == 0 ? start : 0, n = high - low;
+  from += first + low + lane * W - shift;
+  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  int left[NV];
+  float count = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    left[k] = vector_left<W>(k, n, lane, kThreads, shift);
+    count += (float)__popc(inside<W>(k, n, lane, kThreads, shift));
+  }
+  unsigned char *const slots = smem + threadIdx.x * kBytes;
+#pragma unroll
+  for (int q = 0; q < kCutStages; ++q) clear_row<W, NV, kPitch, TX>(slots + q * kStage, left);
+  const float inv_count = count > 0.0f ? 1.0f / count : 0.0f, all = warp_sum_f32(count), inv_all = all > 0.0f ? 1.0f / all : 0.0f;
+  int stage_in = 0, stage = 0, fetched = 0;
+  auto fetch = [&] {
+    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, left);
+    copy_commit();
+    ++fetched;
+    from = next_row(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
+  };
+#pragma unroll
+  for (int q = 0; q < kCutStages - 1; ++q) fetch();
+  for (int turn = 0; turn < at.rows; ++turn) {
+    fetch();
+    copy_wait<kCutStages - 1>();
+    if (have.front) clear_front<TX>(slots + stage, shift);
+    F2 v[NV][W / 2], t{0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      take_pairs<W, TX>(slots + stage + k * kPitch, v[k]);
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) t = add2(t, v[k][e]);
+    }
+    stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
+    // Around the thread's mean, then the threads' means around the warp's.
+    const float sum = t.x + t.y, mean = sum * inv_count;
+    t = {0.0f, 0.0f};
+    if (have.edges) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const unsigned in = inside<W>(k, n, lane, kThreads, shift);
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) {
+          const F2 d = add2(v[k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
+          t = fma2(d, d, t);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const F2 off = both(have.whole >> k & 1 ? -mean : 0.0f);
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) {
+          const F2 d = add2(v[k][e], off);
+          t = fma2(d, d, t);
+        }
+      }
+    }
+    const float warp_mean = warp_sum_f32(sum) * inv_all, d = mean - warp_mean;
+    const float m2 = warp_sum_f32(fmaf(count * d, d, t.x + t.y));
+    if ((lane & 31) == 0)
+      shares[((at.i - cut.first + (int64_t)turn * cut.parts) * cut.runs + at.run) * kCutWarps + (lane >> 5)] = make_float4(all, warp_mean, m2, 0.0f);
+  }
+  copy_wait<0>();
+}
+
+// Second pass: the rows' statistics from the shares, and the output.
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kThreads, 2)
+ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w, const void *b,
+           int wtype, int64_t cols, float eps, float *mean_out, float *rstd_out, const __grid_constant__ Cut cut, const float4 *shares) {
+  constexpr int NV = kCutMost / W, kBytes = W * sizeof(TX), kPitch = kThreads * kBytes, kStage = NV * kPitch;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float2 stats[kCutRows];  // -mean, rstd
+  const CutPlace at = cut_place(cut);
+  if (at.rows == 0) return;
+  const int lane = threadIdx.x;
+  const TX *from = x + row_offset(xr.r, at.i);
+  const int64_t first = at.run * kRun;
+  const int start = (int)((uintptr_t)from / sizeof(TX) % W);
+  const int low = at.run == 0 ? 0 : -start, high = cols - first < kRun - start ? (int)(cols - first) : kRun - start;
+  const int shift = at.run == 0 ? start : 0, n = high - low;
+  TY *to = y + row_offset(yr.r, at.i) + first + low + lane * W - shift;
+  from += first + low + lane * W - shift;
+  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  int left[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
+  unsigned char *const slots = smem + threadIdx.x * kBytes;
+#pragma unroll
+  for (int q = 0; q < kCutStages; ++q) clear_row<W, NV, kPitch, TX>(slots + q * kStage, left);
+  int stage_in = 0, stage = 0, fetched = 0;
+  auto fetch = [&] {
+    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, left);
+    copy_commit();
+    ++fetched;
+    from = next_row(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
+  };
+#pragma unroll
+  for (int q = 0; q < kCutStages - 1; ++q) fetch();
+  float wv[NV][W], bv[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, true>(w, wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, wv[k]);
+    load_weight<W, true>(b, wtype, first + low, 0, n, k, lane, kThreads, shift, 0.0f, bv[k]);
+  }
+  for (int r = lane >> 5; r < at.rows; r += kCutWarps) {  // a warp a row, in one order
+    const int64_t i = at.i + (int64_t)r * cut.parts;
+    Moments m{0.0f, 0.0f, 0.0f};
+    for (int64_t q = lane & 31; q < cut.runs * kCutWarps; q += 32) {
+      const float4 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
+      m = join(m, {s.x, s.y, s.z});
+    }
+    m = join_warp(m);
+    const float rstd = 1.0f / sqrtf(m.m2 / (float)cols + eps);
+    if ((lane & 31) == 0) {
+      stats[r] = make_float2(-m.mean, rstd);
+      if (at.run == 0) {
+        if (mean_out) mean_out[i] = m.mean;
+        if (rstd_out) rstd_out[i] = rstd;
+      }
+    }
+  }
+  __syncthreads();
+  for (int turn = 0; turn < at.rows; ++turn) {
+    fetch();
+    copy_wait<kCutStages - 1>();
+    const float2 stat = stats[turn];
+    F2 v[NV][W / 2];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      take_pairs<W, TX>(slots + stage + k * kPitch, v[k]);
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e)
+        v[k][e] = fma2(mul2(add2(v[k][e], both(stat.x)), both(stat.y)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
+    }
+    stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
+    stream_store<W, NV>(to, have, n, lane, kThreads, shift, v);
+    to = next_row(to, y + first + low + lane * W - shift, yr, at.i + (int64_t)(turn + 1) * cut.parts);
+  }
+  copy_wait<0>();
+}
+
+// Longer rows of any strides: a cluster reads them twice, the second time from L2.
+// A thread's elements are taken kMost at a time.
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kLongLanes)
 ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, int wtype, int64_t rows, int64_t cols,
                 float eps, float *mean_out, float *rstd_out) {
-  constexpr int NV = kWideMost / W;
-  __shared__ Moments sh[kWideLanes / 32], mine;
+  constexpr int NV = kMost / W;
+  __shared__ Moments sh[kLongLanes / 32], mine;
   cg::cluster_group cluster = cg::this_cluster();
-  const int lane = threadIdx.x & 31;
-  const int64_t runs = (cols + kWideHeld - 1) / kWideHeld;
-  for (int64_t i = blockIdx.x / kCluster; i < rows; i += gridDim.x / kCluster) {
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
+  const int64_t runs = (cols + kLongRun - 1) / kLongRun;
+  for (int64_t i = blockIdx.x / blocks; i < rows; i += gridDim.x / blocks) {
     const TX *px = x + row_offset(xr, i);
+    TY *py = y + row_offset(yr, i);
     Moments m{0.0f, 0.0f, 0.0f};
     float v[NV][W];
-    for (int64_t r = cluster.block_rank(); r < runs; r += kCluster) {
-      const int64_t first = r * kWideHeld;
-      const int n = cols - first < kWideHeld ? (int)(cols - first) : (int)kWideHeld;
-      load_row<W, NV, VEC>(px + first * xr.sc, xr.sc, n, threadIdx.x, kWideLanes, 0.0f, v);
+    for (int64_t r = rank; r < runs; r += blocks) {
+      const int n = cols - r * kLongRun < kLongRun ? (int)(cols - r * kLongRun) : (int)kLongRun;
+      load_row<W, NV, false>(px + r * kLongRun * xr.sc, xr.sc, 0, n, threadIdx.x, kLongLanes, 0, 0.0f, v);
       Moments t{0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           t.mean += v[k][e];
-          t.n += column<W, VEC>(k, e, threadIdx.x, kWideLanes) < n ? 1.0f : 0.0f;
+          t.n += column<W, false>(k, e, threadIdx.x, kLongLanes, 0) < n ? 1.0f : 0.0f;
         }
       t.mean /= fmaxf(t.n, 1.0f);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < W; ++e)
-          if (column<W, VEC>(k, e, threadIdx.x, kWideLanes) < n) t.m2 = fmaf(v[k][e] - t.mean, v[k][e] - t.mean, t.m2);
+          if (column<W, false>(k, e, threadIdx.x, kLongLanes, 0) < n) t.m2 = fmaf(v[k][e] - t.mean, v[k][e] - t.mean, t.m2);
       m = join(m, t);
     }
-    auto over_warp = [](Moments a) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        a = join(a, {__shfl_xor_sync(0xffffffffu, a.n, o), __shfl_xor_sync(0xffffffffu, a.mean, o),
-                     __shfl_xor_sync(0xffffffffu, a.m2, o)});
-      return a;
-    };
-    m = over_warp(m);
+    m = join_warp(m);
     if (lane == 0) sh[threadIdx.x >> 5] = m;
     __syncthreads();
-    m = over_warp(sh[lane]);
+    m = join_warp(sh[lane]);
     if (threadIdx.x == 0) mine = m;
     cluster.sync();
-    m = over_warp(lane < kCluster ? *cluster.map_shared_rank(&mine, lane) : Moments{0.0f, 0.0f, 0.0f});
-    // Lanes join in orders of their own: the first one's result is the row's.
-    const float mean = __shfl_sync(0xffffffffu, m.mean, 0);
-    const float rstd = 1.0f / sqrtf(__shfl_sync(0xffffffffu, m.m2, 0) / (float)cols + eps);
-    TY *py = y + row_offset(yr, i);
-    for (int64_t r = cluster.block_rank(); r < runs; r += kCluster) {
-      const int64_t first = r * kWideHeld;
-      const int n = cols - first < kWideHeld ? (int)(cols - first) : (int)kWideHeld;
-      load_row<W, NV, VEC>(px + first * xr.sc, xr.sc, n, threadIdx.x, kWideLanes, 0.0f, v);
+    m = join_warp(lane < blocks ? *cluster.map_shared_rank(&mine, lane) : Moments{0.0f, 0.0f, 0.0f});
+    const float rstd = 1.0f / sqrtf(m.m2 / (float)cols + eps);
+    for (int64_t r = rank; r < runs; r += blocks) {
+      const int n = cols - r * kLongRun < kLongRun ? (int)(cols - r * kLongRun) : (int)kLongRun;
+      load_row<W, NV, false>(px + r * kLongRun * xr.sc, xr.sc, 0, n, threadIdx.x, kLongLanes, 0, 0.0f, v);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         float wv[W], bv[W];
-        load_weight<W, VEC>(w, wtype, first, n, k, threadIdx.x, kWideLanes, 1.0f, wv);
-        load_weight<W, VEC>(b, wtype, first, n, k, threadIdx.x, kWideLanes, 0.0f, bv);
+        load_weight<W, false>(w, wtype, r * kLongRun, 0, n, k, threadIdx.x, kLongLanes, 0, 1.0f, wv);
+        load_weight<W, false>(b, wtype, r * kLongRun, 0, n, k, threadIdx.x, kLongLanes, 0, 0.0f, bv);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - mean) * rstd, wv[e], bv[e]);
+        for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - m.mean) * rstd, wv[e], bv[e]);
       }
-      store_row<W, NV, VEC>(py + first * yr.sc, yr.sc, n, threadIdx.x, kWideLanes, v);
+      store_row<W, NV, false>(py + r * kLongRun * yr.sc, yr.sc, 0, n, threadIdx.x, kLongLanes, 0, v);
     }
-    if (threadIdx.x == 0 && cluster.block_rank() == 0) {
-      if (mean_out) mean_out[i] = mean;
+    if (threadIdx.x == 0 && rank == 0) {
+      if (mean_out) mean_out[i] = m.mean;
       if (rstd_out) rstd_out[i] = rstd;
     }
     cluster.sync();  // the others have read `mine`, and sh may be written again
@@ -292,37 +430,13 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
 }
 
 // ---- launches ---------------------------------------------------------------------
-struct Launch {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute at[1];
-  Launch(int64_t blocks, int threads, int cluster, cudaStream_t s) {
-    cfg.gridDim = dim3(grid_for(blocks < ((int64_t)1 << 30) ? blocks : (int64_t)1 << 30));  // a multiple of the cluster
-    cfg.blockDim = dim3(threads);
-    cfg.stream = s;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-  }
-};
-
-template <class TX, class TY, int NV, bool VEC, int MAXT, bool CLUSTER>
-cudaError_t forward_rows(const LayerNormProblem &p, int lanes, int cluster, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
-  const int threads = CLUSTER || lanes > kThreads ? lanes : kThreads;
-  const int64_t per_block = threads / lanes;
-  const Launch l(CLUSTER ? (p.rows < (1 << 24) ? p.rows : (1 << 24)) * cluster : (p.rows + per_block - 1) / per_block, threads, cluster, s);
-  return cudaLaunchKernelEx(&l.cfg, ln_forward<TX, TY, W, NV, VEC, MAXT, CLUSTER>, static_cast<const TX *>(p.x), p.xr,
-                            static_cast<TY *>(p.y), p.yr, p.w, p.b, p.wtype, p.rows, p.cols, p.eps, p.mean, p.rstd, lanes);
-}
-
 template <class TX, class TY, int NV, int R, int MAXT>
-cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int grid, cudaStream_t s) {
+cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, bytes = kStages * R * NV * MAXT * W * (int)sizeof(TX);
   auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-  const int64_t step = (int64_t)grid * (MAXT / lanes);
+  const int groups = MAXT / lanes, grid = stream_grid(p.rows, groups, most, W);
+  const int64_t step = (int64_t)grid * groups;
   kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, step), static_cast<TY *>(p.y),
                                    row_walk(p.yr, p.rows, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
   return cudaGetLastError();
@@ -332,57 +446,89 @@ cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int grid, cudaStre
 // where those are fewer (then one row at a time).
 template <class TX, class TY>
 cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, NV = kStreamMost / W;
-  if (p.cols + spare > kThreads * kStreamMost)
-    return stream_rows<TX, TY, NV, 1, 2 * kThreads>(p, 2 * kThreads, stream_grid(p.rows, 1, device_sms(), W), s);
-  const int lanes = row_lanes(p.rows, p.cols, W, kStreamMost, spare), groups = kThreads / lanes;
+  constexpr int W = kWidth<TX, TY>, NV = kMost / W;
+  if (p.cols + spare > kHeld) {
+    if (p.rows <= device_sms()) return stream_rows<TX, TY, NV, 1, kHalfLanes>(p, kHalfLanes, device_sms(), s);
+    return stream_rows<TX, TY, NV, 2, kHalfLanes>(p, kHalfLanes, device_sms(), s);
+  }
+  const int lanes = row_lanes(p.rows, p.cols, W, kMost, spare), groups = kThreads / lanes;
   const int nv = row_vectors(p.cols + spare, lanes, W), most = (nv * W > 8 ? 2 : 3) * device_sms();
-  const int grid = stream_grid(p.rows, groups, most, W);
-  if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads>(p, lanes, grid, s);
-  if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads>(p, lanes, grid, s);
-  if (p.rows <= (int64_t)most * groups) return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, grid, s);
-  return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, grid, s);
+  if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads>(p, lanes, most, s);
+  if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads>(p, lanes, most, s);
+  if (p.rows <= (int64_t)most * groups) return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, most, s);
+  return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, most, s);
 }
 
-template <class TX, class TY, bool VEC>
-cudaError_t forward_of(const LayerNormProblem &p, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
-  if (p.cols > kWideHeld * kCluster) {
-    const Launch l((p.rows < (1 << 24) ? p.rows : (1 << 24)) * kCluster, kWideLanes, kCluster, s);
-    return cudaLaunchKernelEx(&l.cfg, ln_forward_long<TX, TY, W, VEC>, static_cast<const TX *>(p.x), p.xr,
-                              static_cast<TY *>(p.y), p.yr, p.w, p.b, p.wtype, p.rows, p.cols, p.eps, p.mean, p.rstd);
+template <class TX, class TY>
+cudaError_t forward_cut(const LayerNormProblem &p, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, bytes = kCutStages * kRun * (int)sizeof(TX);
+  auto first = ln_moments<TX, W>;
+  auto second = ln_outputs<TX, TY, W>;
+  if (cudaError_t e = cudaFuncSetAttribute(first, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  if (cudaError_t e = cudaFuncSetAttribute(second, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  const int64_t runs = most_runs(p.cols), batch = batch_rows(p.rows, p.cols, sizeof(TX));
+  const int period = row_period(p.xr, p.rows, W);
+  const int parts1 = cut_parts(batch, runs, 4 * device_sms(), period), parts2 = cut_parts(batch, runs, 2 * device_sms(), period);
+  float4 *shares = static_cast<float4 *>(p.ws);
+  for (int64_t row = 0; row < p.rows; row += batch) {
+    const int64_t last = row + batch < p.rows ? row + batch : p.rows;
+    first<<<grid_for(runs * parts1), kThreads, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, parts1), p.cols,
+                                                           Cut{row, last, runs, parts1}, shares);
+    if (cudaError_t e = cudaGetLastError()) return e;
+    second<<<grid_for(runs * parts2), kThreads, bytes, s>>>(
+        static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, parts2), static_cast<TY *>(p.y), row_walk(p.yr, p.rows, parts2), p.w,
+        p.b, p.wtype, p.cols, p.eps, p.mean, p.rstd, Cut{row, last, runs, parts2}, shares);
+    if (cudaError_t e = cudaGetLastError()) return e;
   }
-  if (p.cols > kWideHeld) {
-    int cluster = 2;
-    while (p.cols > kWideHeld * cluster) cluster *= 2;
-    return forward_rows<TX, TY, kWideMost / W, VEC, kWideLanes, true>(p, kWideLanes, cluster, s);
-  }
-  if (p.cols > kHeld) return forward_rows<TX, TY, kWideMost / W, VEC, kWideLanes, false>(p, kWideLanes, 1, s);
-  if constexpr (VEC) {  // what is left of shorter rows: weights at odd addresses
-    return forward_rows<TX, TY, kMost / W, true, kThreads, false>(p, kThreads, 1, s);
-  }
-  const int lanes = row_lanes(p.rows, p.cols, W, kMost, 0);
-  switch (row_vectors(p.cols, lanes, W)) {
-    case 1: return forward_rows<TX, TY, 1, false, kThreads, false>(p, lanes, 1, s);
-    case 2: return forward_rows<TX, TY, 2, false, kThreads, false>(p, lanes, 1, s);
-    case 4: return forward_rows<TX, TY, 4, false, kThreads, false>(p, lanes, 1, s);
-    default: return forward_rows<TX, TY, kMost / W, false, kThreads, false>(p, lanes, 1, s);
-  }
+  return cudaSuccess;
+}
+
+template <class TX, class TY, int NV>
+cudaError_t strided_rows(const LayerNormProblem &p, int lanes, cudaStream_t s) {
+  const int64_t groups = kThreads / lanes;
+  ln_forward<TX, TY, kWidth<TX, TY>, NV><<<grid_for((p.rows + groups - 1) / groups), kThreads, 0, s>>>(
+      static_cast<const TX *>(p.x), p.xr, static_cast<TY *>(p.y), p.yr, p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean,
+      p.rstd, lanes);
+  return cudaGetLastError();
+}
+
+template <class TX, class TY>
+cudaError_t long_rows(const LayerNormProblem &p, cudaStream_t s) {
+  int cluster = 1;
+  while (cluster < kCluster && p.cols > kLongRun * cluster) cluster *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.rows < (1 << 24) ? p.rows : (1 << 24)) * cluster));
+  cfg.blockDim = dim3(kLongLanes);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, ln_forward_long<TX, TY, kWidth<TX, TY>>, static_cast<const TX *>(p.x), p.xr,
+                            static_cast<TY *>(p.y), p.yr, p.w, p.b, p.wtype, p.rows, p.cols, p.eps, p.mean, p.rstd);
 }
 
 template <class TX, class TY>
 cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
+  constexpr int W = kWidth<TX, TY>, NV = kMost / W;
   const int spare = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) ? 0 : W - 1;
-  if (p.cols + spare <= 2 * kThreads * kStreamMost && p.xr.sc == 1 && p.yr.sc == 1 &&
-      same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
-    return forward_streamed<TX, TY>(p, spare, s);
-  const bool vec = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) && vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) &&
-                   vec_weight(p.w) && vec_weight(p.b);
-  return vec ? forward_of<TX, TY, true>(p, s) : forward_of<TX, TY, false>(p, s);
+  if (p.xr.sc == 1 && p.yr.sc == 1 && same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
+    return p.cols + spare <= kHalfHeld ? forward_streamed<TX, TY>(p, spare, s) : forward_cut<TX, TY>(p, s);
+  if (p.cols > kHeld) return long_rows<TX, TY>(p, s);
+  const int lanes = row_lanes(p.rows, p.cols, W, kMost, 0), nv = row_vectors(p.cols, lanes, W);
+  if (nv == 1) return strided_rows<TX, TY, 1>(p, lanes, s);
+  if (nv < NV) return strided_rows<TX, TY, 2>(p, lanes, s);
+  return strided_rows<TX, TY, NV>(p, lanes, s);
 }
 
 }  // namespace
+
+size_t layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols) {
+  if (cols <= kHalfHeld - 7) return 0;
+  return (size_t)batch_rows(rows, cols, 2) * (size_t)most_runs(cols) * kCutWarps * sizeof(float4);
+}
 
 cudaError_t launch_layer_norm(const LayerNormProblem &p, cudaStream_t s) {
   return by_types(p.xtype, p.ytype, [&](auto tx, auto ty) { return forward<decltype(tx), decltype(ty)>(p, s); });

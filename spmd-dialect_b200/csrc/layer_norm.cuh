@@ -1,16 +1,14 @@
 // layer_norm.cuh -- what the two directions of the layer norm share.
 //
 // A row is taken by `lanes` threads (a power of two), each with NV vectors of W
-// elements; W is what 16 bytes of the wider type hold.  Three layouts:
-// - Streamed rows (up to a few thousand columns, last dimension contiguous): a
-//   block goes through rows with stride, the next rows on their way to shared
-//   memory while one is computed.  Thread t copies and reads the aligned vectors
-//   t, t + lanes, ... that cover the row.  A row may start `shift` elements into
-//   its first vector (odd lengths, odd addresses): the stride of rows is a
-//   multiple of W, so that a thread's rows all have one shift, and its columns,
-//   with their weights and sums in registers, are the same in all of them.
-// - VEC: rows at vector alignment, thread t's vectors t, t + lanes, ...
+// elements; W is what 16 bytes of the wider type hold.  Two layouts:
+// - Vectors: thread t has the aligned vectors t, t + lanes, ... that cover the
+//   row, whose last dimension is contiguous.  The row may start `shift` elements
+//   into its first vector (odd lengths, odd addresses).
 // - Any strides and addresses: single elements t, t + lanes, ...
+// A block that goes through rows with vectors does so with a stride of rows that
+// is a multiple of W, so that a thread's rows all have one shift, and its
+// columns, with their weights and sums in registers, are the same in all of them.
 // Columns are 32-bit numbers: a block holds at most a few thousand, longer rows
 // are cut into runs.
 #pragma once
@@ -70,59 +68,111 @@ __device__ __forceinline__ F2 row_sum2(F2 v, int lanes, F2 *sh) {
   return t;
 }
 
-// Which column element e of a thread's vector k is.
-template <int W, bool VEC>
-__device__ __forceinline__ int column(int k, int e, int lane, int lanes) {
-  return VEC ? (k * lanes + lane) * W + e : (k * W + e) * lanes + lane;
+// Four sums at once, for two rows; `sh` holds four floats per warp.
+struct F4 {
+  F2 a, b;
+};
+__device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
+  const int lane = threadIdx.x & 31;
+  const unsigned all = 0xffffffffu;
+  if (lanes < 4) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      v.a = add2(v.a, {__shfl_xor_sync(all, v.a.x, o), __shfl_xor_sync(all, v.a.y, o)});
+      v.b = add2(v.b, {__shfl_xor_sync(all, v.b.x, o), __shfl_xor_sync(all, v.b.y, o)});
+    }
+    return v;
+  }
+  const int wide = lanes < 32 ? lanes : 32, half = wide >> 1, quarter = wide >> 2;
+  const bool second = lane & half, odd = lane & quarter;
+  const F2 keep = second ? v.b : v.a, give = second ? v.a : v.b;
+  const F2 two = add2(keep, {__shfl_xor_sync(all, give.x, half), __shfl_xor_sync(all, give.y, half)});
+  float s = (odd ? two.y : two.x) + __shfl_xor_sync(all, odd ? two.x : two.y, quarter);
+  for (int o = wide >> 3; o > 0; o >>= 1) s += __shfl_xor_sync(all, s, o);
+  if (lanes <= 32) {
+    const int base = lane & ~(wide - 1);
+    return {{__shfl_sync(all, s, base), __shfl_sync(all, s, base | quarter)},
+            {__shfl_sync(all, s, base | half), __shfl_sync(all, s, base | half | quarter)}};
+  }
+  const int warp = threadIdx.x >> 5, warps = lanes >> 5;
+  if ((lane & 7) == 0) reinterpret_cast<float *>(sh + warp)[lane >> 3] = s;
+  __syncthreads();
+  const float4 *row = sh + (warp & ~(warps - 1));
+  F4 t{{0.0f, 0.0f}, {0.0f, 0.0f}};
+#pragma unroll
+  for (int q = 0; q < 16; ++q)
+    if (q < warps) {
+      const float4 f = row[q];
+      t.a = add2(t.a, {f.x, f.y});
+      t.b = add2(t.b, {f.z, f.w});
+    }
+  return t;
 }
 
-// A thread's part of a row of n columns; `rest` past the end.
+// Column of element e of vector k of a thread (relative to a run's first, where a
+// row is cut).
+template <int W, bool VEC>
+__device__ __forceinline__ int column(int k, int e, int lane, int lanes, int shift) {
+  return VEC ? (k * lanes + lane) * W + e - shift : (k * W + e) * lanes + lane;
+}
+// The part of a row that a thread has of columns low <= c < high; `rest` elsewhere.
+// `p` is column 0's address.
 template <int W, int NV, bool VEC, class T>
-__device__ __forceinline__ void load_row(const T *p, int64_t stride, int n, int lane, int lanes, float rest, float (&v)[NV][W]) {
+__device__ __forceinline__ void load_row(const T *p, int64_t stride, int low, int high, int lane, int lanes, int shift, float rest,
+                                         float (&v)[NV][W]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int j = column<W, VEC>(k, 0, lane, lanes);
-    if (VEC && j + W <= n) {
+    const int j = column<W, VEC>(k, 0, lane, lanes, shift);
+    if (VEC && j >= low && j + W <= high) {
       load_vec<W>(p + j, v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const int c = column<W, VEC>(k, e, lane, lanes);
-        v[k][e] = c < n ? to_f32(p[c * stride]) : rest;
+        const int c = column<W, VEC>(k, e, lane, lanes, shift);
+        v[k][e] = c >= low && c < high ? to_f32(p[VEC ? (int64_t)c : c * stride]) : rest;
       }
     }
   }
 }
 template <int W, int NV, bool VEC, class T>
-__device__ __forceinline__ void store_row(T *p, int64_t stride, int n, int lane, int lanes, const float (&v)[NV][W]) {
+__device__ __forceinline__ void store_row(T *p, int64_t stride, int low, int high, int lane, int lanes, int shift,
+                                          const float (&v)[NV][W]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int j = column<W, VEC>(k, 0, lane, lanes);
-    if (VEC && j + W <= n) {
+    const int j = column<W, VEC>(k, 0, lane, lanes, shift);
+    if (VEC && j >= low && j + W <= high) {
       store_vec<W>(p + j, v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const int c = column<W, VEC>(k, e, lane, lanes);
-        if (c < n) p[c * stride] = from_f32<T>(v[k][e]);
+        const int c = column<W, VEC>(k, e, lane, lanes, shift);
+        if (c >= low && c < high) p[VEC ? (int64_t)c : c * stride] = from_f32<T>(v[k][e]);
       }
     }
   }
 }
-// The same of weight or bias, elements `first` on; `rest` without one.
+// The same of one vector of weight or bias; `rest` without one.  Column 0 is
+// element `first`.
 template <int W, bool VEC>
-__device__ __forceinline__ void load_weight(const void *p, int type, int64_t first, int n, int k, int lane, int lanes,
-                                            float rest, float (&v)[W]) {
-  const int j = column<W, VEC>(k, 0, lane, lanes);
-  if (VEC && p && j + W <= n) {
+__device__ __forceinline__ void load_weight(const void *p, int type, int64_t first, int low, int high, int k, int lane, int lanes,
+                                            int shift, float rest, float (&v)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = rest;
+  if (!p) return;
+  const int j = column<W, VEC>(k, 0, lane, lanes, shift);
+  if (VEC && j >= low && j + W <= high && ((first + j) & 3) == 0 && (uintptr_t)p % 16 == 0) {
     load_kept<W>(p, type, first + j, v);
-  } else {
+    return;
+  }
+  auto each = [&](auto *q) {
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      const int c = column<W, VEC>(k, e, lane, lanes);
-      v[e] = p && c < n ? load_as_f32(p, type, first + c) : rest;
+      const int c = column<W, VEC>(k, e, lane, lanes, shift);
+      if (c >= low && c < high) v[e] = to_f32(q[first + c]);
     }
-  }
+  };
+  if (type == kF32) each(static_cast<const float *>(p));
+  else if (type == kF16) each(static_cast<const __half *>(p));
+  else each(static_cast<const __nv_bfloat16 *>(p));
 }
 
 // ---- streamed rows ------------------------------------------------------------------
@@ -143,33 +193,32 @@ __device__ __forceinline__ int row_count(int64_t i, int64_t rows, int64_t step) 
   return i < rows ? (int)((rows - i + step - 1) / step) : 0;
 }
 
-// Column of element e of vector k of a thread whose rows have `shift`.
 template <int W>
 __device__ __forceinline__ int shifted(int k, int e, int lane, int lanes, int shift) {
-  return (k * lanes + lane) * W + e - shift;
+  return column<W, true>(k, e, lane, lanes, shift);
 }
-// Bytes of vector k that a row has (from the vector's start: one that holds the
+// Elements of vector k that a row has, from the vector's start: one that holds the
 // row's start is read from there, in the same aligned 16 bytes, so in the same
-// allocation; of one that holds its end only the row's are read).
+// allocation; of one that holds its end only the row's are read.
 template <int W>
-__device__ __forceinline__ int vector_bytes(int k, int cols, int lane, int lanes, int shift, int size) {
+__device__ __forceinline__ int vector_left(int k, int cols, int lane, int lanes, int shift) {
   const int left = cols - shifted<W>(k, 0, lane, lanes, shift);
-  return (left < 0 ? 0 : left < W ? left : W) * size;
+  return left < 0 ? 0 : left < W ? left : W;
 }
 // Starts the copies of a row's vectors into a thread's slots, `PITCH` bytes apart;
 // what a vector past the row's end does not have of it becomes zero.  Slots of
 // vectors that have nothing of it are zero from the start.
 template <int W, int NV, int PITCH, class T>
-__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, const int (&bytes)[NV]) {
+__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, const int (&left)[NV]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if (bytes[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, bytes[k]);
+    if (left[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, left[k] * (int)sizeof(T));
 }
 template <int W, int NV, int PITCH, class T>
-__device__ __forceinline__ void clear_row(unsigned char *slot, const int (&bytes)[NV]) {
+__device__ __forceinline__ void clear_row(unsigned char *slot, const int (&left)[NV]) {
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if (!bytes[k]) {
+    if (!left[k]) {
 #pragma unroll
       for (int q = 0; q < W * (int)sizeof(T); q += 8) *reinterpret_cast<uint2 *>(slot + k * PITCH + q) = make_uint2(0, 0);
     }
@@ -195,7 +244,7 @@ struct Held {
 };
 template <int W, int NV>
 __device__ __forceinline__ Held held(int cols, int lane, int lanes, int shift) {
-  Held h{0, false, lane == 0 && shift > 0};
+  Held h{0, false, lane == 0 && shift > 0 && shift < W};
   bool part = false;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -219,23 +268,6 @@ template <class T>
 __device__ __forceinline__ void clear_front(unsigned char *slot, int shift) {
 #pragma unroll 1
   for (int e = 0; e < shift; ++e) reinterpret_cast<T *>(slot)[e] = from_f32<T>(0.0f);
-}
-// Weight or bias of a thread's columns; `rest` without one and past the row's ends.
-template <int W, int NV>
-__device__ __forceinline__ void stream_weight(const void *p, int type, int cols, int lane, int lanes, int shift, float rest,
-                                              float (&v)[NV][W]) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if (p && shift == 0 && (uintptr_t)p % 16 == 0 && shifted<W>(k, W, lane, lanes, 0) <= cols) {
-      load_kept<W>(p, type, shifted<W>(k, 0, lane, lanes, 0), v[k]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const int c = shifted<W>(k, e, lane, lanes, shift);
-        v[k][e] = p && c >= 0 && c < cols ? load_as_f32(p, type, c) : rest;
-      }
-    }
-  }
 }
 // A row's vectors to memory: whole ones at once, the others element by element.
 template <int W, int NV, class T>
@@ -261,6 +293,56 @@ __device__ __forceinline__ void stream_store(T *vector, const Held &have, int co
   }
 }
 
+// ---- rows longer than a block holds -----------------------------------------------------
+// They are cut into runs of kRun columns (of the row's vectors).  Two passes over
+// as many rows as L2 holds: each warp's share of a row's sums into the workspace,
+// with no barrier, then the rest of the work.  Block (run, part) takes every
+// parts-th of the rows `first` to `last`, streamed, its columns' weights in
+// registers.
+constexpr int kCutMost = 16;                // elements of a run in a thread
+constexpr int kRun = kThreads * kCutMost;
+constexpr int kCutWarps = kThreads / 32;    // shares of a run
+constexpr int kCutRows = 64;                // rows of a block at most
+
+struct Cut {
+  int64_t first, last, runs;
+  int parts;
+};
+
+// Runs at the most: a start within a vector may need one more.
+inline int64_t most_runs(int64_t cols) { return (cols + 7 + kRun - 1) / kRun; }
+// Rows of a batch at `bytes` read per column.
+inline int64_t batch_rows(int64_t rows, int64_t cols, int bytes) {
+  if (rows <= 8 || rows * cols * bytes <= (int64_t)100 << 20) return rows;
+  const int64_t fit = ((int64_t)72 << 20) / bytes / cols, batch = fit < 8 ? 8 : fit / 8 * 8;
+  return batch < rows ? batch : rows;
+}
+// Parts of a batch that give about `blocks` blocks.  A block's rows have one
+// start within a vector: where starts come around after `period` rows, parts are a
+// multiple of it, or one row each.
+inline int cut_parts(int64_t batch, int64_t runs, int blocks, int period) {
+  int64_t p = blocks / runs, least = (batch + kCutRows - 1) / kCutRows;
+  if (p < least) p = least;
+  if (period > 1) p = (p + period - 1) / period * period;
+  p = p < batch ? p : batch;
+  return (int)(p < 1 ? 1 : p);
+}
+// Rows after which starts within a vector come around.
+inline int row_period(const Rows &r, int64_t rows, int w) {
+  return rows < 2 || ((uint64_t)r.s1 % w == 0 && (rows <= r.n1 || (uint64_t)r.s0 % w == 0)) ? 1 : w;
+}
+
+// A block's place in its cut: rows i, i + parts, ..., `rows` of them, and column 0
+// relative to its first vector.
+struct CutPlace {
+  int64_t run, i;
+  int rows;
+};
+__device__ __forceinline__ CutPlace cut_place(const Cut &cut) {
+  const int64_t run = blockIdx.x % cut.runs, i = cut.first + blockIdx.x / cut.runs;
+  return {run, i, row_count(i, cut.last, cut.parts)};
+}
+
 // Rows of views that start equally far into a vector, all of them or a period
 // of w rows: where an element lies modulo w.
 inline bool same_shift(const void *p, const Rows &r, int p_size, const void *q, const Rows &t, int q_size, int64_t rows, int w) {
@@ -283,9 +365,8 @@ inline bool vec_rows(const void *p, const Rows &r, int64_t rows, int size, int w
   return r.sc == 1 && (uintptr_t)p % unit == 0 &&
          (rows < 2 || ((uint64_t)r.s1 * size % unit == 0 && (rows <= r.n1 || (uint64_t)r.s0 * size % unit == 0)));
 }
-inline bool vec_weight(const void *p) { return (uintptr_t)p % 16 == 0; }
 
-// Lanes of a row: as few as hold it at `most` elements each (`spare` of them
+// Lanes of a row: as few as hold it at `most` elements each (with `spare` more
 // for a start within a vector), which leaves a thread several loads in flight;
 // more, down to one vector each, where that leaves the GPU unfilled (a few rows:
 // latency counts).

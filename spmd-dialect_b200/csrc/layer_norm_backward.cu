@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
   float w[NV][W], sw[NV][W], sb[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    load_weight<W, false>(p.w, p.wtype, 0, cols, k, lane, lanes, 1.0f, w[k]);
+    load_weight<W, false>(p.w, p.wtype, 0, 0, cols, k, lane, lanes, 0, 1.0f, w[k]);
 #pragma unroll
     for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
   }
@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     const int n = i < p.rows ? cols : 0;
     const float mean = n ? p.mean[i] : 0.0f, rstd = n ? p.rstd[i] : 0.0f;
     float g[NV][W], x[NV][W];
-    load_row<W, NV, false>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
-    load_row<W, NV, false>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
+    load_row<W, NV, false>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, 0, n, lane, lanes, 0, 0.0f, g);
+    load_row<W, NV, false>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, 0, n, lane, lanes, 0, mean, x);
     F2 s{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -105,24 +105,29 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
-    if (n) store_row<W, NV, false>(p.dx + row_offset(p.dr, i), p.dr.sc, n, lane, lanes, g);
+    if (n) store_row<W, NV, false>(p.dx + row_offset(p.dr, i), p.dr.sc, 0, n, lane, lanes, 0, g);
   }
   if (p.part)
-    reduce_columns<W, NV>(sw, sb, lanes, cols, sums, p.part, [&](int k, int e) { return column<W, false>(k, e, lane, lanes); });
+    reduce_columns<W, NV>(sw, sb, lanes, cols, sums, p.part, [&](int k, int e) { return column<W, false>(k, e, lane, lanes, 0); });
 }
 
 // Streamed rows (layer_norm.cuh): x and dy of the next rows are on their way
-// while one is computed, its mean and rstd with them.
+// while R are computed, their mean and rstd with them.  The row's sums come first,
+// then, with x and dy read from shared memory once more, dx and the column sums:
+// holding them in registers over the reduction would leave no room for a second
+// row, whose instructions fill the reduction's waits.
 constexpr int kStages = 3;
+template <class TX, class TY>
+constexpr int kRowsAtOnce = sizeof(TX) + sizeof(TY) <= 6 ? 2 : 1;  // as two blocks' stages fit an SM
 
-template <class TX, class TY, int W, int NV, int MAXT>
+template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3)
 ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
                    const __grid_constant__ RowWalk dr, int lanes) {
-  constexpr int kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * MAXT * (kXBytes + kGBytes);
+  constexpr int kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kRow = NV * MAXT * (kXBytes + kGBytes), kStage = R * kRow;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(16) F2 sh[2][32];
-  __shared__ float2 stats[kStages][MAXT];  // a group's row, or a warp's where the group is wider
+  __shared__ __align__(16) float4 sh[2][32];
+  __shared__ float2 stats[STAGES * R][MAXT];  // a group's row, or a warp's where the group is wider
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols, slot = lanes <= 32 ? group : threadIdx.x >> 5;
   const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
@@ -136,84 +141,108 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   TX *to = p.dx + (mine && p.dx ? row_offset(dr.r, i) : 0) + start;
   x_from += start;
   const Held have = held<W, NV>(cols, lane, lanes, shift);
-  int x_bytes[NV], g_bytes[NV];
+  int left[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    x_bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TX));
-    g_bytes[k] = vector_bytes<W>(k, cols, lane, lanes, shift, sizeof(TY));
-  }
+  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
   unsigned char *const x_slots = smem + threadIdx.x * kXBytes, *const g_slots = smem + NV * MAXT * kXBytes + threadIdx.x * kGBytes;
 #pragma unroll
-  for (int q = 0; q < kStages; ++q) {
-    clear_row<W, NV, MAXT * kXBytes, TX>(x_slots + q * kStage, x_bytes);
-    clear_row<W, NV, MAXT * kGBytes, TY>(g_slots + q * kStage, g_bytes);
+  for (int q = 0; q < STAGES * R; ++q) {
+    clear_row<W, NV, MAXT * kXBytes, TX>(x_slots + q * kRow, left);
+    clear_row<W, NV, MAXT * kGBytes, TY>(g_slots + q * kRow, left);
   }
   int stage_in = 0, stage = 0, fetched = 0;
+  const float *mean_in = p.mean + i, *rstd_in = p.rstd + i;
   auto fetch = [&] {
-    if (fetched < mine) {
-      stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage, x_from, lanes, x_bytes);
-      stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage, g_from, lanes, g_bytes);
-      if (first) {
-        copy_async<4>(&stats[stage_in][slot].x, p.mean + (i + fetched * step));
-        copy_async<4>(&stats[stage_in][slot].y, p.rstd + (i + fetched * step));
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (fetched < mine) {
+        stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage + q * kRow, x_from, lanes, left);
+        stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage + q * kRow, g_from, lanes, left);
+        if (first) {
+          copy_async<4>(&stats[stage_in * R + q][slot].x, mean_in);
+          copy_async<4>(&stats[stage_in * R + q][slot].y, rstd_in);
+        }
       }
+      ++fetched;
+      mean_in += step, rstd_in += step;
+      x_from = next_row(x_from, p.x + start, xr, i + fetched * step);
+      g_from = next_row(g_from, p.dy + start, gr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
-    ++fetched;
-    x_from = next_row(x_from, p.x + start, xr, i + fetched * step);
-    g_from = next_row(g_from, p.dy + start, gr, i + fetched * step);
-    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
   };
 #pragma unroll
-  for (int q = 0; q < kStages - 1; ++q) fetch();
+  for (int q = 0; q < STAGES - 1; ++q) fetch();
   float w[NV][W];
   F2 sw[NV][W / 2], sb[NV][W / 2];
-  stream_weight<W, NV>(p.w, p.wtype, cols, lane, lanes, shift, 1.0f, w);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) load_weight<W, true>(p.w, p.wtype, 0, 0, cols, k, lane, lanes, shift, 1.0f, w[k]);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < W / 2; ++e) sw[k][e] = sb[k][e] = {0.0f, 0.0f};
-  for (int turn = 0; turn < turns; ++turn) {
+  for (int turn = 0; turn < turns; turn += R) {
     fetch();
-    copy_wait<kStages - 1>();
+    copy_wait<STAGES - 1>();
     __syncwarp();  // the first lane's copies are there too
-    const bool live = turn < mine;
-    const float2 stat = stats[stage][slot];
-    F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f}, g[NV][W / 2], x[NV][W / 2];
-    if (live) {
-      // An element outside the row has g = 0 and a finite x, and adds nothing to any sum.
-      unsigned char *const xs = x_slots + stage * kStage, *const gs = g_slots + stage * kStage;
+    float2 stat[R];
+    F2 c[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      // An element outside the row, or of a row past the last, has g = 0 and a finite x: it adds nothing to any sum.
+      const bool live = turn + q < mine;
+      unsigned char *const xs = x_slots + stage * kStage + q * kRow, *const gs = g_slots + stage * kStage + q * kRow;
+      stat[q] = live ? stats[stage * R + q][slot] : make_float2(0.0f, 0.0f);
       if (have.front) {
         clear_front<TX>(xs, shift);
         clear_front<TY>(gs, shift);
       }
+      F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x[k]);
-        take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g[k]);
+        F2 x[W / 2], g[W / 2];
+        take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x);
+        take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g);
 #pragma unroll
         for (int e = 0; e < W / 2; ++e) {
-          x[k][e] = mul2(add2(x[k][e], both(-stat.x)), both(stat.y));
-          sw[k][e] = fma2(g[k][e], x[k][e], sw[k][e]);
-          sb[k][e] = add2(g[k][e], sb[k][e]);
-          g[k][e] = mul2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]});
-          s1 = add2(s1, g[k][e]);
-          s2 = fma2(g[k][e], x[k][e], s2);
+          const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
+          s1 = add2(s1, a);
+          s2 = fma2(a, mul2(add2(x[e], both(-stat[q].x)), both(stat[q].y)), s2);
         }
       }
+      c[q] = {s1.x + s1.y, s2.x + s2.y};
     }
     __syncwarp();  // every lane has its statistics: the slot may be filled again
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (!p.dx) continue;
-    const F2 c = mul2(row_sum2({s1.x + s1.y, s2.x + s2.y}, lanes, sh[turn & 1]), both(-inv_n));
-    if (live) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < W / 2; ++e) g[k][e] = mul2(fma2(x[k][e], both(c.y), add2(g[k][e], both(c.x))), both(stat.y));
-      stream_store<W, NV>(to, have, cols, lane, lanes, shift, g);
+    if constexpr (R == 2) {
+      const F4 t = row_sum4({c[0], c[1]}, lanes, sh[(turn / R) & 1]);
+      c[0] = t.a, c[1] = t.b;
+    } else {
+      c[0] = row_sum2(c[0], lanes, reinterpret_cast<F2 *>(sh[turn & 1]));
     }
-    to = next_row(to, p.dx + start, dr, i + (turn + 1) * step);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (turn + q < mine) {
+        const F2 c1 = both(-c[q].x * inv_n), c2 = both(-c[q].y * inv_n);
+        unsigned char *const xs = x_slots + stage * kStage + q * kRow, *const gs = g_slots + stage * kStage + q * kRow;
+        F2 g[NV][W / 2];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          F2 x[W / 2];
+          take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x);
+          take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g[k]);
+#pragma unroll
+          for (int e = 0; e < W / 2; ++e) {
+            const F2 xh = mul2(add2(x[e], both(-stat[q].x)), both(stat[q].y));
+            sw[k][e] = fma2(g[k][e], xh, sw[k][e]);
+            sb[k][e] = add2(g[k][e], sb[k][e]);
+            g[k][e] = mul2(fma2(xh, c2, fma2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]}, c1)), both(stat[q].y));
+          }
+        }
+        if (p.dx) stream_store<W, NV>(to, have, cols, lane, lanes, shift, g);
+      }
+      to = next_row(to, p.dx + start, dr, i + (turn + q + 1) * step);
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   copy_wait<0>();
   if (p.part) {
@@ -230,90 +259,291 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   }
 }
 
-// Longer rows, first pass: the two sums of each run of kRun columns of a row.
-constexpr int kRun = kThreads * kMost;
+// Longer rows (layer_norm.cuh), first pass: each warp's share of a row's two sums.
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kThreads, 2)
+ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
+          const __grid_constant__ Cut cut, float2 *shares) {
+  constexpr int NV = kCutMost / W, kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * kThreads * (kXBytes + kGBytes);
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float2 stats[kCutRows];
+  const CutPlace at = cut_place(cut);
+  if (at.rows == 0) return;
+  const int lane = threadIdx.x;
+  for (int r = lane; r < at.rows; r += kThreads) stats[r] = make_float2(-p.mean[at.i + (int64_t)r * cut.parts], p.rstd[at.i + (int64_t)r * cut.parts]);
+  const TX *x_from = p.x + row_offset(xr.r, at.i);
+  const int64_t first = at.run * kRun;
+  const int begin = (int)((uintptr_t)x_from / sizeof(TX) % W);
+  const int low = at.run == 0 ? 0 : -begin, high = p.cols - first < kRun - begin ? (int)(p.cols - first) : kRun - begin;
+  const int shift = at.run == 0 ? begin : 0, n = high - low;
+  const int64_t start = first + low + lane * W - shift;
+  const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
+  x_from += start;
+  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  int left[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
+  unsigned char *const x_slots = smem + lane * kXBytes, *const g_slots = smem + NV * kThreads * kXBytes + lane * kGBytes;
+#pragma unroll
+  for (int q = 0; q < kStages; ++q) {
+    clear_row<W, NV, kThreads * kXBytes, TX>(x_slots + q * kStage, left);
+    clear_row<W, NV, kThreads * kGBytes, TY>(g_slots + q * kStage, left);
+  }
+  int stage_in = 0, stage = 0, fetched = 0;
+  auto fetch = [&] {
+    if (fetched < at.rows) {
+      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, left);
+      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, left);
+    }
+    copy_commit();
+    ++fetched;
+    x_from = next_row(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
+  };
+#pragma unroll
+  for (int q = 0; q < kStages - 1; ++q) fetch();
+  float w[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
+  __syncthreads();
+  for (int turn = 0; turn < at.rows; ++turn) {
+    fetch();
+    copy_wait<kStages - 1>();
+    const float2 stat = stats[turn];
+    if (have.front) {
+      clear_front<TX>(x_slots + stage, shift);
+      clear_front<TY>(g_slots + stage, shift);
+    }
+    F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      F2 x[W / 2], g[W / 2];
+      take_pairs<W, TX>(x_slots + stage + k * (kThreads * kXBytes), x);
+      take_pairs<W, TY>(g_slots + stage + k * (kThreads * kGBytes), g);
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
+        s1 = add2(s1, a);
+        s2 = fma2(a, mul2(add2(x[e], both(stat.x)), both(stat.y)), s2);
+      }
+    }
+    stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
+    const F2 s = row_sum2({s1.x + s1.y, s2.x + s2.y}, 32, nullptr);
+    if ((lane & 31) == 0)
+      shares[((at.i - cut.first + (int64_t)turn * cut.parts) * cut.runs + at.run) * kCutWarps + (lane >> 5)] = make_float2(s.x, s.y);
+  }
+  copy_wait<0>();
+}
 
-template <class TX, class TY, int W, bool VEC>
-__global__ void __launch_bounds__(kThreads) ln_row_sums(const __grid_constant__ Back<TX, TY> p, float2 *run_sums, int64_t runs) {
-  constexpr int NV = kMost / W;
-  __shared__ float sh[2][2][32];
-  int turn = 0;
-  for (int64_t item = blockIdx.x; item < p.rows * runs; item += gridDim.x, turn ^= 1) {
-    const int64_t i = item / runs, first = (item - i * runs) * kRun;
-    const int n = p.cols - first < kRun ? (int)(p.cols - first) : kRun;
+// Second pass: dx and the column sums, which go on from what the batches before
+// left in the part's partial row.
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kThreads, 2)
+ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
+         const __grid_constant__ RowWalk dr, const __grid_constant__ Cut cut, const float2 *shares) {
+  constexpr int NV = kCutMost / W, kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * kThreads * (kXBytes + kGBytes);
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float4 stats[kCutRows];  // -mean, rstd, -c1, -c2
+  const CutPlace at = cut_place(cut);
+  if (at.rows == 0) return;
+  const int lane = threadIdx.x;
+  const float inv_n = 1.0f / (float)p.cols;
+  const TX *x_from = p.x + row_offset(xr.r, at.i);
+  const int64_t first = at.run * kRun, part = blockIdx.x / cut.runs;
+  const int begin = (int)((uintptr_t)x_from / sizeof(TX) % W);
+  const int low = at.run == 0 ? 0 : -begin, high = p.cols - first < kRun - begin ? (int)(p.cols - first) : kRun - begin;
+  const int shift = at.run == 0 ? begin : 0, n = high - low;
+  const int64_t start = first + low + lane * W - shift;
+  const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
+  TX *to = p.dx + (p.dx ? row_offset(dr.r, at.i) : 0) + start;
+  x_from += start;
+  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  int left[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
+  unsigned char *const x_slots = smem + lane * kXBytes, *const g_slots = smem + NV * kThreads * kXBytes + lane * kGBytes;
+#pragma unroll
+  for (int q = 0; q < kStages; ++q) {
+    clear_row<W, NV, kThreads * kXBytes, TX>(x_slots + q * kStage, left);
+    clear_row<W, NV, kThreads * kGBytes, TY>(g_slots + q * kStage, left);
+  }
+  int stage_in = 0, stage = 0, fetched = 0;
+  auto fetch = [&] {
+    if (fetched < at.rows) {
+      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, left);
+      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, left);
+    }
+    copy_commit();
+    ++fetched;
+    x_from = next_row(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
+  };
+#pragma unroll
+  for (int q = 0; q < kStages - 1; ++q) fetch();
+  float *const part_w = p.part + 2 * part * p.cols + first + low, *const part_b = part_w + p.cols;
+  float w[NV][W];
+  F2 sw[NV][W / 2], sb[NV][W / 2];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
+    float tw[W], tb[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int c = shifted<W>(k, e, lane, kThreads, shift);
+      const bool goes_on = p.part && cut.first > 0 && c >= 0 && c < n;
+      tw[e] = goes_on ? part_w[c] : 0.0f;
+      tb[e] = goes_on ? part_b[c] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < W / 2; ++e) sw[k][e] = {tw[2 * e], tw[2 * e + 1]}, sb[k][e] = {tb[2 * e], tb[2 * e + 1]};
+  }
+  for (int r = lane >> 5; r < at.rows; r += kCutWarps) {  // a warp a row, in one order
+    const int64_t i = at.i + (int64_t)r * cut.parts;
+    float c1 = 0.0f, c2 = 0.0f;
+    if (p.dx)
+      for (int64_t q = lane & 31; q < cut.runs * kCutWarps; q += 32) {
+        const float2 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
+        c1 += s.x;
+        c2 += s.y;
+      }
+    c1 = warp_sum_f32(c1);
+    c2 = warp_sum_f32(c2);
+    if ((lane & 31) == 0) stats[r] = make_float4(-p.mean[i], p.rstd[i], -c1 * inv_n, -c2 * inv_n);
+  }
+  __syncthreads();
+  for (int turn = 0; turn < at.rows; ++turn) {
+    fetch();
+    copy_wait<kStages - 1>();
+    const float4 stat = stats[turn];
+    if (have.front) {
+      clear_front<TX>(x_slots + stage, shift);
+      clear_front<TY>(g_slots + stage, shift);
+    }
+    F2 g[NV][W / 2];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      F2 x[W / 2];
+      take_pairs<W, TX>(x_slots + stage + k * (kThreads * kXBytes), x);
+      take_pairs<W, TY>(g_slots + stage + k * (kThreads * kGBytes), g[k]);
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        const F2 xh = mul2(add2(x[e], both(stat.x)), both(stat.y));
+        sw[k][e] = fma2(g[k][e], xh, sw[k][e]);
+        sb[k][e] = add2(g[k][e], sb[k][e]);
+        g[k][e] = mul2(fma2(xh, both(stat.w), fma2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]}, both(stat.z))), both(stat.y));
+      }
+    }
+    stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
+    if (p.dx) stream_store<W, NV>(to, have, n, lane, kThreads, shift, g);
+    to = next_row(to, p.dx + start, dr, at.i + (int64_t)(turn + 1) * cut.parts);
+  }
+  copy_wait<0>();
+  if (!p.part) return;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int c = shifted<W>(k, e, lane, kThreads, shift);
+      if (c >= 0 && c < n) {
+        part_w[c] = e & 1 ? sw[k][e / 2].y : sw[k][e / 2].x;
+        part_b[c] = e & 1 ? sb[k][e / 2].y : sb[k][e / 2].x;
+      }
+    }
+}
+
+// Longer rows of any strides, the same two passes with single elements and one
+// share a block.
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kThreads, 2) ln_strided_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ Cut cut, float2 *shares) {
+  constexpr int NV = kCutMost / W;
+  __shared__ __align__(16) F2 sh[2][32];
+  const CutPlace at = cut_place(cut);
+  const int64_t first = at.run * kRun;
+  const int n = p.cols - first < kRun ? (p.cols > first ? (int)(p.cols - first) : 0) : kRun;
+  for (int turn = 0; turn < at.rows; ++turn) {
+    const int64_t i = at.i + (int64_t)turn * cut.parts;
     const float mean = p.mean[i], rstd = p.rstd[i];
     float g[NV][W], x[NV][W];
-    load_row<W, NV, VEC>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
-    load_row<W, NV, VEC>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
-    float s1 = 0.0f, s2 = 0.0f;
+    load_row<W, NV, false>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, 0, n, threadIdx.x, kThreads, 0, 0.0f, g);
+    load_row<W, NV, false>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, 0, n, threadIdx.x, kThreads, 0, mean, x);
+    F2 s{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float w[W];
-      load_weight<W, VEC>(p.w, p.wtype, first, n, k, threadIdx.x, kThreads, 1.0f, w);
+      load_weight<W, false>(p.w, p.wtype, first, 0, n, k, threadIdx.x, kThreads, 0, 1.0f, w);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const float a = g[k][e] * w[e];
-        s1 += a;
-        s2 = fmaf(a, (x[k][e] - mean) * rstd, s2);
+        s.x += a;
+        s.y = fmaf(a, (x[k][e] - mean) * rstd, s.y);
       }
     }
-    s1 = row_sum(s1, kThreads, sh[turn][0]);
-    s2 = row_sum(s2, kThreads, sh[turn][1]);
-    if (threadIdx.x == 0) run_sums[item] = make_float2(s1, s2);
+    s = row_sum2(s, kThreads, sh[turn & 1]);
+    if (threadIdx.x < kCutWarps)
+      shares[((i - cut.first) * cut.runs + at.run) * kCutWarps + threadIdx.x] = threadIdx.x ? make_float2(0.0f, 0.0f) : make_float2(s.x, s.y);
   }
 }
 
-// Second pass: block (run, part) takes kRun columns of the part's rows, writes
-// dx and keeps the column sums.  x and dy come from L2 where they fit there.
-template <class TX, class TY, int W, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-ln_row_grads(const __grid_constant__ Back<TX, TY> p, const float2 *run_sums, int64_t runs, int parts) {
-  constexpr int NV = kMost / W;
-  const int64_t run = blockIdx.x % runs, part = blockIdx.x / runs, first = run * kRun;
-  const int n = p.cols - first < kRun ? (int)(p.cols - first) : kRun;
+template <class TX, class TY, int W>
+__global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ Cut cut, const float2 *shares) {
+  constexpr int NV = kCutMost / W;
+  const CutPlace at = cut_place(cut);
+  if (at.rows == 0) return;
+  const int64_t first = at.run * kRun, part = blockIdx.x / cut.runs;
+  const int n = p.cols - first < kRun ? (p.cols > first ? (int)(p.cols - first) : 0) : kRun;
   const float inv_n = 1.0f / (float)p.cols;
-  float w[NV][W], sw[NV][W], sb[NV][W];
+  float *const part_w = p.part + 2 * part * p.cols + first, *const part_b = part_w + p.cols;
+  float sw[NV][W], sb[NV][W];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    load_weight<W, VEC>(p.w, p.wtype, first, n, k, threadIdx.x, kThreads, 1.0f, w[k]);
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int e = 0; e < W; ++e) sw[k][e] = sb[k][e] = 0.0f;
-  }
-  for (int64_t i = part; i < p.rows; i += parts) {
+    for (int e = 0; e < W; ++e) {
+      const int c = column<W, false>(k, e, threadIdx.x, kThreads, 0);
+      const bool goes_on = p.part && cut.first > 0 && c < n;
+      sw[k][e] = goes_on ? part_w[c] : 0.0f;
+      sb[k][e] = goes_on ? part_b[c] : 0.0f;
+    }
+  for (int turn = 0; turn < at.rows; ++turn) {
+    const int64_t i = at.i + (int64_t)turn * cut.parts;
     const float mean = p.mean[i], rstd = p.rstd[i];
-    float g[NV][W], x[NV][W];
-    load_row<W, NV, VEC>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
-    load_row<W, NV, VEC>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
     float c1 = 0.0f, c2 = 0.0f;
-    if (p.dx) {  // every warp adds up the row's runs for itself, in one order
-      for (int64_t q = threadIdx.x & 31; q < runs; q += 32) {
-        const float2 s = run_sums[i * runs + q];
+    if (p.dx) {  // every warp adds up the row's shares for itself, in one order
+      for (int64_t q = threadIdx.x & 31; q < cut.runs * kCutWarps; q += 32) {
+        const float2 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
         c1 += s.x;
         c2 += s.y;
       }
       c1 = warp_sum_f32(c1) * inv_n;
       c2 = warp_sum_f32(c2) * inv_n;
     }
+    float g[NV][W], x[NV][W];
+    load_row<W, NV, false>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, 0, n, threadIdx.x, kThreads, 0, 0.0f, g);
+    load_row<W, NV, false>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, 0, n, threadIdx.x, kThreads, 0, mean, x);
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      float w[W];
+      load_weight<W, false>(p.w, p.wtype, first, 0, n, k, threadIdx.x, kThreads, 0, 1.0f, w);
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const float xh = (x[k][e] - mean) * rstd;
         sw[k][e] = fmaf(g[k][e], xh, sw[k][e]);
         sb[k][e] += g[k][e];
-        g[k][e] = (g[k][e] * w[k][e] - c1 - xh * c2) * rstd;
+        g[k][e] = (g[k][e] * w[e] - c1 - xh * c2) * rstd;
       }
-    if (p.dx) store_row<W, NV, VEC>(p.dx + row_offset(p.dr, i) + first * p.dr.sc, p.dr.sc, n, threadIdx.x, kThreads, g);
+    }
+    if (p.dx) store_row<W, NV, false>(p.dx + row_offset(p.dr, i) + first * p.dr.sc, p.dr.sc, 0, n, threadIdx.x, kThreads, 0, g);
   }
   if (!p.part) return;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      const int c = column<W, VEC>(k, e, threadIdx.x, kThreads);
+      const int c = column<W, false>(k, e, threadIdx.x, kThreads, 0);
       if (c < n) {
-        p.part[2 * part * p.cols + first + c] = sw[k][e];
-        p.part[(2 * part + 1) * p.cols + first + c] = sb[k][e];
+        part_w[c] = sw[k][e];
+        part_b[c] = sb[k][e];
       }
     }
 }
@@ -344,18 +574,13 @@ ln_finish(const float *__restrict__ part, int parts, int64_t cols, void *dw, voi
 }
 
 // ---- launches ---------------------------------------------------------------------
-// Partial rows of the column sums for rows that a block holds, and for longer
-// ones: there, few parts of few rows each, so that blocks fill the GPU.
+// Partial rows of the column sums for rows that a block holds.
 int held_parts(int64_t rows, int groups) {
   const int64_t p = (rows + groups - 1) / groups;
   return (int)(p < 1 ? 1 : p < kMaxParts ? p : kMaxParts);
 }
-int64_t long_runs(int64_t cols) { return (cols + kRun - 1) / kRun; }
-int long_parts(int64_t rows, int64_t cols) {
-  const int64_t most = (4 * kMaxParts + long_runs(cols) - 1) / long_runs(cols);
-  const int64_t p = rows < most ? rows : most;
-  return (int)(p < 1 ? 1 : p);
-}
+// Blocks of the two passes over longer rows.
+constexpr int kShareBlocks = 592, kGradBlocks = 296;
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 template <class TX, class TY, int NV, int MAXT>
@@ -367,9 +592,10 @@ cudaError_t backward_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStre
 
 template <class TX, class TY, int NV, int MAXT>
 cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, staged = kStages * NV * MAXT * W * (int)(sizeof(TX) + sizeof(TY));
+  constexpr int W = kWidth<TX, TY>, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;
+  constexpr int staged = stages * R * NV * MAXT * W * (int)(sizeof(TX) + sizeof(TY));
   const int sums = b.part ? (int)(MAXT / lanes * b.cols * sizeof(float)) : 0, bytes = staged > sums ? staged : sums;
-  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT>;
+  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
   const int64_t groups = MAXT / lanes;
   const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
@@ -379,33 +605,52 @@ cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream
   return cudaGetLastError();
 }
 
-template <class TX, class TY, bool VEC>
-cudaError_t backward_long(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>;
-  const int64_t runs = long_runs(b.cols);
-  *parts = long_parts(b.rows, b.cols);
-  float2 *run_sums = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)*parts * 2 * b.cols * sizeof(float)));
-  if (b.dx) {
-    ln_row_sums<TX, TY, W, VEC><<<grid_for(b.rows * runs), kThreads, 0, s>>>(b, run_sums, runs);
+template <class TX, class TY>
+cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, bool vectors, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, bytes = kStages * kRun * (int)(sizeof(TX) + sizeof(TY));
+  auto shares_of = ln_shares<TX, TY, W>;
+  auto grads_of = ln_grads<TX, TY, W>;
+  if (vectors) {
+    if (cudaError_t e = cudaFuncSetAttribute(shares_of, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    if (cudaError_t e = cudaFuncSetAttribute(grads_of, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  }
+  const int64_t runs = most_runs(b.cols), batch = batch_rows(b.rows, b.cols, sizeof(TX) + sizeof(TY));
+  const int period = vectors ? row_period(b.xr, b.rows, W) : 1;
+  const int parts1 = cut_parts(batch, runs, kShareBlocks, period), parts2 = cut_parts(batch, runs, kGradBlocks, period);
+  float2 *shares = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)parts2 * 2 * b.cols * sizeof(float)));
+  *parts = parts2;
+  for (int64_t row = 0; row < b.rows; row += batch) {
+    const int64_t last = row + batch < b.rows ? row + batch : b.rows;
+    const Cut cut1{row, last, runs, parts1}, cut2{row, last, runs, parts2};
+    const unsigned grid1 = grid_for(runs * parts1), grid2 = grid_for(runs * parts2);
+    if (b.dx) {
+      if (vectors)
+        shares_of<<<grid1, kThreads, bytes, s>>>(b, row_walk(b.gr, b.rows, parts1), row_walk(b.xr, b.rows, parts1), cut1, shares);
+      else
+        ln_strided_shares<TX, TY, W><<<grid1, kThreads, 0, s>>>(b, cut1, shares);
+      if (cudaError_t e = cudaGetLastError()) return e;
+    }
+    if (vectors)
+      grads_of<<<grid2, kThreads, bytes, s>>>(b, row_walk(b.gr, b.rows, parts2), row_walk(b.xr, b.rows, parts2),
+                                              row_walk(b.dr, b.rows, parts2), cut2, shares);
+    else
+      ln_strided_grads<TX, TY, W><<<grid2, kThreads, 0, s>>>(b, cut2, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
-  ln_row_grads<TX, TY, W, VEC><<<grid_for(runs * *parts), kThreads, 0, s>>>(b, run_sums, runs, *parts);
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 template <class TX, class TY>
 cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W;
-  const bool even = vec_rows(b.x, b.xr, b.rows, sizeof(TX), W) && vec_rows(b.dy, b.gr, b.rows, sizeof(TY), W) &&
-                    (!b.dx || vec_rows(b.dx, b.dr, b.rows, sizeof(TX), W));
-  const int spare = even ? 0 : W - 1;
-  if (b.cols > kHeld - spare)
-    return even && vec_weight(b.w) ? backward_long<TX, TY, true>(b, ws, parts, s) : backward_long<TX, TY, false>(b, ws, parts, s);
+  const bool vectors = b.xr.sc == 1 && b.gr.sc == 1 && (!b.dx || b.dr.sc == 1) &&
+                       same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
+                       (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W));
+  const int spare = vectors && !vec_rows(b.x, b.xr, b.rows, sizeof(TX), W) ? W - 1 : 0;
+  if (b.cols > kHeld - spare) return backward_cut<TX, TY>(b, ws, vectors, parts, s);
   const bool wide = b.cols + spare > kThreads * kMost;
   const int lanes = wide ? kWideLanes : row_lanes(b.rows, b.cols, W, kMost, spare), nv = row_vectors(b.cols + spare, lanes, W);
-  if (b.xr.sc == 1 && b.gr.sc == 1 && (!b.dx || b.dr.sc == 1) &&
-      same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
-      (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W))) {
+  if (vectors) {
     if (wide) return stream_rows<TX, TY, NV, kWideLanes>(b, lanes, parts, s);
     if (nv == 1) return stream_rows<TX, TY, 1, kThreads>(b, lanes, parts, s);
     if (nv < NV) return stream_rows<TX, TY, 2, kThreads>(b, lanes, parts, s);
@@ -435,11 +680,13 @@ cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
 
 size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   // Rows a few columns short of what a block holds may take either way, as their addresses have it.
-  const size_t held = cols <= kHeld ? (size_t)held_parts(rows, 1) * 2 * (size_t)cols * sizeof(float) : 0;
-  if (cols <= kHeld - 7) return held;
-  const size_t cut = round16((size_t)long_parts(rows, cols) * 2 * (size_t)cols * sizeof(float)) +
-                     (size_t)rows * (size_t)long_runs(cols) * sizeof(float2);
-  return held > cut ? held : cut;
+  const size_t whole = cols <= kHeld ? (size_t)held_parts(rows, 1) * 2 * (size_t)cols * sizeof(float) : 0;
+  if (cols <= kHeld - 7) return whole;
+  // The fewest bytes an element leave the most rows to a batch; parts grow with rows and the period.
+  const int64_t runs = most_runs(cols), batch = batch_rows(rows, cols, 4);
+  const size_t cut = round16((size_t)cut_parts(batch, runs, kGradBlocks, 8) * 2 * (size_t)cols * sizeof(float)) +
+                     (size_t)batch * (size_t)runs * kCutWarps * sizeof(float2);
+  return whole > cut ? whole : cut;
 }
 
 cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s) {

@@ -8,6 +8,7 @@ All compute happens in libspmdb200.so; nothing here computes anything.
 from __future__ import annotations
 
 import ctypes
+import math
 from array import array
 
 import torch
@@ -282,16 +283,17 @@ def _norm_types(x: torch.Tensor, y: torch.dtype) -> None:
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5, dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
-               stats: bool = True, stream=None):
+               stats: bool = True, ws: torch.Tensor | None = None, stream=None):
     """(out, mean, rstd): layer norm over the last dimension, out = (x - mean) *
     rstd * weight + bias.  x is any strided view; out has `dtype` (default
     x's; one of the two may be float32) and may be x itself.  mean and rstd
     (float32, x's leading shape) are what layer_norm_backward takes; stats=False
-    leaves them out (None)."""
+    leaves them out (None).  Rows of more than 8185 elements use a workspace of
+    layer_norm_workspace(rows, cols, backward=False)."""
     dev = x.get_device()
     if _elsewhere(dev, stream):
         with _at(dev, stream):
-            return layer_norm(x, weight, bias, eps, dtype, out, stats)
+            return layer_norm(x, weight, bias, eps, dtype, out, stats, ws)
     shape = x.shape
     if not shape:
         raise ValueError("layer_norm: x needs a dimension to normalise over")
@@ -313,18 +315,30 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         rstd = torch.empty_like(mean)
         m, r = mean.data_ptr(), rstd.data_ptr()
     xv, ov = _norm_rows("x", x), _norm_rows("out", out)
-    rank = xv.dim()
+    rank, room, room_bytes = xv.dim(), None, 0
+    if ws is not None or shape[-1] > 8185:
+        ws = _norm_room(ws, math.prod(shape[:-1]), shape[-1], x, False)
+        room, room_bytes = ws.data_ptr(), ws.nbytes
     dims = array("q", (*xv.shape, *xv.stride(), *ov.stride()))
     at = _ptr(dims)
     call("spmdb200_layer_norm", rank, at, xv.data_ptr(), _TYPES[x.dtype], at + 8 * rank, ov.data_ptr(),
-         _TYPES[out.dtype], at + 16 * rank, w, b, wtype, eps, m, r, _raw_stream(dev))
+         _TYPES[out.dtype], at + 16 * rank, w, b, wtype, eps, m, r, room, room_bytes, _raw_stream(dev))
     return out, mean, rstd
 
 
-def layer_norm_workspace(rows: int, cols: int, device=None) -> torch.Tensor:
-    """Workspace for layer_norm_backward (contents irrelevant, reusable)."""
-    nbytes = int(lib().spmdb200_layer_norm_workspace_bytes(rows, cols))
-    return torch.empty(nbytes, dtype=torch.uint8, device=device or "cuda")
+def layer_norm_workspace(rows: int, cols: int, device=None, backward: bool = True) -> torch.Tensor:
+    """Workspace for layer_norm_backward, or for layer_norm (contents irrelevant,
+    reusable; calls that share it must not overlap on the GPU)."""
+    size = lib().spmdb200_layer_norm_workspace_bytes if backward else lib().spmdb200_layer_norm_forward_workspace_bytes
+    return torch.empty(size(rows, cols), dtype=torch.uint8, device=device or "cuda")
+
+
+def _norm_room(ws: torch.Tensor | None, rows: int, cols: int, x: torch.Tensor, backward: bool) -> torch.Tensor:
+    if ws is None:
+        return layer_norm_workspace(rows, cols, x.device, backward)
+    if ws.get_device() != x.get_device() or not ws.is_contiguous():
+        raise ValueError("layer_norm: ws is a contiguous tensor on x's device")
+    return ws
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -368,10 +382,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     else:
         _norm_operand("dx", dx, shape, dev, x.dtype)
     gv, xv, dv = _norm_rows("dy", dy), _norm_rows("x", x), _norm_rows("dx", dx)
-    if ws is None:
-        ws = layer_norm_workspace(mean.numel(), shape[-1], x.device)
-    elif ws.get_device() != dev or not ws.is_contiguous():
-        raise ValueError("layer_norm: ws is a contiguous tensor on x's device")
+    ws = _norm_room(ws, mean.numel(), shape[-1], x, True)
     rank = xv.dim()
     dims = array("q", (*xv.shape, *gv.stride(), *xv.stride(), *dv.stride()))
     at = _ptr(dims)

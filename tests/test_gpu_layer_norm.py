@@ -79,6 +79,31 @@ def test_row_counts(kernels, rows, cols):
     check_backward(kernels, dy, x, w, stats=(mean, rstd))
 
 
+@pytest.mark.parametrize("rows,cols", [(700, 60001), (1500, 20000), (9, 4000001), (40, 1500000), (5000, 8190)])
+def test_long_rows_in_batches(kernels, rows, cols):
+    """More long rows than one batch holds: statistics and sums go on from batch to batch."""
+    x, dy = make((rows, cols), BF16, rows), make((rows, cols), BF16, rows + 1)
+    w, b = weights(cols, F32, 2)
+    y, mean, rstd = kernels.layer_norm(x, w, b)
+    dx, dw, db = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+    tw, tb = (torch.zeros(cols, device="cuda", dtype=torch.float64) for _ in range(2))
+    aw, ab = torch.zeros_like(tw), torch.zeros_like(tb)
+    for i in range(0, rows, 64):
+        s = slice(i, i + 64)
+        want, m, r, e_m, e_r, e_y = norm_ref(x[s], w, b, EPS)
+        assert_within(mean[s], m, e_m, "mean")
+        assert_within(rstd[s], r, e_r, "rstd")
+        assert_within(y[s], want, e_y + rounded(want.abs() + e_y, BF16), "y")
+        ref = norm_back_ref(dy[s], x[s], mean[s], rstd[s], w)
+        assert_within(dx[s], ref[0], ref[3] + rounded(ref[0].abs() + ref[3], BF16), "dx")
+        tw += ref[1]
+        tb += ref[2]
+        aw += ref[4] / (min(64, rows - i) + 20)
+        ab += ref[5] / (min(64, rows - i) + 16)
+    assert_within(dw, tw, (rows + 20) * aw + rounded(tw.abs(), F32), "dweight")
+    assert_within(db, tb, (rows + 16) * ab + rounded(tb.abs(), F32), "dbias")
+
+
 @pytest.mark.parametrize("x_t,y_t", PAIRS)
 @pytest.mark.parametrize("w_t", [None, F32, F16, BF16])
 def test_types(kernels, x_t, y_t, w_t):
@@ -182,6 +207,10 @@ def test_no_rows(kernels):
     assert dx.shape == (0, 100) and bool((dw == 0).all()) and bool((db == 0).all())
     y, _, _ = kernels.layer_norm(torch.empty((3, 0, 100), device="cuda"), w, b)
     assert y.shape == (3, 0, 100)
+    x, (w, b) = torch.empty((0, 30000), device="cuda"), weights(30000, F32, 1)
+    y, mean, rstd = kernels.layer_norm(x, w, b)
+    _, dw, db = kernels.layer_norm_backward(x, x, mean, rstd, w)
+    assert y.shape == (0, 30000) and bool((dw == 0).all()) and bool((db == 0).all())
 
 
 @pytest.mark.parametrize("cols", [8, 1001, 4096, 40000])

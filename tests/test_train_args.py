@@ -23,11 +23,12 @@ def ptr(a):
 
 def norm_args(**kw):
     a = {"rank": 2, "sizes": [4, 32], "x": P, "xt": 0, "xs": [32, 1], "y": 2 * P, "yt": 0, "ys": [32, 1], "w": 3 * P,
-         "b": 4 * P, "wt": 0, "eps": 1e-5, "mean": 5 * P, "rstd": 6 * P}
+         "b": 4 * P, "wt": 0, "eps": 1e-5, "mean": 5 * P, "rstd": 6 * P, "ws": None, "bytes": 0}
     a.update(kw)
     arrays = [array("q", a[n]) if a[n] is not None else None for n in ("sizes", "xs", "ys")]
     st = lib().spmdb200_layer_norm(a["rank"], ptr(arrays[0]), a["x"], a["xt"], ptr(arrays[1]), a["y"], a["yt"],
-                                   ptr(arrays[2]), a["w"], a["b"], a["wt"], a["eps"], a["mean"], a["rstd"], None)
+                                   ptr(arrays[2]), a["w"], a["b"], a["wt"], a["eps"], a["mean"], a["rstd"], a["ws"],
+                                   a["bytes"], None)
     return st
 
 
@@ -45,6 +46,9 @@ def test_layer_norm_refuses(bad):
 def test_layer_norm_refuses_type_pairs_and_many_rows():
     assert norm_args(xt=1, yt=2) == -4
     assert norm_args(rank=3, sizes=[1 << 30, 1 << 30, 4], xs=[4, 4, 1], ys=[1 << 32, 4, 1]) == -1
+    long = {"sizes": [4, 20000], "xs": [20000, 1], "ys": [20000, 1]}  # rows that need a workspace
+    assert norm_args(**long) == -5 and norm_args(**long, ws=7 * P + 8, bytes=1 << 30) == -5
+    assert norm_args(**long, ws=7 * P, bytes=64) == -5
 
 
 def test_layer_norm_accepts():
@@ -83,7 +87,10 @@ def test_workspace_sizes():
     assert f(-1, 4) == 0 and f(4, 0) == 0
     for rows in (0, 1, 100, 1 << 20):
         for cols in (1, 64, 1000, 8192, 8193, 100000, 1 << 18, 1 << 24):
-            assert 8 * cols <= f(rows, cols) <= (40 << 20) + 64 * cols + 64 * rows, (rows, cols)
+            # Column sums of at most 444 rows of 8192 or so, or eight partial rows; shares of 72 MB of rows, or of eight.
+            assert 8 * cols <= f(rows, cols) <= (32 << 20) + 80 * cols, (rows, cols)
+            assert lib().spmdb200_layer_norm_forward_workspace_bytes(rows, cols) <= (8 << 20) + 2 * cols, (rows, cols)
+    assert lib().spmdb200_layer_norm_forward_workspace_bytes(1000, 8185) == 0
     g = lib().spmdb200_grad_norm_workspace_bytes
     assert 0 < g(0) <= g(1) <= g(5000) <= 1 << 20
 
