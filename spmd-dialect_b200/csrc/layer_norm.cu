@@ -28,7 +28,7 @@ constexpr int64_t kLongRun = (int64_t)kLongLanes * kMost;
 // are a long chain of waits, and a second row fills them.
 constexpr int kStages = 3;
 
-template <class TX, class TY, int W, int NV, int R, int MAXT>
+template <class TX, class TY, int W, int NV, int R, int MAXT, bool WRAPS>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
 ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
                   const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int lanes) {
@@ -54,9 +54,9 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   auto fetch = [&] {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, left);
+      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, have.full, left);
       ++fetched;
-      from = next_row(from, x + lane * W - shift, xr, i + fetched * step);
+      from = next_row<WRAPS>(from, x + lane * W - shift, xr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
     stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
@@ -71,7 +71,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   }
   // R sums of a row each, as a pair.
   auto sums = [&](const F2 (&t)[R], int space) {
-    if constexpr (R == 2) return row_sum2({t[0].x + t[0].y, t[1].x + t[1].y}, lanes, sh[space]);
+    if constexpr (R == 2) return row_sum2<MAXT>({t[0].x + t[0].y, t[1].x + t[1].y}, lanes, sh[space]);
     else return both(row_sum(t[0].x + t[0].y, lanes, &sh[space]->x));
   };
   for (int turn = 0; turn < turns; turn += R) {
@@ -81,7 +81,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       unsigned char *const slot = slots + stage + q * (NV * kPitch);
-      if (have.front) clear_front<TX>(slot, shift);
+      if (!have.full && have.front) clear_front<TX>(slot, shift);
       t[q] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
@@ -94,29 +94,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
     const F2 mean2 = mul2(sums(t, 0), both(inv_n));
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const float mean = q ? mean2.y : mean2.x;
-      t[q] = {0.0f, 0.0f};
-      if (have.edges) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const unsigned in = inside<W>(k, cols, lane, lanes, shift);
-#pragma unroll
-          for (int e = 0; e < W / 2; ++e) {  // elements outside the row stay zero
-            v[q][k][e] = add2(v[q][k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
-            t[q] = fma2(v[q][k][e], v[q][k][e], t[q]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const F2 off = both(have.whole >> k & 1 ? -mean : 0.0f);
-#pragma unroll
-          for (int e = 0; e < W / 2; ++e) {
-            v[q][k][e] = add2(v[q][k][e], off);
-            t[q] = fma2(v[q][k][e], v[q][k][e], t[q]);
-          }
-        }
-      }
+      t[q] = deviations<W, NV>(v[q], q ? mean2.y : mean2.x, have.full, cols, lane, lanes, shift);
     }
     const F2 var2 = mul2(sums(t, 1), both(inv_n));
 #pragma unroll
@@ -128,13 +106,13 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 #pragma unroll
           for (int e = 0; e < W / 2; ++e)
             v[q][k][e] = fma2(mul2(v[q][k][e], both(rstd)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
-        stream_store<W, NV>(to, have, cols, lane, lanes, shift, v[q]);
+        stream_store<W, NV>(to, have.full, cols, lane, lanes, shift, v[q]);
         if (lane == 0) {
           if (mean_out) mean_out[i + (turn + q) * step] = q ? mean2.y : mean2.x;
           if (rstd_out) rstd_out[i + (turn + q) * step] = rstd;
         }
       }
-      to = next_row(to, y + lane * W - shift, yr, i + (turn + q + 1) * step);
+      to = next_row<WRAPS>(to, y + lane * W - shift, yr, i + (turn + q + 1) * step);
     }
   }
   copy_wait<0>();
@@ -205,7 +183,7 @@ __device__ __forceinline__ Moments join_warp(Moments a) {
 // Longer rows, first pass: moments of each warp's share of a run.
 constexpr int kCutStages = 4;
 
-template <class TX, int W>
+template <class TX, int W, bool WRAPS>
 __global__ void __launch_bounds__(kThreads, 4)
 ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const __grid_constant__ Cut cut, float4 *shares) {
   constexpr int NV = kCutMost / W, kBytes = W * sizeof(TX), kPitch = kThreads * kBytes, kStage = NV * kPitch;
@@ -235,10 +213,10 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   const float inv_count = count > 0.0f ? 1.0f / count : 0.0f, all = warp_sum_f32(count), inv_all = all > 0.0f ? 1.0f / all : 0.0f;
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
-    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, left);
+    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, have.full, left);
     copy_commit();
     ++fetched;
-    from = next_row(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    from = next_row<WRAPS>(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -246,7 +224,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
     copy_wait<kCutStages - 1>();
-    if (have.front) clear_front<TX>(slots + stage, shift);
+    if (!have.full && have.front) clear_front<TX>(slots + stage, shift);
     F2 v[NV][W / 2], t{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -257,28 +235,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
     stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
     // Around the thread's mean, then the threads' means around the warp's.
     const float sum = t.x + t.y, mean = sum * inv_count;
-    t = {0.0f, 0.0f};
-    if (have.edges) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const unsigned in = inside<W>(k, n, lane, kThreads, shift);
-#pragma unroll
-        for (int e = 0; e < W / 2; ++e) {
-          const F2 d = add2(v[k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
-          t = fma2(d, d, t);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const F2 off = both(have.whole >> k & 1 ? -mean : 0.0f);
-#pragma unroll
-        for (int e = 0; e < W / 2; ++e) {
-          const F2 d = add2(v[k][e], off);
-          t = fma2(d, d, t);
-        }
-      }
-    }
+    t = deviations<W, NV>(v, mean, have.full, n, lane, kThreads, shift);
     const float warp_mean = warp_sum_f32(sum) * inv_all, d = mean - warp_mean;
     const float m2 = warp_sum_f32(fmaf(count * d, d, t.x + t.y));
     if ((lane & 31) == 0)
@@ -288,7 +245,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
 }
 
 // Second pass: the rows' statistics from the shares, and the output.
-template <class TX, class TY, int W>
+template <class TX, class TY, int W, bool WRAPS>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w, const void *b,
            int wtype, int64_t cols, float eps, float *mean_out, float *rstd_out, const __grid_constant__ Cut cut, const float4 *shares) {
@@ -314,10 +271,10 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
   for (int q = 0; q < kCutStages; ++q) clear_row<W, NV, kPitch, TX>(slots + q * kStage, left);
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
-    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, left);
+    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, have.full, left);
     copy_commit();
     ++fetched;
-    from = next_row(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    from = next_row<WRAPS>(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -359,8 +316,8 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
         v[k][e] = fma2(mul2(add2(v[k][e], both(stat.x)), both(stat.y)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
     }
     stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
-    stream_store<W, NV>(to, have, n, lane, kThreads, shift, v);
-    to = next_row(to, y + first + low + lane * W - shift, yr, at.i + (int64_t)(turn + 1) * cut.parts);
+    stream_store<W, NV>(to, have.full, n, lane, kThreads, shift, v);
+    to = next_row<WRAPS>(to, y + first + low + lane * W - shift, yr, at.i + (int64_t)(turn + 1) * cut.parts);
   }
   copy_wait<0>();
 }
@@ -430,16 +387,22 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
 }
 
 // ---- launches ---------------------------------------------------------------------
-template <class TX, class TY, int NV, int R, int MAXT>
-cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
+template <class TX, class TY, int NV, int R, int MAXT, bool WRAPS>
+cudaError_t stream_rows_as(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, bytes = kStages * R * NV * MAXT * W * (int)sizeof(TX);
-  auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT, WRAPS>;
+  if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int groups = MAXT / lanes, grid = stream_grid(p.rows, groups, most, W);
   const int64_t step = (int64_t)grid * groups;
-  kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, step), static_cast<TY *>(p.y),
-                                   row_walk(p.yr, p.rows, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
+  kernel<<<grid, MAXT, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, step), static_cast<TY *>(p.y),
+                                   row_walk(p.yr, step), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean, p.rstd, lanes);
   return cudaGetLastError();
+}
+
+template <class TX, class TY, int NV, int R, int MAXT>
+cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
+  return p.rows > p.xr.n1 || p.rows > p.yr.n1 ? stream_rows_as<TX, TY, NV, R, MAXT, true>(p, lanes, most, s)
+                                              : stream_rows_as<TX, TY, NV, R, MAXT, false>(p, lanes, most, s);
 }
 
 // Streamed rows: as many blocks as are resident, or one for each block of rows
@@ -459,24 +422,24 @@ cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t 
   return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, most, s);
 }
 
-template <class TX, class TY>
+template <class TX, class TY, bool WRAPS>
 cudaError_t forward_cut(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, bytes = kCutStages * kRun * (int)sizeof(TX);
-  auto first = ln_moments<TX, W>;
-  auto second = ln_outputs<TX, TY, W>;
-  if (cudaError_t e = cudaFuncSetAttribute(first, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-  if (cudaError_t e = cudaFuncSetAttribute(second, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  auto first = ln_moments<TX, W, WRAPS>;
+  auto second = ln_outputs<TX, TY, W, WRAPS>;
+  if (cudaError_t e = allow_shared(first, bytes)) return e;
+  if (cudaError_t e = allow_shared(second, bytes)) return e;
   const int64_t runs = most_runs(p.cols), batch = batch_rows(p.rows, p.cols, sizeof(TX));
   const int period = row_period(p.xr, p.rows, W);
   const int parts1 = cut_parts(batch, runs, 4 * device_sms(), period), parts2 = cut_parts(batch, runs, 2 * device_sms(), period);
   float4 *shares = static_cast<float4 *>(p.ws);
   for (int64_t row = 0; row < p.rows; row += batch) {
     const int64_t last = row + batch < p.rows ? row + batch : p.rows;
-    first<<<grid_for(runs * parts1), kThreads, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, parts1), p.cols,
+    first<<<grid_for(runs * parts1), kThreads, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, parts1), p.cols,
                                                            Cut{row, last, runs, parts1}, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
     second<<<grid_for(runs * parts2), kThreads, bytes, s>>>(
-        static_cast<const TX *>(p.x), row_walk(p.xr, p.rows, parts2), static_cast<TY *>(p.y), row_walk(p.yr, p.rows, parts2), p.w,
+        static_cast<const TX *>(p.x), row_walk(p.xr, parts2), static_cast<TY *>(p.y), row_walk(p.yr, parts2), p.w,
         p.b, p.wtype, p.cols, p.eps, p.mean, p.rstd, Cut{row, last, runs, parts2}, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
   }
@@ -515,7 +478,9 @@ cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W;
   const int spare = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) ? 0 : W - 1;
   if (p.xr.sc == 1 && p.yr.sc == 1 && same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
-    return p.cols + spare <= kHalfHeld ? forward_streamed<TX, TY>(p, spare, s) : forward_cut<TX, TY>(p, s);
+    return p.cols + spare <= kHalfHeld ? forward_streamed<TX, TY>(p, spare, s)
+           : p.rows > p.xr.n1 || p.rows > p.yr.n1 ? forward_cut<TX, TY, true>(p, s)
+                                                  : forward_cut<TX, TY, false>(p, s);
   if (p.cols > kHeld) return long_rows<TX, TY>(p, s);
   const int lanes = row_lanes(p.rows, p.cols, W, kMost, 0), nv = row_vectors(p.cols, lanes, W);
   if (nv == 1) return strided_rows<TX, TY, 1>(p, lanes, s);

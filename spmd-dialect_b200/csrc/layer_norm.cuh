@@ -40,31 +40,47 @@ __device__ __forceinline__ float row_sum(float v, int lanes, float *sh) {
   return warp_sum_f32(lane < warps ? sh[(warp & ~(warps - 1)) + lane] : 0.0f);
 }
 
-// Two such sums at once, for rows of one block; `sh` as above, of pairs.  The
-// first exchange gives either half of the lanes one of the two to go on with.
+// Two such sums at once; `sh` as above, of pairs.  The first exchange gives either
+// half of the lanes one of the two to go on with.
+__device__ __forceinline__ float add_lanes(float v, int from) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o <= from) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int MAXT>
 __device__ __forceinline__ F2 row_sum2(F2 v, int lanes, F2 *sh) {
   const int lane = threadIdx.x & 31;
-  if (lanes == 1) return v;
-  int o = lanes < 32 ? lanes >> 1 : 16;
-  const int half = o;
-  const bool upper = lane & half;
-  float s = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, o);
-  for (o >>= 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lanes <= 32) {
+  if (lanes < 32) {
+    if (lanes == 1) return v;
+    const int half = lanes >> 1;
+    const bool upper = lane & half;
+    float s = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, half);
+    for (int o = half >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     const float t = __shfl_xor_sync(0xffffffffu, s, half);
     return upper ? F2{t, s} : F2{s, t};
   }
+  const bool upper = lane & 16;
+  float s = (upper ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+  s = add_lanes(s, 8);
+  if (lanes == 32) return {__shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, s, 16)};
   const int warp = threadIdx.x >> 5, warps = lanes >> 5;
   if ((lane & 15) == 0) (upper ? sh[warp].y : sh[warp].x) = s;
   __syncthreads();
   const float4 *two = reinterpret_cast<const float4 *>(sh + (warp & ~(warps - 1)));
   F2 t{0.0f, 0.0f};
+  if (warps == MAXT / 32) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (q < warps / 2) {
+    for (int q = 0; q < MAXT / 64; ++q) {
       const float4 f = two[q];
       t = add2(t, add2({f.x, f.y}, {f.z, f.w}));
     }
+  } else {
+    for (int q = 0; q < warps / 2; ++q) {
+      const float4 f = two[q];
+      t = add2(t, add2({f.x, f.y}, {f.z, f.w}));
+    }
+  }
   return t;
 }
 
@@ -72,6 +88,7 @@ __device__ __forceinline__ F2 row_sum2(F2 v, int lanes, F2 *sh) {
 struct F4 {
   F2 a, b;
 };
+template <int MAXT>
 __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
   const int lane = threadIdx.x & 31;
   const unsigned all = 0xffffffffu;
@@ -82,29 +99,39 @@ __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
     }
     return v;
   }
-  const int wide = lanes < 32 ? lanes : 32, half = wide >> 1, quarter = wide >> 2;
-  const bool second = lane & half, odd = lane & quarter;
-  const F2 keep = second ? v.b : v.a, give = second ? v.a : v.b;
-  const F2 two = add2(keep, {__shfl_xor_sync(all, give.x, half), __shfl_xor_sync(all, give.y, half)});
-  float s = (odd ? two.y : two.x) + __shfl_xor_sync(all, odd ? two.x : two.y, quarter);
-  for (int o = wide >> 3; o > 0; o >>= 1) s += __shfl_xor_sync(all, s, o);
-  if (lanes <= 32) {
-    const int base = lane & ~(wide - 1);
-    return {{__shfl_sync(all, s, base), __shfl_sync(all, s, base | quarter)},
-            {__shfl_sync(all, s, base | half), __shfl_sync(all, s, base | half | quarter)}};
+  auto halves = [&](int half, int quarter) {
+    const bool second = lane & half, odd = lane & quarter;
+    const F2 keep = second ? v.b : v.a, give = second ? v.a : v.b;
+    const F2 two = add2(keep, {__shfl_xor_sync(all, give.x, half), __shfl_xor_sync(all, give.y, half)});
+    return (odd ? two.y : two.x) + __shfl_xor_sync(all, odd ? two.x : two.y, quarter);
+  };
+  auto spread = [&](float s, int base, int half, int quarter) {
+    return F4{{__shfl_sync(all, s, base), __shfl_sync(all, s, base | quarter)},
+              {__shfl_sync(all, s, base | half), __shfl_sync(all, s, base | half | quarter)}};
+  };
+  if (lanes < 32) {
+    float s = halves(lanes >> 1, lanes >> 2);
+    for (int o = lanes >> 3; o > 0; o >>= 1) s += __shfl_xor_sync(all, s, o);
+    return spread(s, lane & ~(lanes - 1), lanes >> 1, lanes >> 2);
   }
+  const float s = add_lanes(halves(16, 8), 4);
+  if (lanes == 32) return spread(s, 0, 16, 8);
   const int warp = threadIdx.x >> 5, warps = lanes >> 5;
   if ((lane & 7) == 0) reinterpret_cast<float *>(sh + warp)[lane >> 3] = s;
   __syncthreads();
   const float4 *row = sh + (warp & ~(warps - 1));
   F4 t{{0.0f, 0.0f}, {0.0f, 0.0f}};
+  auto add = [&](int q) {
+    const float4 f = row[q];
+    t.a = add2(t.a, {f.x, f.y});
+    t.b = add2(t.b, {f.z, f.w});
+  };
+  if (warps == MAXT / 32) {
 #pragma unroll
-  for (int q = 0; q < 16; ++q)
-    if (q < warps) {
-      const float4 f = row[q];
-      t.a = add2(t.a, {f.x, f.y});
-      t.b = add2(t.b, {f.z, f.w});
-    }
+    for (int q = 0; q < MAXT / 32; ++q) add(q);
+  } else {
+    for (int q = 0; q < warps; ++q) add(q);
+  }
   return t;
 }
 
@@ -177,16 +204,16 @@ __device__ __forceinline__ void load_weight(const void *p, int type, int64_t fir
 
 // ---- streamed rows ------------------------------------------------------------------
 // A view as a block goes through its rows: `step` elements from one to the next,
-// or, where the rows are not at one stride (wraps), each row's own offset.
+// or (WRAPS), where the rows are not at one stride, each row's own offset.
 struct RowWalk {
   Rows r;
   int64_t step;
-  bool wraps;
 };
-inline RowWalk row_walk(const Rows &r, int64_t rows, int64_t step) { return {r, step * r.s1, rows > r.n1}; }
-template <class T>
+inline RowWalk row_walk(const Rows &r, int64_t step) { return {r, step * r.s1}; }
+template <bool WRAPS, class T>
 __device__ __forceinline__ T *next_row(T *row, T *view, const RowWalk &w, int64_t i) {
-  return w.wraps ? view + row_offset(w.r, i) : row + w.step;
+  if constexpr (WRAPS) return view + row_offset(w.r, i);
+  else return row + w.step;
 }
 // Rows i, i + step, ... below `rows`.
 __device__ __forceinline__ int row_count(int64_t i, int64_t rows, int64_t step) {
@@ -207,12 +234,18 @@ __device__ __forceinline__ int vector_left(int k, int cols, int lane, int lanes,
 }
 // Starts the copies of a row's vectors into a thread's slots, `PITCH` bytes apart;
 // what a vector past the row's end does not have of it becomes zero.  Slots of
-// vectors that have nothing of it are zero from the start.
+// vectors that have nothing of it are zero from the start.  `full`: the warp's
+// vectors are all whole.
 template <int W, int NV, int PITCH, class T>
-__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, const int (&left)[NV]) {
+__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, bool full, const int (&left)[NV]) {
+  if (full) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (left[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, left[k] * (int)sizeof(T));
+    for (int k = 0; k < NV; ++k) copy_async<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W);
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (left[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, left[k] * (int)sizeof(T));
+  }
 }
 template <int W, int NV, int PITCH, class T>
 __device__ __forceinline__ void clear_row(unsigned char *slot, const int (&left)[NV]) {
@@ -234,26 +267,20 @@ __device__ __forceinline__ unsigned inside(int k, int cols, int lane, int lanes,
   }
   return m;
 }
-// What of its vectors a thread has in a row: bit k of `whole`, all of vector k.
-// `edges`: whether a lane of the warp has one that is there in part (the row's
-// start or end); `front`: this one has the start, `shift` elements of another row
-// before it.
+// Whether all vectors of the warp are whole in a row; `front`: this thread has the
+// row's start, with `shift` elements of another row before it.
 struct Held {
-  unsigned whole;
-  bool edges, front;
+  bool full, front;
 };
 template <int W, int NV>
 __device__ __forceinline__ Held held(int cols, int lane, int lanes, int shift) {
-  Held h{0, false, lane == 0 && shift > 0 && shift < W};
-  bool part = false;
+  bool whole = true;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const unsigned in = inside<W>(k, cols, lane, lanes, shift);
-    if (in == (1u << W) - 1) h.whole |= 1u << k;
-    else part |= in != 0;
+    const int c = shifted<W>(k, 0, lane, lanes, shift);
+    whole &= c >= 0 && c + W <= cols;
   }
-  h.edges = __any_sync(0xffffffffu, part);
-  return h;
+  return {(bool)__all_sync(0xffffffffu, whole), lane == 0 && shift > 0 && shift < W};
 }
 // A vector out of a thread's slot as pairs.  What of another row is before this
 // one's start is made zero first, so that sums need no tests.
@@ -271,26 +298,55 @@ __device__ __forceinline__ void clear_front(unsigned char *slot, int shift) {
 }
 // A row's vectors to memory: whole ones at once, the others element by element.
 template <int W, int NV, class T>
-__device__ __forceinline__ void stream_store(T *vector, const Held &have, int cols, int lane, int lanes, int shift,
+__device__ __forceinline__ void stream_store(T *vector, bool full, int cols, int lane, int lanes, int shift,
                                              const F2 (&v)[NV][W / 2]) {
+  auto put = [&](int k) {
+    float f[W];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (have.whole >> k & 1) {
-      float f[W];
+    for (int e = 0; e < W / 2; ++e) f[2 * e] = v[k][e].x, f[2 * e + 1] = v[k][e].y;
+    store_vec<W>(vector + k * lanes * W, f);
+  };
+  if (full) {
 #pragma unroll
-      for (int e = 0; e < W / 2; ++e) f[2 * e] = v[k][e].x, f[2 * e + 1] = v[k][e].y;
-      store_vec<W>(vector + k * lanes * W, f);
-    }
-  if (have.edges) {
+    for (int k = 0; k < NV; ++k) put(k);
+  } else {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (!(have.whole >> k & 1)) {
-        const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+    for (int k = 0; k < NV; ++k) {
+      const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+      if (in == (1u << W) - 1) {
+        put(k);
+      } else if (in) {
 #pragma unroll
         for (int e = 0; e < W; ++e)
           if (in >> e & 1) vector[k * lanes * W + e] = from_f32<T>(e & 1 ? v[k][e / 2].y : v[k][e / 2].x);
       }
+    }
   }
+}
+// v - mean inside the row (zero elsewhere, as it was), and the squares' sum.
+template <int W, int NV>
+__device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, bool full, int cols, int lane, int lanes, int shift) {
+  F2 t{0.0f, 0.0f};
+  if (full) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        v[k][e] = add2(v[k][e], both(-mean));
+        t = fma2(v[k][e], v[k][e], t);
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        v[k][e] = add2(v[k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
+        t = fma2(v[k][e], v[k][e], t);
+      }
+    }
+  }
+  return t;
 }
 
 // ---- rows longer than a block holds -----------------------------------------------------
@@ -356,6 +412,12 @@ inline bool same_shift(const void *p, const Rows &r, int p_size, const void *q, 
 inline int device_sms() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess ? num_sms(dev) : 148;
+}
+// Shared memory past 48 KB, with a kernel's own arrays of up to 20 KB, has to be
+// asked for.
+template <class Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes) {
+  return bytes <= 28 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 inline unsigned grid_for(int64_t items) { return (unsigned)(items < INT32_MAX ? items : INT32_MAX); }
 

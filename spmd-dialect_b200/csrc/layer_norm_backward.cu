@@ -15,7 +15,6 @@ namespace {
 constexpr int kMost = 16;        // elements of a row in a thread: two sums are held for each too
 constexpr int kWideLanes = 512;  // threads of a block for rows past kThreads * kMost columns
 constexpr int kMaxParts = 444;   // three blocks per SM
-constexpr int kColWidth = 32, kColDepth = 32;
 constexpr int64_t kHeld = (int64_t)kWideLanes * kMost;  // columns that a block holds
 
 // What the kernels are given.
@@ -99,7 +98,7 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
         x[k][e] = xh;
       }
     if (!p.dx) continue;
-    s = row_sum2(s, lanes, sh[turn]);
+    s = row_sum2<MAXT>(s, lanes, sh[turn]);
     const float c1 = s.x * inv_n, c2 = s.y * inv_n;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -120,7 +119,7 @@ constexpr int kStages = 3;
 template <class TX, class TY>
 constexpr int kRowsAtOnce = sizeof(TX) + sizeof(TY) <= 6 ? 2 : 1;  // as two blocks' stages fit an SM
 
-template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES>
+template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES, bool WRAPS>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3)
 ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
                    const __grid_constant__ RowWalk dr, int lanes) {
@@ -156,8 +155,8 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       if (fetched < mine) {
-        stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage + q * kRow, x_from, lanes, left);
-        stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage + q * kRow, g_from, lanes, left);
+        stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage + q * kRow, x_from, lanes, have.full, left);
+        stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage + q * kRow, g_from, lanes, have.full, left);
         if (first) {
           copy_async<4>(&stats[stage_in * R + q][slot].x, mean_in);
           copy_async<4>(&stats[stage_in * R + q][slot].y, rstd_in);
@@ -165,8 +164,8 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
       }
       ++fetched;
       mean_in += step, rstd_in += step;
-      x_from = next_row(x_from, p.x + start, xr, i + fetched * step);
-      g_from = next_row(g_from, p.dy + start, gr, i + fetched * step);
+      x_from = next_row<WRAPS>(x_from, p.x + start, xr, i + fetched * step);
+      g_from = next_row<WRAPS>(g_from, p.dy + start, gr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
@@ -193,7 +192,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
       const bool live = turn + q < mine;
       unsigned char *const xs = x_slots + stage * kStage + q * kRow, *const gs = g_slots + stage * kStage + q * kRow;
       stat[q] = live ? stats[stage * R + q][slot] : make_float2(0.0f, 0.0f);
-      if (have.front) {
+      if (!have.full && have.front) {
         clear_front<TX>(xs, shift);
         clear_front<TY>(gs, shift);
       }
@@ -214,10 +213,10 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
     }
     __syncwarp();  // every lane has its statistics: the slot may be filled again
     if constexpr (R == 2) {
-      const F4 t = row_sum4({c[0], c[1]}, lanes, sh[(turn / R) & 1]);
+      const F4 t = row_sum4<MAXT>({c[0], c[1]}, lanes, sh[(turn / R) & 1]);
       c[0] = t.a, c[1] = t.b;
     } else {
-      c[0] = row_sum2(c[0], lanes, reinterpret_cast<F2 *>(sh[turn & 1]));
+      c[0] = row_sum2<MAXT>(c[0], lanes, reinterpret_cast<F2 *>(sh[turn & 1]));
     }
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -238,9 +237,9 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
             g[k][e] = mul2(fma2(xh, c2, fma2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]}, c1)), both(stat[q].y));
           }
         }
-        if (p.dx) stream_store<W, NV>(to, have, cols, lane, lanes, shift, g);
+        if (p.dx) stream_store<W, NV>(to, have.full, cols, lane, lanes, shift, g);
       }
-      to = next_row(to, p.dx + start, dr, i + (turn + q + 1) * step);
+      to = next_row<WRAPS>(to, p.dx + start, dr, i + (turn + q + 1) * step);
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
@@ -260,7 +259,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
 }
 
 // Longer rows (layer_norm.cuh), first pass: each warp's share of a row's two sums.
-template <class TX, class TY, int W>
+template <class TX, class TY, int W, bool WRAPS>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
           const __grid_constant__ Cut cut, float2 *shares) {
@@ -292,13 +291,13 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
     if (fetched < at.rows) {
-      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, left);
-      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, left);
+      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, have.full, left);
+      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, have.full, left);
     }
     copy_commit();
     ++fetched;
-    x_from = next_row(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
-    g_from = next_row(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    x_from = next_row<WRAPS>(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row<WRAPS>(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -311,7 +310,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
     fetch();
     copy_wait<kStages - 1>();
     const float2 stat = stats[turn];
-    if (have.front) {
+    if (!have.full && have.front) {
       clear_front<TX>(x_slots + stage, shift);
       clear_front<TY>(g_slots + stage, shift);
     }
@@ -329,7 +328,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
       }
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
-    const F2 s = row_sum2({s1.x + s1.y, s2.x + s2.y}, 32, nullptr);
+    const F2 s = row_sum2<kThreads>({s1.x + s1.y, s2.x + s2.y}, 32, nullptr);
     if ((lane & 31) == 0)
       shares[((at.i - cut.first + (int64_t)turn * cut.parts) * cut.runs + at.run) * kCutWarps + (lane >> 5)] = make_float2(s.x, s.y);
   }
@@ -338,7 +337,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
 
 // Second pass: dx and the column sums, which go on from what the batches before
 // left in the part's partial row.
-template <class TX, class TY, int W>
+template <class TX, class TY, int W, bool WRAPS>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
          const __grid_constant__ RowWalk dr, const __grid_constant__ Cut cut, const float2 *shares) {
@@ -371,13 +370,13 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
     if (fetched < at.rows) {
-      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, left);
-      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, left);
+      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, have.full, left);
+      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, have.full, left);
     }
     copy_commit();
     ++fetched;
-    x_from = next_row(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
-    g_from = next_row(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    x_from = next_row<WRAPS>(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row<WRAPS>(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -417,7 +416,7 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
     fetch();
     copy_wait<kStages - 1>();
     const float4 stat = stats[turn];
-    if (have.front) {
+    if (!have.full && have.front) {
       clear_front<TX>(x_slots + stage, shift);
       clear_front<TY>(g_slots + stage, shift);
     }
@@ -436,8 +435,8 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
       }
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
-    if (p.dx) stream_store<W, NV>(to, have, n, lane, kThreads, shift, g);
-    to = next_row(to, p.dx + start, dr, at.i + (int64_t)(turn + 1) * cut.parts);
+    if (p.dx) stream_store<W, NV>(to, have.full, n, lane, kThreads, shift, g);
+    to = next_row<WRAPS>(to, p.dx + start, dr, at.i + (int64_t)(turn + 1) * cut.parts);
   }
   copy_wait<0>();
   if (!p.part) return;
@@ -480,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_shares(const __grid_co
         s.y = fmaf(a, (x[k][e] - mean) * rstd, s.y);
       }
     }
-    s = row_sum2(s, kThreads, sh[turn & 1]);
+    s = row_sum2<kThreads>(s, kThreads, sh[turn & 1]);
     if (threadIdx.x < kCutWarps)
       shares[((i - cut.first) * cut.runs + at.run) * kCutWarps + threadIdx.x] = threadIdx.x ? make_float2(0.0f, 0.0f) : make_float2(s.x, s.y);
   }
@@ -548,29 +547,33 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
     }
 }
 
-// dw and db from the partial rows (part p: dw at row 2p, db at row 2p + 1).
-__global__ void __launch_bounds__(kColWidth *kColDepth)
-ln_finish(const float *__restrict__ part, int parts, int64_t cols, void *dw, void *db, int type) {
-  __shared__ float sh[2][kColDepth][kColWidth];
-  const int tx = threadIdx.x & (kColWidth - 1), ty = threadIdx.x / kColWidth;
-  const int64_t j = (int64_t)blockIdx.x * kColWidth + tx;
+// dw and db from the partial rows (part p: dw at row 2p, db at row 2p + 1): `depth`
+// threads a column, each of them every depth-th part.
+__global__ void __launch_bounds__(1024)
+ln_finish(const float *__restrict__ part, int parts, int64_t cols, int depth, void *dw, void *db, int type) {
+  __shared__ float sh[2][1024];
+  const int width = blockDim.x / depth, tx = threadIdx.x % width, ty = threadIdx.x / width;
+  const int64_t j = (int64_t)blockIdx.x * width + tx;
   float sw = 0.0f, sb = 0.0f;
   if (j < cols)
 #pragma unroll 4
-    for (int p = ty; p < parts; p += kColDepth) {
+    for (int p = ty; p < parts; p += depth) {
       sw += part[(2 * (int64_t)p) * cols + j];
       sb += part[(2 * (int64_t)p + 1) * cols + j];
     }
-  sh[0][ty][tx] = sw;
-  sh[1][ty][tx] = sb;
-  __syncthreads();
-  if (ty < 2 && j < cols) {
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kColDepth; ++k) s += sh[ty][k][tx];
-    void *out = ty == 0 ? dw : db;
-    if (out) store_from_f32(out, type, j, s);
+  if (depth > 1) {
+    sh[0][threadIdx.x] = sw;
+    sh[1][threadIdx.x] = sb;
+    __syncthreads();
+    if (ty > 0) return;
+    for (int k = 1; k < depth; ++k) {
+      sw += sh[0][k * width + tx];
+      sb += sh[1][k * width + tx];
+    }
   }
+  if (j >= cols || ty > 0) return;
+  if (dw) store_from_f32(dw, type, j, sw);
+  if (db) store_from_f32(db, type, j, sb);
 }
 
 // ---- launches ---------------------------------------------------------------------
@@ -590,29 +593,39 @@ cudaError_t backward_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStre
   return cudaGetLastError();
 }
 
-template <class TX, class TY, int NV, int MAXT>
-cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
+template <class TX, class TY>
+bool wraps(const Back<TX, TY> &b) {
+  return b.rows > b.xr.n1 || b.rows > b.gr.n1 || (b.dx && b.rows > b.dr.n1);
+}
+
+template <class TX, class TY, int NV, int MAXT, bool WRAPS>
+cudaError_t stream_rows_as(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;
   constexpr int staged = stages * R * NV * MAXT * W * (int)(sizeof(TX) + sizeof(TY));
   const int sums = b.part ? (int)(MAXT / lanes * b.cols * sizeof(float)) : 0, bytes = staged > sums ? staged : sums;
-  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages, WRAPS>;
+  if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int64_t groups = MAXT / lanes;
   const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
   *parts = stream_grid(b.rows, groups, most < kMaxParts ? most : kMaxParts, W);
   const int64_t step = *parts * groups;
-  kernel<<<*parts, MAXT, bytes, s>>>(b, row_walk(b.gr, b.rows, step), row_walk(b.xr, b.rows, step), row_walk(b.dr, b.rows, step), lanes);
+  kernel<<<*parts, MAXT, bytes, s>>>(b, row_walk(b.gr, step), row_walk(b.xr, step), row_walk(b.dr, step), lanes);
   return cudaGetLastError();
 }
 
-template <class TX, class TY>
+template <class TX, class TY, int NV, int MAXT>
+cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
+  return wraps(b) ? stream_rows_as<TX, TY, NV, MAXT, true>(b, lanes, parts, s) : stream_rows_as<TX, TY, NV, MAXT, false>(b, lanes, parts, s);
+}
+
+template <class TX, class TY, bool WRAPS>
 cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, bool vectors, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, bytes = kStages * kRun * (int)(sizeof(TX) + sizeof(TY));
-  auto shares_of = ln_shares<TX, TY, W>;
-  auto grads_of = ln_grads<TX, TY, W>;
+  auto shares_of = ln_shares<TX, TY, W, WRAPS>;
+  auto grads_of = ln_grads<TX, TY, W, WRAPS>;
   if (vectors) {
-    if (cudaError_t e = cudaFuncSetAttribute(shares_of, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-    if (cudaError_t e = cudaFuncSetAttribute(grads_of, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    if (cudaError_t e = allow_shared(shares_of, bytes)) return e;
+    if (cudaError_t e = allow_shared(grads_of, bytes)) return e;
   }
   const int64_t runs = most_runs(b.cols), batch = batch_rows(b.rows, b.cols, sizeof(TX) + sizeof(TY));
   const int period = vectors ? row_period(b.xr, b.rows, W) : 1;
@@ -625,14 +638,14 @@ cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, bool vectors, int *par
     const unsigned grid1 = grid_for(runs * parts1), grid2 = grid_for(runs * parts2);
     if (b.dx) {
       if (vectors)
-        shares_of<<<grid1, kThreads, bytes, s>>>(b, row_walk(b.gr, b.rows, parts1), row_walk(b.xr, b.rows, parts1), cut1, shares);
+        shares_of<<<grid1, kThreads, bytes, s>>>(b, row_walk(b.gr, parts1), row_walk(b.xr, parts1), cut1, shares);
       else
         ln_strided_shares<TX, TY, W><<<grid1, kThreads, 0, s>>>(b, cut1, shares);
       if (cudaError_t e = cudaGetLastError()) return e;
     }
     if (vectors)
-      grads_of<<<grid2, kThreads, bytes, s>>>(b, row_walk(b.gr, b.rows, parts2), row_walk(b.xr, b.rows, parts2),
-                                              row_walk(b.dr, b.rows, parts2), cut2, shares);
+      grads_of<<<grid2, kThreads, bytes, s>>>(b, row_walk(b.gr, parts2), row_walk(b.xr, parts2),
+                                              row_walk(b.dr, parts2), cut2, shares);
     else
       ln_strided_grads<TX, TY, W><<<grid2, kThreads, 0, s>>>(b, cut2, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
@@ -647,7 +660,8 @@ cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_
                        same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
                        (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W));
   const int spare = vectors && !vec_rows(b.x, b.xr, b.rows, sizeof(TX), W) ? W - 1 : 0;
-  if (b.cols > kHeld - spare) return backward_cut<TX, TY>(b, ws, vectors, parts, s);
+  if (b.cols > kHeld - spare)
+    return wraps(b) ? backward_cut<TX, TY, true>(b, ws, vectors, parts, s) : backward_cut<TX, TY, false>(b, ws, vectors, parts, s);
   const bool wide = b.cols + spare > kThreads * kMost;
   const int lanes = wide ? kWideLanes : row_lanes(b.rows, b.cols, W, kMost, spare), nv = row_vectors(b.cols + spare, lanes, W);
   if (vectors) {
@@ -671,8 +685,11 @@ cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
     if (cudaError_t e = backward_of<TX, TY>(b, p.ws, &parts, s)) return e;
   }
   if (!b.part) return cudaSuccess;
-  const int64_t tiles = (p.cols + kColWidth - 1) / kColWidth;
-  ln_finish<<<grid_for(tiles), kColWidth * kColDepth, 0, s>>>(b.part, parts, p.cols, p.dw, p.db, p.dwtype);
+  // Eight parts or so a thread, up to 32 threads a column in blocks of 1024.
+  int depth = 1;
+  while (depth < 32 && depth * 8 < parts) depth *= 2;
+  const int threads = depth < 32 ? 256 : 1024, width = threads / depth;
+  ln_finish<<<grid_for((p.cols + width - 1) / width), threads, 0, s>>>(b.part, parts, p.cols, depth, p.dw, p.db, p.dwtype);
   return cudaGetLastError();
 }
 
