@@ -25,8 +25,11 @@ constexpr int64_t kLongRun = (int64_t)kLongLanes * kMost;
 
 // Streamed rows (layer_norm.cuh): weight and bias are loaded once a thread.  A
 // group of lanes takes R rows at a time, one or two: the two reductions of a row
-// are a long chain of waits, and a second row fills them.
-constexpr int kStages = 3;
+// are a long chain of waits, and a second row fills them where rows are 16-bit (101
+// against 121 us for 32768 x 4096; f32 rows wait for memory, and are faster with one
+// at a time and a stage more: 124 against 141 us).
+template <int MAXT>
+constexpr int kStages = MAXT > kThreads ? 2 : 3;
 
 template <class TX, class TY, int W, int NV, int R, int MAXT, bool WRAPS>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
@@ -43,13 +46,13 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   const int shift = (int)((uintptr_t)from / sizeof(TX) % W);
   TY *to = y + (mine ? row_offset(yr.r, i) : 0) + lane * W - shift;
   from += lane * W - shift;
-  const Held have = held<W, NV>(cols, lane, lanes, shift);
+  const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
   int left[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
   unsigned char *const slots = smem + threadIdx.x * kBytes;
 #pragma unroll
-  for (int q = 0; q < kStages * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), left);
+  for (int q = 0; q < kStages<MAXT> * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), left);
   int stage_in = 0, stage = 0, fetched = 0;  // stages as offsets
   auto fetch = [&] {
 #pragma unroll
@@ -59,10 +62,10 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
       from = next_row<WRAPS>(from, x + lane * W - shift, xr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
-    stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
+    stage_in = stage_in == (kStages<MAXT> - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
-  for (int q = 0; q < kStages - 1; ++q) fetch();
+  for (int q = 0; q < kStages<MAXT> - 1; ++q) fetch();
   float wv[NV][W], bv[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -76,7 +79,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   };
   for (int turn = 0; turn < turns; turn += R) {
     fetch();
-    copy_wait<kStages - 1>();
+    copy_wait<kStages<MAXT> - 1>();
     F2 v[R][NV][W / 2], t[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -90,11 +93,11 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
         for (int e = 0; e < W / 2; ++e) t[q] = add2(t[q], v[q][k][e]);
       }
     }
-    stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
+    stage = stage == (kStages<MAXT> - 1) * kStage ? 0 : stage + kStage;
     const F2 mean2 = mul2(sums(t, 0), both(inv_n));
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      t[q] = deviations<W, NV>(v[q], q ? mean2.y : mean2.x, have.full, cols, lane, lanes, shift);
+      t[q] = deviations<W, NV>(v[q], q ? mean2.y : mean2.x, have);
     }
     const F2 var2 = mul2(sums(t, 1), both(inv_n));
 #pragma unroll
@@ -106,7 +109,7 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 #pragma unroll
           for (int e = 0; e < W / 2; ++e)
             v[q][k][e] = fma2(mul2(v[q][k][e], both(rstd)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
-        stream_store<W, NV>(to, have.full, cols, lane, lanes, shift, v[q]);
+        stream_store<W, NV>(to, have, lanes, v[q]);
         if (lane == 0) {
           if (mean_out) mean_out[i + (turn + q) * step] = q ? mean2.y : mean2.x;
           if (rstd_out) rstd_out[i + (turn + q) * step] = rstd;
@@ -199,13 +202,13 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   // As a row of its own that starts `shift` elements into its first vector.
   const int shift = at.run == 0 ? start : 0, n = high - low;
   from += first + low + lane * W - shift;
-  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
   int left[NV];
   float count = 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     left[k] = vector_left<W>(k, n, lane, kThreads, shift);
-    count += (float)__popc(inside<W>(k, n, lane, kThreads, shift));
+    count += (float)__popc(have.in[k]);
   }
   unsigned char *const slots = smem + threadIdx.x * kBytes;
 #pragma unroll
@@ -235,7 +238,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
     stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
     // Around the thread's mean, then the threads' means around the warp's.
     const float sum = t.x + t.y, mean = sum * inv_count;
-    t = deviations<W, NV>(v, mean, have.full, n, lane, kThreads, shift);
+    t = deviations<W, NV>(v, mean, have);
     const float warp_mean = warp_sum_f32(sum) * inv_all, d = mean - warp_mean;
     const float m2 = warp_sum_f32(fmaf(count * d, d, t.x + t.y));
     if ((lane & 31) == 0)
@@ -262,7 +265,7 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
   const int shift = at.run == 0 ? start : 0, n = high - low;
   TY *to = y + row_offset(yr.r, at.i) + first + low + lane * W - shift;
   from += first + low + lane * W - shift;
-  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
   int left[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
@@ -316,7 +319,7 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
         v[k][e] = fma2(mul2(add2(v[k][e], both(stat.x)), both(stat.y)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
     }
     stage = stage == (kCutStages - 1) * kStage ? 0 : stage + kStage;
-    stream_store<W, NV>(to, have.full, n, lane, kThreads, shift, v);
+    stream_store<W, NV>(to, have, kThreads, v);
     to = next_row<WRAPS>(to, y + first + low + lane * W - shift, yr, at.i + (int64_t)(turn + 1) * cut.parts);
   }
   copy_wait<0>();
@@ -389,7 +392,7 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
 // ---- launches ---------------------------------------------------------------------
 template <class TX, class TY, int NV, int R, int MAXT, bool WRAPS>
 cudaError_t stream_rows_as(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, bytes = kStages * R * NV * MAXT * W * (int)sizeof(TX);
+  constexpr int W = kWidth<TX, TY>, bytes = kStages<MAXT> * R * NV * MAXT * W * (int)sizeof(TX);
   auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT, WRAPS>;
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int groups = MAXT / lanes, grid = stream_grid(p.rows, groups, most, W);
@@ -418,8 +421,9 @@ cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t 
   const int nv = row_vectors(p.cols + spare, lanes, W), most = (nv * W > 8 ? 2 : 3) * device_sms();
   if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads>(p, lanes, most, s);
   if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads>(p, lanes, most, s);
-  if (p.rows <= (int64_t)most * groups) return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, most, s);
-  return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, most, s);
+  if constexpr (sizeof(TX) == 2)
+    if (p.rows > (int64_t)most * groups) return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, most, s);
+  return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, most, s);
 }
 
 template <class TX, class TY, bool WRAPS>

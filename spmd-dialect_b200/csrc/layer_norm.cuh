@@ -267,20 +267,26 @@ __device__ __forceinline__ unsigned inside(int k, int cols, int lane, int lanes,
   }
   return m;
 }
-// Whether all vectors of the warp are whole in a row; `front`: this thread has the
-// row's start, with `shift` elements of another row before it.
+// Which elements of its vectors a thread has in a row; `full`: whether the warp's
+// vectors are all whole; `front`: this thread has the row's start, with `shift`
+// elements of another row before it.
+template <int W, int NV>
 struct Held {
+  unsigned in[NV];
   bool full, front;
 };
 template <int W, int NV>
-__device__ __forceinline__ Held held(int cols, int lane, int lanes, int shift) {
+__device__ __forceinline__ Held<W, NV> held(int cols, int lane, int lanes, int shift) {
+  Held<W, NV> h;
   bool whole = true;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = shifted<W>(k, 0, lane, lanes, shift);
-    whole &= c >= 0 && c + W <= cols;
+    h.in[k] = inside<W>(k, cols, lane, lanes, shift);
+    whole &= h.in[k] == (1u << W) - 1;
   }
-  return {(bool)__all_sync(0xffffffffu, whole), lane == 0 && shift > 0 && shift < W};
+  h.full = __all_sync(0xffffffffu, whole);
+  h.front = lane == 0 && shift > 0 && shift < W;
+  return h;
 }
 // A vector out of a thread's slot as pairs.  What of another row is before this
 // one's start is made zero first, so that sums need no tests.
@@ -298,36 +304,34 @@ __device__ __forceinline__ void clear_front(unsigned char *slot, int shift) {
 }
 // A row's vectors to memory: whole ones at once, the others element by element.
 template <int W, int NV, class T>
-__device__ __forceinline__ void stream_store(T *vector, bool full, int cols, int lane, int lanes, int shift,
-                                             const F2 (&v)[NV][W / 2]) {
+__device__ __forceinline__ void stream_store(T *vector, const Held<W, NV> &have, int lanes, const F2 (&v)[NV][W / 2]) {
   auto put = [&](int k) {
     float f[W];
 #pragma unroll
     for (int e = 0; e < W / 2; ++e) f[2 * e] = v[k][e].x, f[2 * e + 1] = v[k][e].y;
     store_vec<W>(vector + k * lanes * W, f);
   };
-  if (full) {
+  if (have.full) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) put(k);
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const unsigned in = inside<W>(k, cols, lane, lanes, shift);
-      if (in == (1u << W) - 1) {
+      if (have.in[k] == (1u << W) - 1) {
         put(k);
-      } else if (in) {
+      } else if (have.in[k]) {
 #pragma unroll
         for (int e = 0; e < W; ++e)
-          if (in >> e & 1) vector[k * lanes * W + e] = from_f32<T>(e & 1 ? v[k][e / 2].y : v[k][e / 2].x);
+          if (have.in[k] >> e & 1) vector[k * lanes * W + e] = from_f32<T>(e & 1 ? v[k][e / 2].y : v[k][e / 2].x);
       }
     }
   }
 }
 // v - mean inside the row (zero elsewhere, as it was), and the squares' sum.
 template <int W, int NV>
-__device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, bool full, int cols, int lane, int lanes, int shift) {
+__device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, const Held<W, NV> &have) {
   F2 t{0.0f, 0.0f};
-  if (full) {
+  if (have.full) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -338,10 +342,15 @@ __device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, bool fu
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const unsigned in = inside<W>(k, cols, lane, lanes, shift);
+      const float off = have.in[k] ? -mean : 0.0f;
+      const bool part = have.in[k] && have.in[k] != (1u << W) - 1;
 #pragma unroll
       for (int e = 0; e < W / 2; ++e) {
-        v[k][e] = add2(v[k][e], {in >> (2 * e) & 1 ? -mean : 0.0f, in >> (2 * e + 1) & 1 ? -mean : 0.0f});
+        v[k][e] = add2(v[k][e], both(off));
+        if (part) {
+          if (!(have.in[k] >> (2 * e) & 1)) v[k][e].x = 0.0f;
+          if (!(have.in[k] >> (2 * e + 1) & 1)) v[k][e].y = 0.0f;
+        }
         t = fma2(v[k][e], v[k][e], t);
       }
     }

@@ -139,7 +139,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   const TY *g_from = p.dy + (mine ? row_offset(gr.r, i) : 0) + start;
   TX *to = p.dx + (mine && p.dx ? row_offset(dr.r, i) : 0) + start;
   x_from += start;
-  const Held have = held<W, NV>(cols, lane, lanes, shift);
+  const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
   int left[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
@@ -237,7 +237,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
             g[k][e] = mul2(fma2(xh, c2, fma2(g[k][e], {w[k][2 * e], w[k][2 * e + 1]}, c1)), both(stat[q].y));
           }
         }
-        if (p.dx) stream_store<W, NV>(to, have.full, cols, lane, lanes, shift, g);
+        if (p.dx) stream_store<W, NV>(to, have, lanes, g);
       }
       to = next_row<WRAPS>(to, p.dx + start, dr, i + (turn + q + 1) * step);
     }
@@ -278,7 +278,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   const int64_t start = first + low + lane * W - shift;
   const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
   x_from += start;
-  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
   int left[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
@@ -357,7 +357,7 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
   const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
   TX *to = p.dx + (p.dx ? row_offset(dr.r, at.i) : 0) + start;
   x_from += start;
-  const Held have = held<W, NV>(n, lane, kThreads, shift);
+  const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
   int left[NV];
 #pragma unroll
   for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
@@ -435,7 +435,7 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
       }
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
-    if (p.dx) stream_store<W, NV>(to, have.full, n, lane, kThreads, shift, g);
+    if (p.dx) stream_store<W, NV>(to, have, kThreads, g);
     to = next_row<WRAPS>(to, p.dx + start, dr, at.i + (int64_t)(turn + 1) * cut.parts);
   }
   copy_wait<0>();
