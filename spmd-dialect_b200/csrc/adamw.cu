@@ -31,7 +31,6 @@ constexpr float kTopCode = 448.0f, kLeastCode = 0x1p-9f, kLeastScale = 0x1p-120f
 
 struct AdamHyper {
   float beta1, beta2, rest1, rest2;  // 1 - beta, taken in f64
-  float root_beta2, root_rest2;     // sqrt(beta2), sqrt(1 - beta2)
   float eps;
   float lr, step_size, root_scale;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) (host step and lr)
   double beta1_d, beta2_d;          // for a step number on the device
@@ -169,11 +168,8 @@ __device__ __forceinline__ float from_code(uint8_t c) {
 }
 __device__ __forceinline__ uint8_t to_code(float v) { return __nv_fp8_e4m3(v).__x; }
 
-// Square root and reciprocal to within 2^-23 of the value: an 8-bit root and
-// the change of a parameter (a small part of it) are rounded far more coarsely,
-// and exact ones would cost as many instructions as the rest of the step.  The
-// root keeps subnormal arguments, whose roots are normal; the reciprocal's
-// argument is normal or zero.
+// Square root and reciprocal to within 2^-23 of the value.  The root keeps subnormal
+// arguments, whose roots are normal; the reciprocal's argument is normal or zero.
 __device__ __forceinline__ float sqrt_near(float v) {
   float r;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -183,16 +179,6 @@ __device__ __forceinline__ float rcp_near(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
-}
-// To half a unit or so: one step of Newton's on the near one.
-__device__ __forceinline__ float rcp_full(float v) {
-  const float y = rcp_near(v);
-  return fmaf(fmaf(-v, y, 1.0f), y, y);
-}
-__device__ __forceinline__ float ld_f1(const float *p) {
-  float v;
-  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
-  return v;
 }
 // Maxima that keep a NaN.
 __device__ __forceinline__ float top_of(float a, float b, float c) {
@@ -227,46 +213,75 @@ __device__ __forceinline__ uint2 encode8(const float v[8]) {
 }
 
 // The 8-bit step of eight elements a lane, one state block a warp; m and r come
-// as decoded codes and leave as codes' values, with the block's new scales.
-//   m = keep1 code + gain1 g,  v = o^2 + q^2 with o = keep2 code, q = gain2 g
-// (the factors beta1 ms, sqrt(beta2) vs, (1 - beta1) grad_scale and sqrt(1 -
-// beta2) grad_scale are taken once: no square of a scale, which would leave
-// f32's range long before the root does).
+// as decoded codes and leave as the values of new ones, with the block's new
+// scales.  A code is the nearest to value / scale: a rounding of 2^-4 that turns on
+// the last bit of f32 where the quotient lies half way between two codes, and the
+// new m of the next step with it.  So m and v are the formula's in f32, every
+// product and sum rounded as it is written, and a quotient near a half way point is
+// taken again with an exact root and division; elsewhere the near ones give the
+// same code (within 4 units of the last place, against a margin of 8) at half the
+// instructions.
 struct Scales {
   float m, v;
 };
-__device__ __forceinline__ Scales step8(float p[8], const float g[8], float m[8], float r[8], Scales old, const Now &c,
-                                        const AdamHyper &h, float keep, float gain1, float gain2) {
-  const float keep1 = h.beta1 * old.m, keep2 = h.root_beta2 * old.v;
-  const F2 k1{keep1, keep1}, k2{keep2, keep2}, g1{gain1, gain1}, g2{gain2, gain2}, root{c.root_scale, c.root_scale},
-      eps{h.eps, h.eps}, size{-c.step_size, -c.step_size}, kp{keep, keep};
-  float mtop = 0.0f, rtop = 0.0f;
+// 0 to 16 << 12 where a value's last 20 bits, those below a code's, are within 8 of
+// half way (of a code above the subnormal ones).
+__device__ __forceinline__ unsigned half_way(float q) {
+  return (__float_as_uint(q) << 12) + ((8u - 0x80000u) << 12);
+}
+constexpr unsigned kHalfWay = 16u << 12;
+
+__device__ __forceinline__ F2 apart(F2 a, F2 b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
+
+__device__ __forceinline__ Scales step8(float p[8], float g[8], float m[8], float r[8], Scales old, const Now &c,
+                                        const AdamHyper &h, float keep) {
+  const F2 gs = both(c.grad_scale), ms = both(old.m), vs = both(old.v), b1 = both(h.beta1), b2 = both(h.beta2),
+           r1 = both(h.rest1), r2 = both(h.rest2), root = both(c.root_scale), eps = both(h.eps), size = both(-c.step_size),
+           kp = both(keep);
+  float mtop = 0.0f, vtop = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const F2 ge{g[e], g[e + 1]};
-    const F2 me = fma2(k1, {m[e], m[e + 1]}, mul2(g1, ge));
-    const F2 o = mul2(k2, {r[e], r[e + 1]}), q = mul2(g2, ge);
-    const F2 v = fma2(o, o, mul2(q, q));
+    const F2 ge = mul2({g[e], g[e + 1]}, gs);
+    // (The sums are single additions: a packed one is joined with its product into an FMA.)
+    const F2 me = apart(mul2(mul2({m[e], m[e + 1]}, ms), b1), mul2(ge, r1));
+    const F2 o = mul2({r[e], r[e + 1]}, vs);
+    const F2 v = apart(mul2(mul2(o, o), b2), mul2(mul2(ge, ge), r2));
     const F2 re{sqrt_near(v.x), sqrt_near(v.y)};
     const F2 den = fma2(re, root, eps);
     const F2 pe = fma2(mul2(size, me), {rcp_near(den.x), rcp_near(den.y)}, mul2(kp, {p[e], p[e + 1]}));
     m[e] = me.x, m[e + 1] = me.y;
     r[e] = re.x, r[e + 1] = re.y;
+    g[e] = v.x, g[e + 1] = v.y;
     p[e] = pe.x, p[e + 1] = pe.y;
     mtop = top_of(mtop, fabsf(me.x), fabsf(me.y));
-    rtop = top_of(rtop, re.x, re.y);
+    vtop = top_of(vtop, v.x, v.y);
   }
   const Scales now{at_least(warp_top(mtop) * (1.0f / kTopCode), kLeastScale),
-                   at_least(warp_top(rtop) * (1.0f / kTopCode), kLeastScale)};
-  const float mi = rcp_full(now.m), ri = rcp_full(now.v);
-  const F2 mi2{mi, mi}, ri2{ri, ri};
+                   at_least(sqrtf(warp_top(vtop)) * (1.0f / kTopCode), kLeastScale)};
+  const F2 mi = both(rcp_near(now.m)), ri = both(rcp_near(now.v));
+  unsigned nearest = 0xffffffffu;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const F2 me = mul2(mi2, {m[e], m[e + 1]}), re = mul2(ri2, {r[e], r[e + 1]});
-    m[e] = me.x, m[e + 1] = me.y;
-    r[e] = re.x > 0.0f ? at_least(re.x, kLeastCode) : re.x;
-    r[e + 1] = re.y > 0.0f ? at_least(re.y, kLeastCode) : re.y;
+    const F2 qm = mul2(mi, {m[e], m[e + 1]}), qr = mul2(ri, {r[e], r[e + 1]});
+    nearest = min(nearest, min(min(half_way(qm.x), half_way(qm.y)), min(half_way(qr.x), half_way(qr.y))));
   }
+  if (nearest > kHalfWay) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const F2 qm = mul2(mi, {m[e], m[e + 1]}), qr = mul2(ri, {r[e], r[e + 1]});
+      m[e] = qm.x, m[e + 1] = qm.y;
+      r[e] = qr.x, r[e + 1] = qr.y;
+    }
+  } else {  // one lane in 4000 or so
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      m[e] = m[e] / now.m;
+      r[e] = sqrtf(g[e]) / now.v;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (g[e] > 0.0f) r[e] = at_least(r[e], kLeastCode);
   return now;
 }
 
@@ -315,7 +330,6 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ A
   const AdamHyper &h = t.h;
   const Now c = constants(h, &sh);
   if (!isfinite(c.grad_scale)) return;
-  const float gain1 = h.rest1 * c.grad_scale, gain2 = h.root_rest2 * c.grad_scale;
   const int64_t pieces = t.first[t.count];
   int k = tensor_of(t.first, t.count, blockIdx.x);
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ A
       take_chunks<G>(s.g, lane, g);
       take_chunks<P>(s.p, lane, p);
       __syncwarp();  // the stage may be filled again
-      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep, gain1, gain2);
+      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep);
       if (lane == u) mine = now;
       *reinterpret_cast<uint2 *>(w.m + i) = encode8(m);
       *reinterpret_cast<uint2 *>(w.v + i) = encode8(r);
@@ -379,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ A
         m[e] = e < rest ? from_code(w.m[i + e]) : 0.0f;
         r[e] = e < rest ? from_code(w.v[i + e]) : 0.0f;
       }
-      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep, gain1, gain2);
+      const Scales now = step8(p, g, m, r, scales(u), c, h, w.keep);
       if (lane == u) mine = now;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -486,7 +500,6 @@ cudaError_t launch_adamw(const AdamWProblem &p, cudaStream_t s) {
   AdamHyper h{};
   h.beta1 = (float)p.beta1, h.beta2 = (float)p.beta2;
   h.rest1 = (float)(1.0 - p.beta1), h.rest2 = (float)(1.0 - p.beta2);
-  h.root_beta2 = (float)sqrt(p.beta2), h.root_rest2 = (float)sqrt(1.0 - p.beta2);
   h.eps = (float)p.eps;
   h.beta1_d = p.beta1, h.beta2_d = p.beta2;
   h.lr = (float)p.lr;
