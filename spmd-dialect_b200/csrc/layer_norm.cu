@@ -31,11 +31,12 @@ constexpr int64_t kLongRun = (int64_t)kLongLanes * kMost;
 template <int MAXT>
 constexpr int kStages = MAXT > kThreads ? 2 : 3;
 
-template <class TX, class TY, int W, int NV, int R, int MAXT, bool WRAPS>
+template <class TX, class TY, int W, int NV, int R, int MAXT, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W * R > 8 ? 2 : 3)
 ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
                   const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int lanes) {
-  constexpr int kBytes = W * sizeof(TX), kPitch = MAXT * kBytes, kStage = R * NV * kPitch;
+  using In = Source<W, NV, MAXT, APART, TX>;
+  constexpr int kStage = R * In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(16) F2 sh[2][32];
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
@@ -43,23 +44,21 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
   const int mine = row_count(i, rows, step), turns = row_count(i - group, rows, step);
   const TX *from = x + (mine ? row_offset(xr.r, i) : 0);
-  const int shift = (int)((uintptr_t)from / sizeof(TX) % W);
-  TY *to = y + (mine ? row_offset(yr.r, i) : 0) + lane * W - shift;
-  from += lane * W - shift;
+  TY *to = y + (mine ? row_offset(yr.r, i) : 0);
+  const int shift = (int)((APART ? (uintptr_t)to / sizeof(TY) : (uintptr_t)from / sizeof(TX)) % W);
   const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
-  int left[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
-  unsigned char *const slots = smem + threadIdx.x * kBytes;
-#pragma unroll
-  for (int q = 0; q < kStages<MAXT> * R; ++q) clear_row<W, NV, kPitch, TX>(slots + q * (NV * kPitch), left);
+  In in;
+  in.place(from, cols, lane, lanes, shift, have, smem, kStages<MAXT> * R, In::kBytes);
+  to += lane * W - shift;
+  from += in.start;
   int stage_in = 0, stage = 0, fetched = 0;  // stages as offsets
   auto fetch = [&] {
+    In::emptied();
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      if (fetched < mine) stream_row<W, NV, kPitch>(slots + stage_in + q * (NV * kPitch), from, lanes, have.full, left);
+      if (fetched < mine) in.fetch(stage_in + q * In::kBytes, from);
       ++fetched;
-      from = next_row<WRAPS>(from, x + lane * W - shift, xr, i + fetched * step);
+      from = next_row<WRAPS>(from, x + in.start, xr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
     stage_in = stage_in == (kStages<MAXT> - 1) * kStage ? 0 : stage_in + kStage;
@@ -83,12 +82,11 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
     F2 v[R][NV][W / 2], t[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      unsigned char *const slot = slots + stage + q * (NV * kPitch);
-      if (!have.full && have.front) clear_front<TX>(slot, shift);
+      in.arrived(stage + q * In::kBytes);
       t[q] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        take_pairs<W, TX>(slot + k * kPitch, v[q][k]);
+        in.take(stage + q * In::kBytes, k, v[q][k]);
 #pragma unroll
         for (int e = 0; e < W / 2; ++e) t[q] = add2(t[q], v[q][k][e]);
       }
@@ -189,7 +187,9 @@ constexpr int kCutStages = 4;
 template <class TX, int W, bool WRAPS>
 __global__ void __launch_bounds__(kThreads, 4)
 ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const __grid_constant__ Cut cut, float4 *shares) {
-  constexpr int NV = kCutMost / W, kBytes = W * sizeof(TX), kPitch = kThreads * kBytes, kStage = NV * kPitch;
+  constexpr int NV = kCutMost / W;
+  using In = Source<W, NV, kThreads, false, TX>;
+  constexpr int kStage = In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   const CutPlace at = cut_place(cut);
   if (at.rows == 0) return;
@@ -201,25 +201,21 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   const int low = at.run == 0 ? 0 : -start, high = cols - first < kRun - start ? (int)(cols - first) : kRun - start;
   // As a row of its own that starts `shift` elements into its first vector.
   const int shift = at.run == 0 ? start : 0, n = high - low;
-  from += first + low + lane * W - shift;
   const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
-  int left[NV];
+  In in;
+  in.place(from + first + low, n, lane, kThreads, shift, have, smem, kCutStages, kStage);
+  from += first + low + in.start;
   float count = 0.0f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    left[k] = vector_left<W>(k, n, lane, kThreads, shift);
-    count += (float)__popc(have.in[k]);
-  }
-  unsigned char *const slots = smem + threadIdx.x * kBytes;
-#pragma unroll
-  for (int q = 0; q < kCutStages; ++q) clear_row<W, NV, kPitch, TX>(slots + q * kStage, left);
+  for (int k = 0; k < NV; ++k) count += (float)__popc(have.in[k]);
   const float inv_count = count > 0.0f ? 1.0f / count : 0.0f, all = warp_sum_f32(count), inv_all = all > 0.0f ? 1.0f / all : 0.0f;
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
-    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, have.full, left);
+    In::emptied();
+    if (fetched < at.rows) in.fetch(stage_in, from);
     copy_commit();
     ++fetched;
-    from = next_row<WRAPS>(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    from = next_row<WRAPS>(from, x + first + low + in.start, xr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -227,11 +223,11 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
     copy_wait<kCutStages - 1>();
-    if (!have.full && have.front) clear_front<TX>(slots + stage, shift);
+    in.arrived(stage);
     F2 v[NV][W / 2], t{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      take_pairs<W, TX>(slots + stage + k * kPitch, v[k]);
+      in.take(stage, k, v[k]);
 #pragma unroll
       for (int e = 0; e < W / 2; ++e) t = add2(t, v[k][e]);
     }
@@ -248,36 +244,36 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
 }
 
 // Second pass: the rows' statistics from the shares, and the output.
-template <class TX, class TY, int W, bool WRAPS>
+template <class TX, class TY, int W, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w, const void *b,
            int wtype, int64_t cols, float eps, float *mean_out, float *rstd_out, const __grid_constant__ Cut cut, const float4 *shares) {
-  constexpr int NV = kCutMost / W, kBytes = W * sizeof(TX), kPitch = kThreads * kBytes, kStage = NV * kPitch;
+  constexpr int NV = kCutMost / W;
+  using In = Source<W, NV, kThreads, APART, TX>;
+  constexpr int kStage = In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 stats[kCutRows];  // -mean, rstd
   const CutPlace at = cut_place(cut);
   if (at.rows == 0) return;
   const int lane = threadIdx.x;
   const TX *from = x + row_offset(xr.r, at.i);
+  TY *to = y + row_offset(yr.r, at.i);
   const int64_t first = at.run * kRun;
-  const int start = (int)((uintptr_t)from / sizeof(TX) % W);
+  const int start = (int)((APART ? (uintptr_t)to / sizeof(TY) : (uintptr_t)from / sizeof(TX)) % W);
   const int low = at.run == 0 ? 0 : -start, high = cols - first < kRun - start ? (int)(cols - first) : kRun - start;
   const int shift = at.run == 0 ? start : 0, n = high - low;
-  TY *to = y + row_offset(yr.r, at.i) + first + low + lane * W - shift;
-  from += first + low + lane * W - shift;
   const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
-  int left[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
-  unsigned char *const slots = smem + threadIdx.x * kBytes;
-#pragma unroll
-  for (int q = 0; q < kCutStages; ++q) clear_row<W, NV, kPitch, TX>(slots + q * kStage, left);
+  In in;
+  in.place(from + first + low, n, lane, kThreads, shift, have, smem, kCutStages, kStage);
+  to += first + low + lane * W - shift;
+  from += first + low + in.start;
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
-    if (fetched < at.rows) stream_row<W, NV, kPitch>(slots + stage_in, from, kThreads, have.full, left);
+    In::emptied();
+    if (fetched < at.rows) in.fetch(stage_in, from);
     copy_commit();
     ++fetched;
-    from = next_row<WRAPS>(from, x + first + low + lane * W - shift, xr, at.i + (int64_t)fetched * cut.parts);
+    from = next_row<WRAPS>(from, x + first + low + in.start, xr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kCutStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -309,11 +305,12 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
     copy_wait<kCutStages - 1>();
+    if constexpr (APART) in.arrived(stage);  // elements before a row's start are stored nowhere
     const float2 stat = stats[turn];
     F2 v[NV][W / 2];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      take_pairs<W, TX>(slots + stage + k * kPitch, v[k]);
+      in.take(stage, k, v[k]);
 #pragma unroll
       for (int e = 0; e < W / 2; ++e)
         v[k][e] = fma2(mul2(add2(v[k][e], both(stat.x)), both(stat.y)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
@@ -390,10 +387,10 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
 }
 
 // ---- launches ---------------------------------------------------------------------
-template <class TX, class TY, int NV, int R, int MAXT, bool WRAPS>
+template <class TX, class TY, int NV, int R, int MAXT, bool WRAPS, bool APART>
 cudaError_t stream_rows_as(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, bytes = kStages<MAXT> * R * NV * MAXT * W * (int)sizeof(TX);
-  auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT, WRAPS>;
+  constexpr int W = kWidth<TX, TY>, bytes = kStages<MAXT> * R * Source<W, NV, MAXT, APART, TX>::kBytes;
+  auto kernel = ln_forward_stream<TX, TY, W, NV, R, MAXT, WRAPS, APART>;
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int groups = MAXT / lanes, grid = stream_grid(p.rows, groups, most, W);
   const int64_t step = (int64_t)grid * groups;
@@ -402,47 +399,50 @@ cudaError_t stream_rows_as(const LayerNormProblem &p, int lanes, int most, cudaS
   return cudaGetLastError();
 }
 
-template <class TX, class TY, int NV, int R, int MAXT>
+template <class TX, class TY, int NV, int R, int MAXT, bool APART>
 cudaError_t stream_rows(const LayerNormProblem &p, int lanes, int most, cudaStream_t s) {
-  return p.rows > p.xr.n1 || p.rows > p.yr.n1 ? stream_rows_as<TX, TY, NV, R, MAXT, true>(p, lanes, most, s)
-                                              : stream_rows_as<TX, TY, NV, R, MAXT, false>(p, lanes, most, s);
+  if (APART || p.rows > p.xr.n1 || p.rows > p.yr.n1) return stream_rows_as<TX, TY, NV, R, MAXT, true, APART>(p, lanes, most, s);
+  return stream_rows_as<TX, TY, NV, R, MAXT, APART, APART>(p, lanes, most, s);
 }
 
 // Streamed rows: as many blocks as are resident, or one for each block of rows
 // where those are fewer (then one row at a time).
-template <class TX, class TY>
+template <class TX, class TY, bool APART>
 cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W;
   if (p.cols + spare > kHeld) {
-    if (p.rows <= device_sms()) return stream_rows<TX, TY, NV, 1, kHalfLanes>(p, kHalfLanes, device_sms(), s);
-    return stream_rows<TX, TY, NV, 2, kHalfLanes>(p, kHalfLanes, device_sms(), s);
+    if (p.rows <= device_sms()) return stream_rows<TX, TY, NV, 1, kHalfLanes, APART>(p, kHalfLanes, device_sms(), s);
+    return stream_rows<TX, TY, NV, 2, kHalfLanes, APART>(p, kHalfLanes, device_sms(), s);
   }
-  const int lanes = row_lanes(p.rows, p.cols, W, kMost, spare), groups = kThreads / lanes;
+  int lanes = row_lanes(p.rows, p.cols, W, kMost, spare);
+  if (APART && lanes < 8) lanes = 8;
+  const int groups = kThreads / lanes;
   const int nv = row_vectors(p.cols + spare, lanes, W), most = (nv * W > 8 ? 2 : 3) * device_sms();
-  if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads>(p, lanes, most, s);
-  if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads>(p, lanes, most, s);
+  if (nv == 1) return stream_rows<TX, TY, 1, 1, kThreads, APART>(p, lanes, most, s);
+  if (nv < NV) return stream_rows<TX, TY, 2, 1, kThreads, APART>(p, lanes, most, s);
   if constexpr (sizeof(TX) == 2)
-    if (p.rows > (int64_t)most * groups) return stream_rows<TX, TY, NV, 2, kThreads>(p, lanes, most, s);
-  return stream_rows<TX, TY, NV, 1, kThreads>(p, lanes, most, s);
+    if (p.rows > (int64_t)most * groups) return stream_rows<TX, TY, NV, 2, kThreads, APART>(p, lanes, most, s);
+  return stream_rows<TX, TY, NV, 1, kThreads, APART>(p, lanes, most, s);
 }
 
-template <class TX, class TY, bool WRAPS>
+template <class TX, class TY, bool WRAPS, bool APART>
 cudaError_t forward_cut(const LayerNormProblem &p, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, bytes = kCutStages * kRun * (int)sizeof(TX);
+  constexpr int W = kWidth<TX, TY>, bytes1 = kCutStages * kRun * (int)sizeof(TX);
+  constexpr int bytes2 = kCutStages * Source<W, kCutMost / W, kThreads, APART, TX>::kBytes;
   auto first = ln_moments<TX, W, WRAPS>;
-  auto second = ln_outputs<TX, TY, W, WRAPS>;
-  if (cudaError_t e = allow_shared(first, bytes)) return e;
-  if (cudaError_t e = allow_shared(second, bytes)) return e;
+  auto second = ln_outputs<TX, TY, W, WRAPS, APART>;
+  if (cudaError_t e = allow_shared(first, bytes1)) return e;
+  if (cudaError_t e = allow_shared(second, bytes2)) return e;
   const int64_t runs = most_runs(p.cols), batch = batch_rows(p.rows, p.cols, sizeof(TX));
-  const int period = row_period(p.xr, p.rows, W);
-  const int parts1 = cut_parts(batch, runs, 4 * device_sms(), period), parts2 = cut_parts(batch, runs, 2 * device_sms(), period);
+  const int period_x = row_period(p.xr, p.rows, W), period = APART && row_period(p.yr, p.rows, W) > 1 ? W : period_x;
+  const int parts1 = cut_parts(batch, runs, 4 * device_sms(), period_x), parts2 = cut_parts(batch, runs, 2 * device_sms(), period);
   float4 *shares = static_cast<float4 *>(p.ws);
   for (int64_t row = 0; row < p.rows; row += batch) {
     const int64_t last = row + batch < p.rows ? row + batch : p.rows;
-    first<<<grid_for(runs * parts1), kThreads, bytes, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, parts1), p.cols,
+    first<<<grid_for(runs * parts1), kThreads, bytes1, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, parts1), p.cols,
                                                            Cut{row, last, runs, parts1}, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
-    second<<<grid_for(runs * parts2), kThreads, bytes, s>>>(
+    second<<<grid_for(runs * parts2), kThreads, bytes2, s>>>(
         static_cast<const TX *>(p.x), row_walk(p.xr, parts2), static_cast<TY *>(p.y), row_walk(p.yr, parts2), p.w,
         p.b, p.wtype, p.cols, p.eps, p.mean, p.rstd, Cut{row, last, runs, parts2}, shares);
     if (cudaError_t e = cudaGetLastError()) return e;
@@ -480,11 +480,15 @@ cudaError_t long_rows(const LayerNormProblem &p, cudaStream_t s) {
 template <class TX, class TY>
 cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W;
-  const int spare = vec_rows(p.x, p.xr, p.rows, sizeof(TX), W) ? 0 : W - 1;
-  if (p.xr.sc == 1 && p.yr.sc == 1 && same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
-    return p.cols + spare <= kHalfHeld ? forward_streamed<TX, TY>(p, spare, s)
-           : p.rows > p.xr.n1 || p.rows > p.yr.n1 ? forward_cut<TX, TY, true>(p, s)
-                                                  : forward_cut<TX, TY, false>(p, s);
+  if (steady(p.xr, p.rows, W) && steady(p.yr, p.rows, W)) {
+    const int spare = vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) ? 0 : W - 1;
+    const bool held = p.cols + spare <= kHalfHeld;
+    if (!same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
+      return held ? forward_streamed<TX, TY, true>(p, spare, s) : forward_cut<TX, TY, true, true>(p, s);
+    return held ? forward_streamed<TX, TY, false>(p, spare, s)
+           : p.rows > p.xr.n1 || p.rows > p.yr.n1 ? forward_cut<TX, TY, true, false>(p, s)
+                                                  : forward_cut<TX, TY, false, false>(p, s);
+  }
   if (p.cols > kHeld) return long_rows<TX, TY>(p, s);
   const int lanes = row_lanes(p.rows, p.cols, W, kMost, 0), nv = row_vectors(p.cols, lanes, W);
   if (nv == 1) return strided_rows<TX, TY, 1>(p, lanes, s);

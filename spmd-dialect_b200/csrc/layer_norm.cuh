@@ -224,38 +224,6 @@ template <int W>
 __device__ __forceinline__ int shifted(int k, int e, int lane, int lanes, int shift) {
   return column<W, true>(k, e, lane, lanes, shift);
 }
-// Elements of vector k that a row has, from the vector's start: one that holds the
-// row's start is read from there, in the same aligned 16 bytes, so in the same
-// allocation; of one that holds its end only the row's are read.
-template <int W>
-__device__ __forceinline__ int vector_left(int k, int cols, int lane, int lanes, int shift) {
-  const int left = cols - shifted<W>(k, 0, lane, lanes, shift);
-  return left < 0 ? 0 : left < W ? left : W;
-}
-// Starts the copies of a row's vectors into a thread's slots, `PITCH` bytes apart;
-// what a vector past the row's end does not have of it becomes zero.  Slots of
-// vectors that have nothing of it are zero from the start.  `full`: the warp's
-// vectors are all whole.
-template <int W, int NV, int PITCH, class T>
-__device__ __forceinline__ void stream_row(unsigned char *slot, const T *vector, int lanes, bool full, const int (&left)[NV]) {
-  if (full) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) copy_async<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W);
-  } else {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (left[k]) copy_async_part<W * sizeof(T)>(slot + k * PITCH, vector + k * lanes * W, left[k] * (int)sizeof(T));
-  }
-}
-template <int W, int NV, int PITCH, class T>
-__device__ __forceinline__ void clear_row(unsigned char *slot, const int (&left)[NV]) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (!left[k]) {
-#pragma unroll
-      for (int q = 0; q < W * (int)sizeof(T); q += 8) *reinterpret_cast<uint2 *>(slot + k * PITCH + q) = make_uint2(0, 0);
-    }
-}
 // Bit e: whether element e of vector k is in the row.
 template <int W>
 __device__ __forceinline__ unsigned inside(int k, int cols, int lane, int lanes, int shift) {
@@ -288,20 +256,148 @@ __device__ __forceinline__ Held<W, NV> held(int cols, int lane, int lanes, int s
   h.front = lane == 0 && shift > 0 && shift < W;
   return h;
 }
-// A vector out of a thread's slot as pairs.  What of another row is before this
-// one's start is made zero first, so that sums need no tests.
+// Elements `off` to off + W of two vectors side by side.
 template <int W, class T>
-__device__ __forceinline__ void take_pairs(const unsigned char *slot, F2 (&v)[W / 2]) {
-  float f[W];
-  take_vec<W, T>(slot, f);
+__device__ __forceinline__ void take_across(const unsigned char *slot, int off, float (&f)[W]) {
+  constexpr int N = W * sizeof(T) / 4;
+  unsigned w[2 * N];
 #pragma unroll
-  for (int e = 0; e < W / 2; ++e) v[e] = {f[2 * e], f[2 * e + 1]};
+  for (int q = 0; q < 2 * N; q += N) {
+    if constexpr (N == 4) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(slot + q * 4);
+      w[q] = u.x, w[q + 1] = u.y, w[q + 2] = u.z, w[q + 3] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2 *>(slot + q * 4);
+      w[q] = u.x, w[q + 1] = u.y;
+    }
+  }
+  const int words = off * (int)sizeof(T) / 4;
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int q = 0; q < 2 * N - o; ++q) w[q] = words & o ? w[q + o] : w[q];
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const float2 p = unpack(__funnelshift_r(w[q], w[q + 1], 16 * (off & 1)), T{});
+      f[2 * q] = p.x, f[2 * q + 1] = p.y;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < N; ++q) f[q] = __uint_as_float(w[q]);
+  }
 }
-template <class T>
-__device__ __forceinline__ void clear_front(unsigned char *slot, int shift) {
+
+// An input's vectors on their way through shared memory: the copies of a row's
+// vectors go to a thread's slots, kPitch bytes apart.  Vectors are laid out by where
+// the output's rows start.  APART: an input's rows may start elsewhere within a
+// vector.  Then a thread copies the aligned vector that holds its first element and
+// takes its own out of that and the next thread's, `off` elements on; the last
+// thread of a warp (or of a narrower row) copies that next vector too, into a slot
+// of its own.  Rows have eight lanes at least there.
+template <int W, int NV, int THREADS, bool APART, class T>
+struct Source {
+  static constexpr int kVec = W * sizeof(T), kPitch = (APART ? THREADS / 8 * 9 : THREADS) * kVec, kBytes = NV * kPitch;
+  unsigned char *slot;
+  int start;  // the first copy's column
+  int off, front, lanes;  // front: elements before the row's start in the thread's first vector
+  int left[NV], after[APART ? NV : 1];
+  bool full, last;
+
+  // Elements of the vector at column c to copy.  One that holds the row's start is
+  // read from its own, in the same aligned 16 bytes, so in the same allocation; of one
+  // that holds the row's end only the row's are read.
+  static __device__ __forceinline__ int to_copy(int c, int cols) { return c <= -W || c >= cols ? 0 : cols - c < W ? cols - c : W; }
+
+  // `row`: column 0; `area`: kBytes for each of `stages`.
+  __device__ __forceinline__ void place(const T *row, int cols, int lane, int row_lanes, int shift, const Held<W, NV> &have,
+                                        unsigned char *area, int stages, int stage_bytes) {
+    const int t = threadIdx.x, width = row_lanes < 32 ? row_lanes : 32;
+    lanes = row_lanes;
+    off = 0;
+    if constexpr (APART) {
+      off = (int)((uintptr_t)row / sizeof(T) % W) - shift;
+      off += off < 0 ? W : 0;
+    }
+    start = lane * W - shift - off;
+    front = have.front ? shift : 0;
+    slot = area + (APART ? t + t / width : t) * kVec;
+    full = have.full;
+    bool whole = true;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      left[k] = to_copy(start + k * lanes * W, cols);
+      whole &= left[k] == W;
+    }
+    if constexpr (APART) {
+      full = __all_sync(0xffffffffu, whole);
+      last = (t & (width - 1)) == width - 1;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) after[k] = last ? to_copy(start + k * lanes * W + W, cols) : 0;
+    }
+    // Slots of vectors that have nothing of the row are zero from the start.
+    for (int s = 0; s < stages; ++s)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (!left[k]) clear(slot + s * stage_bytes + k * kPitch);
+        if constexpr (APART)
+          if (last && !after[k]) clear(slot + s * stage_bytes + k * kPitch + kVec);
+      }
+  }
+  static __device__ __forceinline__ void clear(unsigned char *p) {
+#pragma unroll
+    for (int q = 0; q < kVec; q += 8) *reinterpret_cast<uint2 *>(p + q) = make_uint2(0, 0);
+  }
+  // The copies of a row into the stage `at` bytes on; what a vector past the row's end
+  // does not have of it becomes zero.  `from`: the row's column `start`.
+  __device__ __forceinline__ void fetch(int at, const T *from) const {
+    if (full) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) copy_async<kVec>(slot + at + k * kPitch, from + k * lanes * W);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (left[k]) copy_async_part<kVec>(slot + at + k * kPitch, from + k * lanes * W, left[k] * (int)sizeof(T));
+    }
+    if constexpr (APART) {
+      if (last) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          if (after[k]) copy_async_part<kVec>(slot + at + k * kPitch + kVec, from + k * lanes * W + W, after[k] * (int)sizeof(T));
+      }
+    }
+  }
+  // Once a stage is there.  What of another row is before this one's start becomes
+  // zero, so that sums need no tests (APART: as it is taken).
+  __device__ __forceinline__ void arrived(int at) const {
+    if constexpr (APART) {
+      __syncwarp();  // the next thread's copies are there too
+    } else if (!full && front) {
 #pragma unroll 1
-  for (int e = 0; e < shift; ++e) reinterpret_cast<T *>(slot)[e] = from_f32<T>(0.0f);
-}
+      for (int e = 0; e < front; ++e) reinterpret_cast<T *>(slot + at)[e] = from_f32<T>(0.0f);
+    }
+  }
+  // Before a stage is filled again.
+  static __device__ __forceinline__ void emptied() {
+    if constexpr (APART) __syncwarp();
+  }
+  // Vector k of a stage, as pairs.
+  __device__ __forceinline__ void take(int at, int k, F2 (&v)[W / 2]) const {
+    float f[W];
+    if constexpr (APART) {
+      take_across<W, T>(slot + at + k * kPitch, off, f);
+      if (k == 0 && front) {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (e < front) f[e] = 0.0f;
+      }
+    } else {
+      take_vec<W, T>(slot + at + k * kPitch, f);
+    }
+#pragma unroll
+    for (int e = 0; e < W / 2; ++e) v[e] = {f[2 * e], f[2 * e + 1]};
+  }
+};
 // A row's vectors to memory: whole ones at once, the others element by element.
 template <int W, int NV, class T>
 __device__ __forceinline__ void stream_store(T *vector, const Held<W, NV> &have, int lanes, const F2 (&v)[NV][W / 2]) {
@@ -416,6 +512,11 @@ inline bool same_shift(const void *p, const Rows &r, int p_size, const void *q, 
          (rows < 2 || ((uint64_t)(r.s1 - t.s1) % uw == 0 && (rows <= r.n1 && rows <= t.n1)) ||
           ((uint64_t)r.s1 % uw == 0 && (uint64_t)t.s1 % uw == 0 && (rows <= r.n1 || (uint64_t)r.s0 % uw == 0) &&
            (rows <= t.n1 || (uint64_t)t.s0 % uw == 0)));
+}
+
+// Rows whose starts within a vector of w come around after w of them, or sooner.
+inline bool steady(const Rows &r, int64_t rows, int w) {
+  return r.sc == 1 && (rows <= r.n1 || ((uint64_t)r.s0 % w == 0 && ((uint64_t)r.s1 % w == 0 || r.n1 % w == 0)));
 }
 
 inline int device_sms() {

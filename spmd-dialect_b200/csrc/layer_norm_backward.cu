@@ -119,14 +119,17 @@ constexpr int kStages = 3;
 template <class TX, class TY>
 constexpr int kRowsAtOnce = sizeof(TX) + sizeof(TY) <= 6 ? 2 : 1;  // as two blocks' stages fit an SM
 
-template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES, bool WRAPS>
+template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3)
 ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
                    const __grid_constant__ RowWalk dr, int lanes) {
-  constexpr int kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kRow = NV * MAXT * (kXBytes + kGBytes), kStage = R * kRow;
+  using InX = Source<W, NV, MAXT, APART, TX>;
+  using InG = Source<W, NV, MAXT, APART, TY>;
+  constexpr int kRow = InX::kBytes + InG::kBytes, kStage = R * kRow;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(16) float4 sh[2][32];
-  __shared__ float2 stats[STAGES * R][MAXT];  // a group's row, or a warp's where the group is wider
+  constexpr int kSlots = MAXT > kThreads ? MAXT / 32 : APART ? MAXT / 8 : MAXT;
+  __shared__ float2 stats[STAGES * R][kSlots];  // a group's row, or a warp's where the group is wider
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols, slot = lanes <= 32 ? group : threadIdx.x >> 5;
   const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
@@ -134,29 +137,27 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
   const int mine = row_count(i, p.rows, step), turns = row_count(i - group, p.rows, step);
   const TX *x_from = p.x + (mine ? row_offset(xr.r, i) : 0);
-  const int shift = (int)((uintptr_t)x_from / sizeof(TX) % W);
-  const int64_t start = lane * W - shift;  // of the thread's first vector in a row
-  const TY *g_from = p.dy + (mine ? row_offset(gr.r, i) : 0) + start;
-  TX *to = p.dx + (mine && p.dx ? row_offset(dr.r, i) : 0) + start;
-  x_from += start;
+  const TY *g_from = p.dy + (mine ? row_offset(gr.r, i) : 0);
+  TX *to = p.dx + (mine && p.dx ? row_offset(dr.r, i) : 0);
+  const int shift = (int)((uintptr_t)(APART && p.dx ? to : x_from) / sizeof(TX) % W);
   const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
-  int left[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, cols, lane, lanes, shift);
-  unsigned char *const x_slots = smem + threadIdx.x * kXBytes, *const g_slots = smem + NV * MAXT * kXBytes + threadIdx.x * kGBytes;
-#pragma unroll
-  for (int q = 0; q < STAGES * R; ++q) {
-    clear_row<W, NV, MAXT * kXBytes, TX>(x_slots + q * kRow, left);
-    clear_row<W, NV, MAXT * kGBytes, TY>(g_slots + q * kRow, left);
-  }
+  InX in_x;
+  InG in_g;
+  in_x.place(x_from, cols, lane, lanes, shift, have, smem, STAGES * R, kRow);
+  in_g.place(g_from, cols, lane, lanes, shift, have, smem + InX::kBytes, STAGES * R, kRow);
+  const int64_t start = lane * W - shift;  // of the thread's first vector in a row
+  x_from += in_x.start;
+  g_from += in_g.start;
+  to += start;
   int stage_in = 0, stage = 0, fetched = 0;
   const float *mean_in = p.mean + i, *rstd_in = p.rstd + i;
   auto fetch = [&] {
+    InX::emptied();
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       if (fetched < mine) {
-        stream_row<W, NV, MAXT * kXBytes>(x_slots + stage_in * kStage + q * kRow, x_from, lanes, have.full, left);
-        stream_row<W, NV, MAXT * kGBytes>(g_slots + stage_in * kStage + q * kRow, g_from, lanes, have.full, left);
+        in_x.fetch(stage_in * kStage + q * kRow, x_from);
+        in_g.fetch(stage_in * kStage + q * kRow, g_from);
         if (first) {
           copy_async<4>(&stats[stage_in * R + q][slot].x, mean_in);
           copy_async<4>(&stats[stage_in * R + q][slot].y, rstd_in);
@@ -164,8 +165,8 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
       }
       ++fetched;
       mean_in += step, rstd_in += step;
-      x_from = next_row<WRAPS>(x_from, p.x + start, xr, i + fetched * step);
-      g_from = next_row<WRAPS>(g_from, p.dy + start, gr, i + fetched * step);
+      x_from = next_row<WRAPS>(x_from, p.x + in_x.start, xr, i + fetched * step);
+      g_from = next_row<WRAPS>(g_from, p.dy + in_g.start, gr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
@@ -190,18 +191,16 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
     for (int q = 0; q < R; ++q) {
       // An element outside the row, or of a row past the last, has g = 0 and a finite x: it adds nothing to any sum.
       const bool live = turn + q < mine;
-      unsigned char *const xs = x_slots + stage * kStage + q * kRow, *const gs = g_slots + stage * kStage + q * kRow;
+      const int here = stage * kStage + q * kRow;
       stat[q] = live ? stats[stage * R + q][slot] : make_float2(0.0f, 0.0f);
-      if (!have.full && have.front) {
-        clear_front<TX>(xs, shift);
-        clear_front<TY>(gs, shift);
-      }
+      in_x.arrived(here);
+      in_g.arrived(here);
       F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         F2 x[W / 2], g[W / 2];
-        take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x);
-        take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g);
+        in_x.take(here, k, x);
+        in_g.take(here, k, g);
 #pragma unroll
         for (int e = 0; e < W / 2; ++e) {
           const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
@@ -222,13 +221,13 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
     for (int q = 0; q < R; ++q) {
       if (turn + q < mine) {
         const F2 c1 = both(-c[q].x * inv_n), c2 = both(-c[q].y * inv_n);
-        unsigned char *const xs = x_slots + stage * kStage + q * kRow, *const gs = g_slots + stage * kStage + q * kRow;
+        const int here = stage * kStage + q * kRow;
         F2 g[NV][W / 2];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
           F2 x[W / 2];
-          take_pairs<W, TX>(xs + k * (MAXT * kXBytes), x);
-          take_pairs<W, TY>(gs + k * (MAXT * kGBytes), g[k]);
+          in_x.take(here, k, x);
+          in_g.take(here, k, g[k]);
 #pragma unroll
           for (int e = 0; e < W / 2; ++e) {
             const F2 xh = mul2(add2(x[e], both(-stat[q].x)), both(stat[q].y));
@@ -259,11 +258,14 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
 }
 
 // Longer rows (layer_norm.cuh), first pass: each warp's share of a row's two sums.
-template <class TX, class TY, int W, bool WRAPS>
+template <class TX, class TY, int W, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
           const __grid_constant__ Cut cut, float2 *shares) {
-  constexpr int NV = kCutMost / W, kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * kThreads * (kXBytes + kGBytes);
+  constexpr int NV = kCutMost / W;
+  using InX = Source<W, NV, kThreads, false, TX>;  // there is no output: as x has it
+  using InG = Source<W, NV, kThreads, APART, TY>;
+  constexpr int kStage = InX::kBytes + InG::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 stats[kCutRows];
   const CutPlace at = cut_place(cut);
@@ -275,29 +277,25 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   const int begin = (int)((uintptr_t)x_from / sizeof(TX) % W);
   const int low = at.run == 0 ? 0 : -begin, high = p.cols - first < kRun - begin ? (int)(p.cols - first) : kRun - begin;
   const int shift = at.run == 0 ? begin : 0, n = high - low;
-  const int64_t start = first + low + lane * W - shift;
-  const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
-  x_from += start;
+  const TY *g_from = p.dy + row_offset(gr.r, at.i);
   const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
-  int left[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
-  unsigned char *const x_slots = smem + lane * kXBytes, *const g_slots = smem + NV * kThreads * kXBytes + lane * kGBytes;
-#pragma unroll
-  for (int q = 0; q < kStages; ++q) {
-    clear_row<W, NV, kThreads * kXBytes, TX>(x_slots + q * kStage, left);
-    clear_row<W, NV, kThreads * kGBytes, TY>(g_slots + q * kStage, left);
-  }
+  InX in_x;
+  InG in_g;
+  in_x.place(x_from + first + low, n, lane, kThreads, shift, have, smem, kStages, kStage);
+  in_g.place(g_from + first + low, n, lane, kThreads, shift, have, smem + InX::kBytes, kStages, kStage);
+  x_from += first + low + in_x.start;
+  g_from += first + low + in_g.start;
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
+    InG::emptied();
     if (fetched < at.rows) {
-      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, have.full, left);
-      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, have.full, left);
+      in_x.fetch(stage_in, x_from);
+      in_g.fetch(stage_in, g_from);
     }
     copy_commit();
     ++fetched;
-    x_from = next_row<WRAPS>(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
-    g_from = next_row<WRAPS>(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    x_from = next_row<WRAPS>(x_from, p.x + first + low + in_x.start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row<WRAPS>(g_from, p.dy + first + low + in_g.start, gr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -310,16 +308,14 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
     fetch();
     copy_wait<kStages - 1>();
     const float2 stat = stats[turn];
-    if (!have.full && have.front) {
-      clear_front<TX>(x_slots + stage, shift);
-      clear_front<TY>(g_slots + stage, shift);
-    }
+    in_x.arrived(stage);
+    in_g.arrived(stage);
     F2 s1{0.0f, 0.0f}, s2{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       F2 x[W / 2], g[W / 2];
-      take_pairs<W, TX>(x_slots + stage + k * (kThreads * kXBytes), x);
-      take_pairs<W, TY>(g_slots + stage + k * (kThreads * kGBytes), g);
+      in_x.take(stage, k, x);
+      in_g.take(stage, k, g);
 #pragma unroll
       for (int e = 0; e < W / 2; ++e) {
         const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
@@ -337,11 +333,14 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
 
 // Second pass: dx and the column sums, which go on from what the batches before
 // left in the part's partial row.
-template <class TX, class TY, int W, bool WRAPS>
+template <class TX, class TY, int W, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
          const __grid_constant__ RowWalk dr, const __grid_constant__ Cut cut, const float2 *shares) {
-  constexpr int NV = kCutMost / W, kXBytes = W * sizeof(TX), kGBytes = W * sizeof(TY), kStage = NV * kThreads * (kXBytes + kGBytes);
+  constexpr int NV = kCutMost / W;
+  using InX = Source<W, NV, kThreads, APART, TX>;
+  using InG = Source<W, NV, kThreads, APART, TY>;
+  constexpr int kStage = InX::kBytes + InG::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float4 stats[kCutRows];  // -mean, rstd, -c1, -c2
   const CutPlace at = cut_place(cut);
@@ -349,34 +348,32 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
   const int lane = threadIdx.x;
   const float inv_n = 1.0f / (float)p.cols;
   const TX *x_from = p.x + row_offset(xr.r, at.i);
+  TX *to = p.dx + (p.dx ? row_offset(dr.r, at.i) : 0);
   const int64_t first = at.run * kRun, part = blockIdx.x / cut.runs;
-  const int begin = (int)((uintptr_t)x_from / sizeof(TX) % W);
+  const int begin = (int)((uintptr_t)(APART && p.dx ? to : x_from) / sizeof(TX) % W);
   const int low = at.run == 0 ? 0 : -begin, high = p.cols - first < kRun - begin ? (int)(p.cols - first) : kRun - begin;
   const int shift = at.run == 0 ? begin : 0, n = high - low;
+  const TY *g_from = p.dy + row_offset(gr.r, at.i);
   const int64_t start = first + low + lane * W - shift;
-  const TY *g_from = p.dy + row_offset(gr.r, at.i) + start;
-  TX *to = p.dx + (p.dx ? row_offset(dr.r, at.i) : 0) + start;
-  x_from += start;
   const Held<W, NV> have = held<W, NV>(n, lane, kThreads, shift);
-  int left[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) left[k] = vector_left<W>(k, n, lane, kThreads, shift);
-  unsigned char *const x_slots = smem + lane * kXBytes, *const g_slots = smem + NV * kThreads * kXBytes + lane * kGBytes;
-#pragma unroll
-  for (int q = 0; q < kStages; ++q) {
-    clear_row<W, NV, kThreads * kXBytes, TX>(x_slots + q * kStage, left);
-    clear_row<W, NV, kThreads * kGBytes, TY>(g_slots + q * kStage, left);
-  }
+  InX in_x;
+  InG in_g;
+  in_x.place(x_from + first + low, n, lane, kThreads, shift, have, smem, kStages, kStage);
+  in_g.place(g_from + first + low, n, lane, kThreads, shift, have, smem + InX::kBytes, kStages, kStage);
+  x_from += first + low + in_x.start;
+  g_from += first + low + in_g.start;
+  to += start;
   int stage_in = 0, stage = 0, fetched = 0;
   auto fetch = [&] {
+    InG::emptied();
     if (fetched < at.rows) {
-      stream_row<W, NV, kThreads * kXBytes>(x_slots + stage_in, x_from, kThreads, have.full, left);
-      stream_row<W, NV, kThreads * kGBytes>(g_slots + stage_in, g_from, kThreads, have.full, left);
+      in_x.fetch(stage_in, x_from);
+      in_g.fetch(stage_in, g_from);
     }
     copy_commit();
     ++fetched;
-    x_from = next_row<WRAPS>(x_from, p.x + start, xr, at.i + (int64_t)fetched * cut.parts);
-    g_from = next_row<WRAPS>(g_from, p.dy + start, gr, at.i + (int64_t)fetched * cut.parts);
+    x_from = next_row<WRAPS>(x_from, p.x + first + low + in_x.start, xr, at.i + (int64_t)fetched * cut.parts);
+    g_from = next_row<WRAPS>(g_from, p.dy + first + low + in_g.start, gr, at.i + (int64_t)fetched * cut.parts);
     stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
@@ -416,16 +413,14 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
     fetch();
     copy_wait<kStages - 1>();
     const float4 stat = stats[turn];
-    if (!have.full && have.front) {
-      clear_front<TX>(x_slots + stage, shift);
-      clear_front<TY>(g_slots + stage, shift);
-    }
+    in_x.arrived(stage);
+    in_g.arrived(stage);
     F2 g[NV][W / 2];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       F2 x[W / 2];
-      take_pairs<W, TX>(x_slots + stage + k * (kThreads * kXBytes), x);
-      take_pairs<W, TY>(g_slots + stage + k * (kThreads * kGBytes), g[k]);
+      in_x.take(stage, k, x);
+      in_g.take(stage, k, g[k]);
 #pragma unroll
       for (int e = 0; e < W / 2; ++e) {
         const F2 xh = mul2(add2(x[e], both(stat.x)), both(stat.y));
@@ -598,12 +593,12 @@ bool wraps(const Back<TX, TY> &b) {
   return b.rows > b.xr.n1 || b.rows > b.gr.n1 || (b.dx && b.rows > b.dr.n1);
 }
 
-template <class TX, class TY, int NV, int MAXT, bool WRAPS>
+template <class TX, class TY, int NV, int MAXT, bool WRAPS, bool APART>
 cudaError_t stream_rows_as(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;
-  constexpr int staged = stages * R * NV * MAXT * W * (int)(sizeof(TX) + sizeof(TY));
+  constexpr int staged = stages * R * (Source<W, NV, MAXT, APART, TX>::kBytes + Source<W, NV, MAXT, APART, TY>::kBytes);
   const int sums = b.part ? (int)(MAXT / lanes * b.cols * sizeof(float)) : 0, bytes = staged > sums ? staged : sums;
-  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages, WRAPS>;
+  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages, WRAPS, APART>;
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int64_t groups = MAXT / lanes;
   const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
@@ -613,64 +608,94 @@ cudaError_t stream_rows_as(const Back<TX, TY> &b, int lanes, int *parts, cudaStr
   return cudaGetLastError();
 }
 
-template <class TX, class TY, int NV, int MAXT>
+template <class TX, class TY, int NV, int MAXT, bool APART>
 cudaError_t stream_rows(const Back<TX, TY> &b, int lanes, int *parts, cudaStream_t s) {
-  return wraps(b) ? stream_rows_as<TX, TY, NV, MAXT, true>(b, lanes, parts, s) : stream_rows_as<TX, TY, NV, MAXT, false>(b, lanes, parts, s);
+  if (APART || wraps(b)) return stream_rows_as<TX, TY, NV, MAXT, true, APART>(b, lanes, parts, s);
+  return stream_rows_as<TX, TY, NV, MAXT, APART, APART>(b, lanes, parts, s);
+}
+template <class TX, class TY, bool APART>
+cudaError_t backward_streamed(const Back<TX, TY> &b, int spare, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, NV = kMost / W;
+  if (b.cols + spare > kThreads * kMost) return stream_rows<TX, TY, NV, kWideLanes, APART>(b, kWideLanes, parts, s);
+  int lanes = row_lanes(b.rows, b.cols, W, kMost, spare);
+  if (APART && lanes < 8) lanes = 8;
+  const int nv = row_vectors(b.cols + spare, lanes, W);
+  if (nv == 1) return stream_rows<TX, TY, 1, kThreads, APART>(b, lanes, parts, s);
+  if (nv < NV) return stream_rows<TX, TY, 2, kThreads, APART>(b, lanes, parts, s);
+  return stream_rows<TX, TY, NV, kThreads, APART>(b, lanes, parts, s);
 }
 
-template <class TX, class TY, bool WRAPS>
-cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, bool vectors, int *parts, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, bytes = kStages * kRun * (int)(sizeof(TX) + sizeof(TY));
-  auto shares_of = ln_shares<TX, TY, W, WRAPS>;
-  auto grads_of = ln_grads<TX, TY, W, WRAPS>;
-  if (vectors) {
-    if (cudaError_t e = allow_shared(shares_of, bytes)) return e;
-    if (cudaError_t e = allow_shared(grads_of, bytes)) return e;
-  }
-  const int64_t runs = most_runs(b.cols), batch = batch_rows(b.rows, b.cols, sizeof(TX) + sizeof(TY));
-  const int period = vectors ? row_period(b.xr, b.rows, W) : 1;
-  const int parts1 = cut_parts(batch, runs, kShareBlocks, period), parts2 = cut_parts(batch, runs, kGradBlocks, period);
-  float2 *shares = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)parts2 * 2 * b.cols * sizeof(float)));
-  *parts = parts2;
-  for (int64_t row = 0; row < b.rows; row += batch) {
-    const int64_t last = row + batch < b.rows ? row + batch : b.rows;
-    const Cut cut1{row, last, runs, parts1}, cut2{row, last, runs, parts2};
-    const unsigned grid1 = grid_for(runs * parts1), grid2 = grid_for(runs * parts2);
-    if (b.dx) {
-      if (vectors)
-        shares_of<<<grid1, kThreads, bytes, s>>>(b, row_walk(b.gr, parts1), row_walk(b.xr, parts1), cut1, shares);
-      else
-        ln_strided_shares<TX, TY, W><<<grid1, kThreads, 0, s>>>(b, cut1, shares);
+// Two passes over each batch of longer rows: shares(cut, grid), where dx is wanted,
+// and grads(cut, grid).
+template <class Shares, class Grads>
+cudaError_t batches(int64_t rows, int64_t batch, int64_t runs, int parts1, int parts2, bool dx, Shares shares, Grads grads) {
+  for (int64_t row = 0; row < rows; row += batch) {
+    const int64_t last = row + batch < rows ? row + batch : rows;
+    if (dx) {
+      shares(Cut{row, last, runs, parts1}, grid_for(runs * parts1));
       if (cudaError_t e = cudaGetLastError()) return e;
     }
-    if (vectors)
-      grads_of<<<grid2, kThreads, bytes, s>>>(b, row_walk(b.gr, parts2), row_walk(b.xr, parts2),
-                                              row_walk(b.dr, parts2), cut2, shares);
-    else
-      ln_strided_grads<TX, TY, W><<<grid2, kThreads, 0, s>>>(b, cut2, shares);
+    grads(Cut{row, last, runs, parts2}, grid_for(runs * parts2));
     if (cudaError_t e = cudaGetLastError()) return e;
   }
   return cudaSuccess;
+}
+template <class TX, class TY>
+float2 *shares_room(const Back<TX, TY> &b, void *ws, int parts) {
+  return reinterpret_cast<float2 *>(static_cast<char *>(ws) + round16((size_t)parts * 2 * b.cols * sizeof(float)));
+}
+
+template <class TX, class TY, bool WRAPS, bool APART>
+cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, NV = kCutMost / W, g_bytes = Source<W, NV, kThreads, APART, TY>::kBytes;
+  constexpr int bytes1 = kStages * (Source<W, NV, kThreads, false, TX>::kBytes + g_bytes);
+  constexpr int bytes2 = kStages * (Source<W, NV, kThreads, APART, TX>::kBytes + g_bytes);
+  auto first = ln_shares<TX, TY, W, WRAPS, APART>;
+  auto second = ln_grads<TX, TY, W, WRAPS, APART>;
+  if (cudaError_t e = allow_shared(first, bytes1)) return e;
+  if (cudaError_t e = allow_shared(second, bytes2)) return e;
+  const int64_t runs = most_runs(b.cols), batch = batch_rows(b.rows, b.cols, sizeof(TX) + sizeof(TY));
+  int period = row_period(b.xr, b.rows, W);
+  if (APART && (row_period(b.gr, b.rows, W) > 1 || (b.dx && row_period(b.dr, b.rows, W) > 1))) period = W;
+  const int parts1 = cut_parts(batch, runs, kShareBlocks, period), parts2 = *parts = cut_parts(batch, runs, kGradBlocks, period);
+  float2 *shares = shares_room(b, ws, parts2);
+  return batches(
+      b.rows, batch, runs, parts1, parts2, b.dx,
+      [&](const Cut &cut, unsigned grid) {
+        first<<<grid, kThreads, bytes1, s>>>(b, row_walk(b.gr, parts1), row_walk(b.xr, parts1), cut, shares);
+      },
+      [&](const Cut &cut, unsigned grid) {
+        second<<<grid, kThreads, bytes2, s>>>(b, row_walk(b.gr, parts2), row_walk(b.xr, parts2), row_walk(b.dr, parts2), cut, shares);
+      });
+}
+
+template <class TX, class TY>
+cudaError_t backward_cut_strided(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>;
+  const int64_t runs = most_runs(b.cols), batch = batch_rows(b.rows, b.cols, sizeof(TX) + sizeof(TY));
+  const int parts1 = cut_parts(batch, runs, kShareBlocks, 1), parts2 = *parts = cut_parts(batch, runs, kGradBlocks, 1);
+  float2 *shares = shares_room(b, ws, parts2);
+  return batches(
+      b.rows, batch, runs, parts1, parts2, b.dx,
+      [&](const Cut &cut, unsigned grid) { ln_strided_shares<TX, TY, W><<<grid, kThreads, 0, s>>>(b, cut, shares); },
+      [&](const Cut &cut, unsigned grid) { ln_strided_grads<TX, TY, W><<<grid, kThreads, 0, s>>>(b, cut, shares); });
 }
 
 template <class TX, class TY>
 cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W;
-  const bool vectors = b.xr.sc == 1 && b.gr.sc == 1 && (!b.dx || b.dr.sc == 1) &&
-                       same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
-                       (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W));
-  const int spare = vectors && !vec_rows(b.x, b.xr, b.rows, sizeof(TX), W) ? W - 1 : 0;
-  if (b.cols > kHeld - spare)
-    return wraps(b) ? backward_cut<TX, TY, true>(b, ws, vectors, parts, s) : backward_cut<TX, TY, false>(b, ws, vectors, parts, s);
-  const bool wide = b.cols + spare > kThreads * kMost;
-  const int lanes = wide ? kWideLanes : row_lanes(b.rows, b.cols, W, kMost, spare), nv = row_vectors(b.cols + spare, lanes, W);
-  if (vectors) {
-    if (wide) return stream_rows<TX, TY, NV, kWideLanes>(b, lanes, parts, s);
-    if (nv == 1) return stream_rows<TX, TY, 1, kThreads>(b, lanes, parts, s);
-    if (nv < NV) return stream_rows<TX, TY, 2, kThreads>(b, lanes, parts, s);
-    return stream_rows<TX, TY, NV, kThreads>(b, lanes, parts, s);
+  if (steady(b.xr, b.rows, W) && steady(b.gr, b.rows, W) && (!b.dx || steady(b.dr, b.rows, W))) {
+    const bool same = same_shift(b.x, b.xr, sizeof(TX), b.dy, b.gr, sizeof(TY), b.rows, W) &&
+                      (!b.dx || same_shift(b.x, b.xr, sizeof(TX), b.dx, b.dr, sizeof(TX), b.rows, W));
+    const bool whole = b.dx ? vec_rows(b.dx, b.dr, b.rows, sizeof(TX), W) : vec_rows(b.x, b.xr, b.rows, sizeof(TX), W);
+    const int spare = whole ? 0 : W - 1;
+    if (b.cols + spare <= kHeld) return same ? backward_streamed<TX, TY, false>(b, spare, parts, s) : backward_streamed<TX, TY, true>(b, spare, parts, s);
+    if (!same) return backward_cut<TX, TY, true, true>(b, ws, parts, s);
+    return wraps(b) ? backward_cut<TX, TY, true, false>(b, ws, parts, s) : backward_cut<TX, TY, false, false>(b, ws, parts, s);
   }
-  if (wide) return backward_rows<TX, TY, NV, kWideLanes>(b, lanes, parts, s);
+  if (b.cols > kHeld) return backward_cut_strided(b, ws, parts, s);
+  if (b.cols > kThreads * kMost) return backward_rows<TX, TY, NV, kWideLanes>(b, kWideLanes, parts, s);
+  const int lanes = row_lanes(b.rows, b.cols, W, kMost, 0), nv = row_vectors(b.cols, lanes, W);
   if (nv == 1) return backward_rows<TX, TY, 1, kThreads>(b, lanes, parts, s);
   if (nv < NV) return backward_rows<TX, TY, 2, kThreads>(b, lanes, parts, s);
   return backward_rows<TX, TY, NV, kThreads>(b, lanes, parts, s);

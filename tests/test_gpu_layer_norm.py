@@ -152,6 +152,46 @@ def test_layouts(kernels, dtype, at):
     assert dx is out and bool((buf[~mask] == 7.0).all()), name
 
 
+def within_nan(t, pitch, at):
+    """t's values as a view of a buffer of NaN: rows `pitch` apart, from column `at` on; and the buffer."""
+    *lead, cols = t.shape
+    buf = torch.full((*lead, pitch), float("nan"), device="cuda", dtype=t.dtype)
+    view = buf[..., at:at + cols]
+    view.copy_(t)
+    return view, buf
+
+
+@pytest.mark.parametrize("x_t,y_t", [(F32, F32), (BF16, BF16), (F16, F32), (F32, BF16)])
+@pytest.mark.parametrize("cols", [1, 3, 8, 15, 33, 100, 257, 1001, 2047, 4090, 4096, 5003, 8185, 8192, 9001, 20001, 70000])
+def test_rows_that_start_apart(kernels, x_t, y_t, cols):
+    """Inputs and outputs whose rows start at different places within a vector, all with NaN around them."""
+    for seed, (rows, px, ax, py, ay, pd, ad) in enumerate((
+            ((3,), 5, 1, 0, 0, 0, 0), ((41,), 0, 0, 7, 3, 2, 1), ((2, 21), 9, 2, 3, 0, 8, 5), ((1,), 9, 7, 9, 1, 9, 3))):
+        x, dy = make((*rows, cols), x_t, seed), make((*rows, cols), y_t, seed + 9)
+        w, b = weights(cols, F32, seed + 5)
+        x, _ = within_nan(x, cols + px, ax)
+        dy, _ = within_nan(dy, cols + py, ay)
+        out, out_buf = within_nan(torch.zeros_like(dy), cols + py + 4, ay + 1)
+        dx, dx_buf = within_nan(torch.zeros_like(x), cols + pd, ad)
+        _, mean, rstd = check_forward(kernels, x, w, b, ydtype=y_t, out=out)
+        _, dw, db = check_backward(kernels, dy, x, w, stats=(mean, rstd), dx=dx)
+        for view, buf in ((out, out_buf), (dx, dx_buf)):
+            view.fill_(float("nan"))
+            assert bool(buf.isnan().all())
+        again = kernels.layer_norm_backward(dy, x, mean, rstd, w, dx=dx)
+        assert torch.equal(dw, again[1]) and torch.equal(db, again[2])
+
+
+@pytest.mark.parametrize("rows,cols", [(20011, 1001), (40009, 60), (3001, 4099), (2500, 9001)])
+def test_many_rows_that_start_apart(kernels, rows, cols):
+    """More rows than blocks: a thread's rows come one after another."""
+    x, _ = within_nan(make((rows, cols), BF16, 1), cols + 5, 3)
+    dy, _ = within_nan(make((rows, cols), BF16, 2), cols + 6, 1)
+    w, b = weights(cols, F32, 3)
+    _, mean, rstd = check_forward(kernels, x, w, b)
+    check_backward(kernels, dy, x, w, stats=(mean, rstd))
+
+
 @pytest.mark.parametrize("cols", [64, 1001, 4096, 20000, 100000])
 def test_broadcast_inputs(kernels, cols):
     """Inputs of stride 0: one row for all, one value for a whole row."""
