@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(kThreads, 4) norm_parts(const __grid_constant_
   __shared__ double sh[kThreads / 32];
   const int64_t pieces = t.first[t.count];
   double acc = 0.0;
+  pdl_trigger();
   int k = tensor_of(t.first, t.count, blockIdx.x);
   for (int64_t piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
     while (piece >= t.first[k + 1]) ++k;
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, 4) norm_parts(const __grid_constant_
     else any_piece<__nv_bfloat16>(t.p[k], lo, t.n[k] - lo, acc);
   }
   acc = block_sum(acc, sh);
+  pdl_wait();  // for the list's tables before: the last kernel's end is the call's
   if (threadIdx.x == 0) parts[blockIdx.x] = acc;
 }
 
@@ -110,6 +112,7 @@ __global__ void __launch_bounds__(kThreads) norm_finish(const double *parts, int
                                                         float *scale) {
   __shared__ double sh[kThreads / 32];
   double acc = 0.0;
+  pdl_wait();
   for (int i = threadIdx.x; i < count; i += kThreads) acc += parts[i];
   acc = block_sum(acc, sh);
   if (threadIdx.x == 0) {
@@ -138,8 +141,13 @@ static cudaError_t launch_lists(const GradNormProblem &p, int most, cudaStream_t
     if (t.count == CAP || (k == p.count && t.count > 0)) {
       const int64_t pieces = t.first[t.count];
       const int grid = (int)(pieces < most ? pieces : most);
-      norm_parts<<<grid, kThreads, 0, s>>>(t, p.ws + parts);
-      if (cudaError_t e = cudaGetLastError()) return e;
+      // Tables after the first, and the sum of the parts, start while the one before ends.
+      if (parts == 0) {
+        norm_parts<<<grid, kThreads, 0, s>>>(t, p.ws);
+        if (cudaError_t e = cudaGetLastError()) return e;
+      } else if (cudaError_t e = launch_pdl(norm_parts<CAP>, grid, kThreads, 0, s, t, p.ws + parts)) {
+        return e;
+      }
       parts += grid;
       t.count = 0;
     }
@@ -151,6 +159,7 @@ static cudaError_t launch_lists(const GradNormProblem &p, int most, cudaStream_t
     t.first[t.count + 1] = t.first[t.count] + (p.sizes[k] + kPiece - 1) / kPiece;
     ++t.count;
   }
+  if (parts > 0) return launch_pdl(norm_finish, 1, kThreads, 0, s, (const double *)p.ws, parts, p.max_norm, p.norm, p.scale);
   norm_finish<<<1, kThreads, 0, s>>>(p.ws, parts, p.max_norm, p.norm, p.scale);
   return cudaGetLastError();
 }

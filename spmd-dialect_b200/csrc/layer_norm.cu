@@ -192,7 +192,8 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   constexpr int kStage = In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
   const CutPlace at = cut_place(cut);
-  if (at.rows == 0) return;
+  pdl_trigger();
+  if (at.rows == 0) return pdl_wait();
   const int lane = threadIdx.x;
   const TX *from = x + row_offset(xr.r, at.i);
   const int64_t first = at.run * kRun;
@@ -220,6 +221,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   };
 #pragma unroll
   for (int q = 0; q < kCutStages - 1; ++q) fetch();
+  pdl_wait();  // the shares of the batch before have been read
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
     copy_wait<kCutStages - 1>();
@@ -254,7 +256,8 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 stats[kCutRows];  // -mean, rstd
   const CutPlace at = cut_place(cut);
-  if (at.rows == 0) return;
+  pdl_trigger();
+  if (at.rows == 0) return pdl_wait();
   const int lane = threadIdx.x;
   const TX *from = x + row_offset(xr.r, at.i);
   TY *to = y + row_offset(yr.r, at.i);
@@ -284,6 +287,7 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
     load_weight<W, true>(w, wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, wv[k]);
     load_weight<W, true>(b, wtype, first + low, 0, n, k, lane, kThreads, shift, 0.0f, bv[k]);
   }
+  pdl_wait();  // the shares are there
   for (int r = lane >> 5; r < at.rows; r += kCutWarps) {  // a warp a row, in one order
     const int64_t i = at.i + (int64_t)r * cut.parts;
     Moments m{0.0f, 0.0f, 0.0f};
@@ -439,13 +443,13 @@ cudaError_t forward_cut(const LayerNormProblem &p, cudaStream_t s) {
   float4 *shares = static_cast<float4 *>(p.ws);
   for (int64_t row = 0; row < p.rows; row += batch) {
     const int64_t last = row + batch < p.rows ? row + batch : p.rows;
-    first<<<grid_for(runs * parts1), kThreads, bytes1, s>>>(static_cast<const TX *>(p.x), row_walk(p.xr, parts1), p.cols,
-                                                           Cut{row, last, runs, parts1}, shares);
-    if (cudaError_t e = cudaGetLastError()) return e;
-    second<<<grid_for(runs * parts2), kThreads, bytes2, s>>>(
-        static_cast<const TX *>(p.x), row_walk(p.xr, parts2), static_cast<TY *>(p.y), row_walk(p.yr, parts2), p.w,
-        p.b, p.wtype, p.cols, p.eps, p.mean, p.rstd, Cut{row, last, runs, parts2}, shares);
-    if (cudaError_t e = cudaGetLastError()) return e;
+    if (cudaError_t e = launch(row == 0, first, grid_for(runs * parts1), kThreads, bytes1, s, static_cast<const TX *>(p.x),
+                               row_walk(p.xr, parts1), p.cols, Cut{row, last, runs, parts1}, shares))
+      return e;
+    if (cudaError_t e = launch(false, second, grid_for(runs * parts2), kThreads, bytes2, s, static_cast<const TX *>(p.x),
+                               row_walk(p.xr, parts2), static_cast<TY *>(p.y), row_walk(p.yr, parts2), p.w, p.b, p.wtype,
+                               p.cols, p.eps, p.mean, p.rstd, Cut{row, last, runs, parts2}, shares))
+      return e;
   }
   return cudaSuccess;
 }

@@ -529,6 +529,16 @@ template <class Kernel>
 cudaError_t allow_shared(Kernel kernel, int bytes) {
   return bytes <= 28 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
+// A call's kernels after its first may start while the one before ends: they
+// begin the copies of their inputs, which no kernel of the call writes (dx or y in an
+// input's place: other rows of it), and wait for the one before with them on their way.
+// Every block waits, so that the last kernel's end is the call's.
+template <class... P, class... A>
+cudaError_t launch(bool first, void (*kernel)(P...), unsigned grid, unsigned threads, size_t bytes, cudaStream_t s, A... args) {
+  if (!first) return launch_pdl(kernel, grid, threads, bytes, s, args...);
+  kernel<<<grid, threads, bytes, s>>>(args...);
+  return cudaGetLastError();
+}
 inline unsigned grid_for(int64_t items) { return (unsigned)(items < INT32_MAX ? items : INT32_MAX); }
 
 // Rows whose every vector of w elements is aligned to its size.

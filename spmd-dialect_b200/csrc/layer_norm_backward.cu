@@ -66,6 +66,7 @@ template <class TX, class TY, int W, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back<TX, TY> p, int lanes) {
   extern __shared__ __align__(16) float sums[];
   __shared__ __align__(16) F2 sh[2][32];
+  pdl_trigger();
   const int lane = threadIdx.x & (lanes - 1), groups = blockDim.x / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols;
   const float inv_n = 1.0f / (float)cols;
@@ -132,6 +133,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   __shared__ float2 stats[STAGES * R][kSlots];  // a group's row, or a warp's where the group is wider
   const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
   const int cols = (int)p.cols, slot = lanes <= 32 ? group : threadIdx.x >> 5;
+  pdl_trigger();
   const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
   const float inv_n = 1.0f / (float)cols;
   const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
@@ -269,7 +271,8 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 stats[kCutRows];
   const CutPlace at = cut_place(cut);
-  if (at.rows == 0) return;
+  pdl_trigger();
+  if (at.rows == 0) return pdl_wait();
   const int lane = threadIdx.x;
   for (int r = lane; r < at.rows; r += kThreads) stats[r] = make_float2(-p.mean[at.i + (int64_t)r * cut.parts], p.rstd[at.i + (int64_t)r * cut.parts]);
   const TX *x_from = p.x + row_offset(xr.r, at.i);
@@ -303,6 +306,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   float w[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k) load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
+  pdl_wait();  // the shares of the batch before have been read
   __syncthreads();
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
@@ -344,7 +348,8 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float4 stats[kCutRows];  // -mean, rstd, -c1, -c2
   const CutPlace at = cut_place(cut);
-  if (at.rows == 0) return;
+  pdl_trigger();
+  if (at.rows == 0) return pdl_wait();
   const int lane = threadIdx.x;
   const float inv_n = 1.0f / (float)p.cols;
   const TX *x_from = p.x + row_offset(xr.r, at.i);
@@ -382,8 +387,10 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
   float w[NV][W];
   F2 sw[NV][W / 2], sb[NV][W / 2];
 #pragma unroll
+  for (int k = 0; k < NV; ++k) load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
+  pdl_wait();  // the shares are there, and the partial row
+#pragma unroll
   for (int k = 0; k < NV; ++k) {
-    load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
     float tw[W], tb[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) {
@@ -454,6 +461,8 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_shares(const __grid_co
   constexpr int NV = kCutMost / W;
   __shared__ __align__(16) F2 sh[2][32];
   const CutPlace at = cut_place(cut);
+  pdl_trigger();
+  pdl_wait();
   const int64_t first = at.run * kRun;
   const int n = p.cols - first < kRun ? (p.cols > first ? (int)(p.cols - first) : 0) : kRun;
   for (int turn = 0; turn < at.rows; ++turn) {
@@ -484,6 +493,8 @@ template <class TX, class TY, int W>
 __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ Cut cut, const float2 *shares) {
   constexpr int NV = kCutMost / W;
   const CutPlace at = cut_place(cut);
+  pdl_trigger();
+  pdl_wait();
   if (at.rows == 0) return;
   const int64_t first = at.run * kRun, part = blockIdx.x / cut.runs;
   const int n = p.cols - first < kRun ? (p.cols > first ? (int)(p.cols - first) : 0) : kRun;
@@ -547,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
 __global__ void __launch_bounds__(1024)
 ln_finish(const float *__restrict__ part, int parts, int64_t cols, int depth, void *dw, void *db, int type) {
   __shared__ float sh[2][1024];
+  pdl_wait();
   const int width = blockDim.x / depth, tx = threadIdx.x % width, ty = threadIdx.x / width;
   const int64_t j = (int64_t)blockIdx.x * width + tx;
   float sw = 0.0f, sb = 0.0f;
@@ -625,18 +637,16 @@ cudaError_t backward_streamed(const Back<TX, TY> &b, int spare, int *parts, cuda
   return stream_rows<TX, TY, NV, kThreads, APART>(b, lanes, parts, s);
 }
 
-// Two passes over each batch of longer rows: shares(cut, grid), where dx is wanted,
-// and grads(cut, grid).
+// Two passes over each batch of longer rows: shares(first, cut, grid), where dx is
+// wanted, and grads(first, cut, grid).
 template <class Shares, class Grads>
 cudaError_t batches(int64_t rows, int64_t batch, int64_t runs, int parts1, int parts2, bool dx, Shares shares, Grads grads) {
   for (int64_t row = 0; row < rows; row += batch) {
     const int64_t last = row + batch < rows ? row + batch : rows;
     if (dx) {
-      shares(Cut{row, last, runs, parts1}, grid_for(runs * parts1));
-      if (cudaError_t e = cudaGetLastError()) return e;
+      if (cudaError_t e = shares(row == 0, Cut{row, last, runs, parts1}, grid_for(runs * parts1))) return e;
     }
-    grads(Cut{row, last, runs, parts2}, grid_for(runs * parts2));
-    if (cudaError_t e = cudaGetLastError()) return e;
+    if (cudaError_t e = grads(row == 0 && !dx, Cut{row, last, runs, parts2}, grid_for(runs * parts2))) return e;
   }
   return cudaSuccess;
 }
@@ -661,11 +671,12 @@ cudaError_t backward_cut(const Back<TX, TY> &b, void *ws, int *parts, cudaStream
   float2 *shares = shares_room(b, ws, parts2);
   return batches(
       b.rows, batch, runs, parts1, parts2, b.dx,
-      [&](const Cut &cut, unsigned grid) {
-        first<<<grid, kThreads, bytes1, s>>>(b, row_walk(b.gr, parts1), row_walk(b.xr, parts1), cut, shares);
+      [&](bool at_first, const Cut &cut, unsigned grid) {
+        return launch(at_first, first, grid, kThreads, bytes1, s, b, row_walk(b.gr, parts1), row_walk(b.xr, parts1), cut, shares);
       },
-      [&](const Cut &cut, unsigned grid) {
-        second<<<grid, kThreads, bytes2, s>>>(b, row_walk(b.gr, parts2), row_walk(b.xr, parts2), row_walk(b.dr, parts2), cut, shares);
+      [&](bool at_first, const Cut &cut, unsigned grid) {
+        return launch(at_first, second, grid, kThreads, bytes2, s, b, row_walk(b.gr, parts2), row_walk(b.xr, parts2),
+                      row_walk(b.dr, parts2), cut, shares);
       });
 }
 
@@ -677,8 +688,12 @@ cudaError_t backward_cut_strided(const Back<TX, TY> &b, void *ws, int *parts, cu
   float2 *shares = shares_room(b, ws, parts2);
   return batches(
       b.rows, batch, runs, parts1, parts2, b.dx,
-      [&](const Cut &cut, unsigned grid) { ln_strided_shares<TX, TY, W><<<grid, kThreads, 0, s>>>(b, cut, shares); },
-      [&](const Cut &cut, unsigned grid) { ln_strided_grads<TX, TY, W><<<grid, kThreads, 0, s>>>(b, cut, shares); });
+      [&](bool first, const Cut &cut, unsigned grid) {
+        return launch(first, ln_strided_shares<TX, TY, W>, grid, kThreads, 0, s, b, cut, shares);
+      },
+      [&](bool first, const Cut &cut, unsigned grid) {
+        return launch(first, ln_strided_grads<TX, TY, W>, grid, kThreads, 0, s, b, cut, shares);
+      });
 }
 
 template <class TX, class TY>
@@ -714,8 +729,8 @@ cudaError_t backward(const LayerNormProblem &p, cudaStream_t s) {
   int depth = 1;
   while (depth < 32 && depth * 8 < parts) depth *= 2;
   const int threads = depth < 32 ? 256 : 1024, width = threads / depth;
-  ln_finish<<<grid_for((p.cols + width - 1) / width), threads, 0, s>>>(b.part, parts, p.cols, depth, p.dw, p.db, p.dwtype);
-  return cudaGetLastError();
+  return launch(p.rows == 0, ln_finish, grid_for((p.cols + width - 1) / width), threads, 0, s, b.part, parts, p.cols, depth, p.dw,
+                p.db, p.dwtype);
 }
 
 }  // namespace
