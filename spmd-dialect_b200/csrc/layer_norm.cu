@@ -119,6 +119,138 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   copy_wait<0>();
 }
 
+// Longer rows that a cluster's blocks hold, several at a time.  One exchange gives
+// both statistics: each warp's sum, and its squares around its own mean.
+constexpr int kSpreadStages = 3;
+template <class TX>
+constexpr int kSpreadRows = 8 / (int)sizeof(TX);
+
+template <class TX, class TY, int W, bool WRAPS, bool APART>
+__global__ void __launch_bounds__(kThreads, 2)
+ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
+                  const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int blocks) {
+  constexpr int NV = kMost / W, R = kSpreadRows<TX>, kWarps = kThreads / 32;
+  using In = Source<W, NV, kThreads, APART, TX>;
+  constexpr int kStage = R * In::kBytes;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(16) float4 sh[2][R / 2][kSpread * kWarps];
+  __shared__ float2 count[kSpread * kWarps];  // a warp's columns of a row, and their reciprocal
+  cluster_arrive();
+  const int rank = blockIdx.x % blocks, lanes = blocks * kThreads, lane = rank * kThreads + threadIdx.x, entry = lane >> 5;
+  const float inv_n = 1.0f / (float)cols;
+  const int64_t step = gridDim.x / blocks, i = blockIdx.x / blocks;
+  const int turns = row_count(i, rows, step);
+  const TX *from = x + row_offset(xr.r, i);
+  TY *to = y + row_offset(yr.r, i);
+  const int shift = (int)((APART ? (uintptr_t)to / sizeof(TY) : (uintptr_t)from / sizeof(TX)) % W);
+  const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
+  In in;
+  in.place(from, cols, lane, lanes, shift, have, smem, kSpreadStages * R, In::kBytes);
+  to += lane * W - shift;
+  from += in.start;
+  int stage_in = 0, stage = 0, fetched = 0;
+  auto fetch = [&] {
+    In::emptied();
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (fetched < turns) in.fetch(stage_in + q * In::kBytes, from);
+      ++fetched;
+      from = next_row<WRAPS>(from, x + in.start, xr, i + fetched * step);
+    }
+    copy_commit();  // empty past the last row, so that the count of groups stays
+    stage_in = stage_in == (kSpreadStages - 1) * kStage ? 0 : stage_in + kStage;
+  };
+#pragma unroll
+  for (int q = 0; q < kSpreadStages - 1; ++q) fetch();
+  for (int e = threadIdx.x; e < blocks * kWarps; e += kThreads) {  // as held() has it
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int low = (k * lanes + 32 * e) * W - shift, high = low + 32 * W;
+      n += max(min(high, cols) - max(low, 0), 0);
+    }
+    count[e] = make_float2((float)n, n ? 1.0f / (float)n : 0.0f);
+  }
+  __syncthreads();
+  const float own = count[entry].y;
+  float wv[NV][W], bv[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    load_weight<W, true>(w, wtype, 0, 0, cols, k, lane, lanes, shift, 1.0f, wv[k]);
+    load_weight<W, true>(b, wtype, 0, 0, cols, k, lane, lanes, shift, 0.0f, bv[k]);
+  }
+  cluster_wait();  // the others have begun
+  for (int turn = 0, space = 0; turn < turns; turn += R, space ^= 1) {
+    fetch();
+    copy_wait<kSpreadStages - 1>();
+    F2 t[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      in.arrived(stage + q * In::kBytes);
+      t[q] = {0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        F2 v[W / 2];
+        in.take(stage + q * In::kBytes, k, v);
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) t[q] = add2(t[q], v[e]);
+      }
+    }
+    F2 sum[R / 2], mean[R / 2], var[R / 2];  // of two rows each
+#pragma unroll
+    for (int p = 0; p < R / 2; ++p) sum[p] = row_sum2<kThreads>({t[2 * p].x + t[2 * p].y, t[2 * p + 1].x + t[2 * p + 1].y}, 32, nullptr);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      F2 v[NV][W / 2];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) in.take(stage + q * In::kBytes, k, v[k]);
+      t[q] = deviations<W, NV>(v, (q & 1 ? sum[q / 2].y : sum[q / 2].x) * own, have);
+    }
+#pragma unroll
+    for (int p = 0; p < R / 2; ++p)
+      cluster_share({sum[p], row_sum2<kThreads>({t[2 * p].x + t[2 * p].y, t[2 * p + 1].x + t[2 * p + 1].y}, 32, nullptr)}, blocks, entry,
+                    sh[space][p]);
+    cluster_arrive();
+    cluster_wait();
+#pragma unroll
+    for (int p = 0; p < R / 2; ++p) {
+      const float4 *shared = sh[space][p];
+      mean[p] = var[p] = {0.0f, 0.0f};
+      for (int e = threadIdx.x & 31; e < blocks * kWarps; e += 32) mean[p] = add2(mean[p], {shared[e].x, shared[e].y});
+      mean[p] = mul2(row_sum2<kThreads>(mean[p], 32, nullptr), both(inv_n));
+      for (int e = threadIdx.x & 31; e < blocks * kWarps; e += 32) {
+        const float4 s = shared[e];
+        const float2 n = count[e];
+        const F2 d = fma2({s.x, s.y}, both(n.y), {-mean[p].x, -mean[p].y});
+        var[p] = add2(var[p], fma2(mul2(d, both(n.x)), d, {s.z, s.w}));
+      }
+      var[p] = mul2(row_sum2<kThreads>(var[p], 32, nullptr), both(inv_n));
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const float m = q & 1 ? mean[q / 2].y : mean[q / 2].x, rstd = 1.0f / sqrtf((q & 1 ? var[q / 2].y : var[q / 2].x) + eps);
+      if (turn + q < turns) {
+        F2 v[NV][W / 2];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          in.take(stage + q * In::kBytes, k, v[k]);
+#pragma unroll
+          for (int e = 0; e < W / 2; ++e)
+            v[k][e] = fma2(mul2(add2(v[k][e], both(-m)), both(rstd)), {wv[k][2 * e], wv[k][2 * e + 1]}, {bv[k][2 * e], bv[k][2 * e + 1]});
+        }
+        stream_store<W, NV>(to, have, lanes, v);
+        if (lane == 0) {
+          if (mean_out) mean_out[i + (turn + q) * step] = m;
+          if (rstd_out) rstd_out[i + (turn + q) * step] = rstd;
+        }
+      }
+      to = next_row<WRAPS>(to, y + lane * W - shift, yr, i + (turn + q + 1) * step);
+    }
+    stage = stage == (kSpreadStages - 1) * kStage ? 0 : stage + kStage;
+  }
+  copy_wait<0>();
+}
+
 // Rows of any strides.  Rows past the last take part in the barriers, with no
 // columns.
 template <class TX, class TY, int W, int NV>
@@ -430,6 +562,19 @@ cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t 
 }
 
 template <class TX, class TY, bool WRAPS, bool APART>
+cudaError_t forward_spread(const LayerNormProblem &p, int blocks, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, bytes = kSpreadStages * kSpreadRows<TX> * Source<W, kMost / W, kThreads, APART, TX>::kBytes;
+  auto kernel = ln_forward_spread<TX, TY, W, WRAPS, APART>;
+  if (cudaError_t e = allow_shared(kernel, bytes)) return e;
+  int most = 0;
+  if (cudaError_t e = resident_clusters(kernel, blocks, kThreads, bytes, &most)) return e;
+  const int clusters = stream_grid(p.rows, 1, most, W);
+  return launch_clusters(kernel, clusters, blocks, kThreads, bytes, s, static_cast<const TX *>(p.x), row_walk(p.xr, clusters),
+                         static_cast<TY *>(p.y), row_walk(p.yr, clusters), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean,
+                         p.rstd, blocks);
+}
+
+template <class TX, class TY, bool WRAPS, bool APART>
 cudaError_t forward_cut(const LayerNormProblem &p, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, bytes1 = kCutStages * kRun * (int)sizeof(TX);
   constexpr int bytes2 = kCutStages * Source<W, kCutMost / W, kThreads, APART, TX>::kBytes;
@@ -487,6 +632,12 @@ cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
   if (steady(p.xr, p.rows, W) && steady(p.yr, p.rows, W)) {
     const int spare = vec_rows(p.y, p.yr, p.rows, sizeof(TY), W) ? 0 : W - 1;
     const bool held = p.cols + spare <= kHalfHeld;
+    if (!held && p.cols + spare <= kSpread * kHeld) {
+      const int blocks = spread_blocks(p.cols + spare);
+      if (!same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W)) return forward_spread<TX, TY, true, true>(p, blocks, s);
+      return p.rows > p.xr.n1 || p.rows > p.yr.n1 ? forward_spread<TX, TY, true, false>(p, blocks, s)
+                                                  : forward_spread<TX, TY, false, false>(p, blocks, s);
+    }
     if (!same_shift(p.x, p.xr, sizeof(TX), p.y, p.yr, sizeof(TY), p.rows, W))
       return held ? forward_streamed<TX, TY, true>(p, spare, s) : forward_cut<TX, TY, true, true>(p, s);
     return held ? forward_streamed<TX, TY, false>(p, spare, s)

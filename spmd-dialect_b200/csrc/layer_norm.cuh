@@ -13,6 +13,8 @@
 // are cut into runs.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "dtypes.cuh"
 #include "internal.h"
 
@@ -133,6 +135,36 @@ __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
     for (int q = 0; q < warps; ++q) add(q);
   }
   return t;
+}
+
+// Sums over a cluster's blocks: every warp puts its own into each block's shared
+// memory, where `sh` has an entry for each warp of the cluster.  Two uses in turn of
+// two of them need no other barrier.
+constexpr int kSpread = 8;  // blocks of a cluster at most
+__device__ __forceinline__ float *in_block(float *p, int rank) {
+  return cooperative_groups::this_cluster().map_shared_rank(p, rank);
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// Four values of a warp into its entry of every block's `sh`.
+__device__ __forceinline__ void cluster_share(F4 s, int blocks, int entry, float4 *sh) {
+  const int lane = threadIdx.x & 31, which = lane >> 3;
+  if ((lane & 7) < blocks)
+    *in_block(reinterpret_cast<float *>(sh + entry) + which, lane & 7) = which < 2 ? (which ? s.a.y : s.a.x) : which == 2 ? s.b.x : s.b.y;
+}
+template <int MAXT>
+__device__ __forceinline__ F4 cluster_sum4(F4 v, int blocks, int entry, float4 *sh) {
+  cluster_share(row_sum4<MAXT>(v, 32, nullptr), blocks, entry, sh);
+  cluster_arrive();
+  cluster_wait();
+  F4 t{{0.0f, 0.0f}, {0.0f, 0.0f}};
+  for (int q = threadIdx.x & 31; q < blocks * (MAXT / 32); q += 32) {
+    const float4 f = sh[q];
+    t.a = add2(t.a, {f.x, f.y});
+    t.b = add2(t.b, {f.z, f.w});
+  }
+  return row_sum4<MAXT>(t, 32, nullptr);
 }
 
 // Column of element e of vector k of a thread (relative to a run's first, where a
@@ -538,6 +570,38 @@ cudaError_t launch(bool first, void (*kernel)(P...), unsigned grid, unsigned thr
   if (!first) return launch_pdl(kernel, grid, threads, bytes, s, args...);
   kernel<<<grid, threads, bytes, s>>>(args...);
   return cudaGetLastError();
+}
+// Blocks of kThreads that hold a row at 16 elements a thread.
+inline int spread_blocks(int64_t cols) { return (int)((cols + kThreads * 16 - 1) / (kThreads * 16)); }
+// Clusters of `blocks` blocks that run at once.
+template <class Kernel>
+cudaError_t resident_clusters(Kernel kernel, int blocks, int threads, int bytes, int *clusters) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = blocks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg);
+}
+template <class... P, class... A>
+cudaError_t launch_clusters(void (*kernel)(P...), int clusters, int blocks, int threads, int bytes, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = blocks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(clusters * blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 inline unsigned grid_for(int64_t items) { return (unsigned)(items < INT32_MAX ? items : INT32_MAX); }
 

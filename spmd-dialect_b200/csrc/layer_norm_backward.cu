@@ -120,7 +120,7 @@ constexpr int kStages = 3;
 template <class TX, class TY>
 constexpr int kRowsAtOnce = sizeof(TX) + sizeof(TY) <= 6 ? 2 : 1;  // as two blocks' stages fit an SM
 
-template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES, bool WRAPS, bool APART>
+template <class TX, class TY, int W, int NV, int MAXT, int R, int STAGES, bool WRAPS, bool APART, bool SPREAD>
 __global__ void __launch_bounds__(MAXT, MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3)
 ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
                    const __grid_constant__ RowWalk dr, int lanes) {
@@ -128,15 +128,18 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   using InG = Source<W, NV, MAXT, APART, TY>;
   constexpr int kRow = InX::kBytes + InG::kBytes, kStage = R * kRow;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(16) float4 sh[2][32];
-  constexpr int kSlots = MAXT > kThreads ? MAXT / 32 : APART ? MAXT / 8 : MAXT;
+  __shared__ __align__(16) float4 sh[2][SPREAD ? kSpread * MAXT / 32 : 32];
+  constexpr int kSlots = SPREAD || MAXT > kThreads ? MAXT / 32 : APART ? MAXT / 8 : MAXT;
   __shared__ float2 stats[STAGES * R][kSlots];  // a group's row, or a warp's where the group is wider
-  const int lane = threadIdx.x & (lanes - 1), groups = MAXT / lanes, group = threadIdx.x / lanes;
+  const int blocks = SPREAD ? lanes / MAXT : 1, rank = SPREAD ? blockIdx.x % blocks : 0, team = blockIdx.x / blocks;
+  const int lane = SPREAD ? rank * MAXT + threadIdx.x : threadIdx.x & (lanes - 1);
+  const int groups = SPREAD ? 1 : MAXT / lanes, group = SPREAD ? 0 : threadIdx.x / lanes;
   const int cols = (int)p.cols, slot = lanes <= 32 ? group : threadIdx.x >> 5;
   pdl_trigger();
+  if constexpr (SPREAD) cluster_arrive();
   const bool first = (threadIdx.x & (lanes <= 32 ? lanes - 1 : 31)) == 0;  // copies the statistics for its group or warp
   const float inv_n = 1.0f / (float)cols;
-  const int64_t step = (int64_t)gridDim.x * groups, i = (int64_t)blockIdx.x * groups + group;
+  const int64_t step = (int64_t)(gridDim.x / blocks) * groups, i = (int64_t)team * groups + group;
   const int mine = row_count(i, p.rows, step), turns = row_count(i - group, p.rows, step);
   const TX *x_from = p.x + (mine ? row_offset(xr.r, i) : 0);
   const TY *g_from = p.dy + (mine ? row_offset(gr.r, i) : 0);
@@ -183,6 +186,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < W / 2; ++e) sw[k][e] = sb[k][e] = {0.0f, 0.0f};
+  if constexpr (SPREAD) cluster_wait();  // the others have begun
   for (int turn = 0; turn < turns; turn += R) {
     fetch();
     copy_wait<STAGES - 1>();
@@ -213,7 +217,10 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
       c[q] = {s1.x + s1.y, s2.x + s2.y};
     }
     __syncwarp();  // every lane has its statistics: the slot may be filled again
-    if constexpr (R == 2) {
+    if constexpr (SPREAD) {
+      const F4 t = cluster_sum4<MAXT>({c[0], c[R - 1]}, blocks, lane >> 5, sh[(turn / R) & 1]);
+      c[0] = t.a, c[R - 1] = R == 2 ? t.b : t.a;
+    } else if constexpr (R == 2) {
       const F4 t = row_sum4<MAXT>({c[0], c[1]}, lanes, sh[(turn / R) & 1]);
       c[0] = t.a, c[1] = t.b;
     } else {
@@ -245,7 +252,20 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   copy_wait<0>();
-  if (p.part) {
+  if constexpr (SPREAD) {  // a column is one thread's
+    if (!p.part) return;
+    float *const part_w = p.part + 2 * (int64_t)team * cols, *const part_b = part_w + cols;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int c = shifted<W>(k, e, lane, lanes, shift);
+        if (c >= 0 && c < cols) {
+          part_w[c] = e & 1 ? sw[k][e / 2].y : sw[k][e / 2].x;
+          part_b[c] = e & 1 ? sb[k][e / 2].y : sb[k][e / 2].x;
+        }
+      }
+  } else if (p.part) {
     float tw[NV][W], tb[NV][W];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -610,7 +630,7 @@ cudaError_t stream_rows_as(const Back<TX, TY> &b, int lanes, int *parts, cudaStr
   constexpr int W = kWidth<TX, TY>, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;
   constexpr int staged = stages * R * (Source<W, NV, MAXT, APART, TX>::kBytes + Source<W, NV, MAXT, APART, TY>::kBytes);
   const int sums = b.part ? (int)(MAXT / lanes * b.cols * sizeof(float)) : 0, bytes = staged > sums ? staged : sums;
-  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages, WRAPS, APART>;
+  auto kernel = ln_backward_stream<TX, TY, W, NV, MAXT, R, stages, WRAPS, APART, false>;
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   const int64_t groups = MAXT / lanes;
   const int most = (MAXT > kThreads ? 1 : NV * W > 8 ? 2 : 3) * device_sms();
@@ -635,6 +655,20 @@ cudaError_t backward_streamed(const Back<TX, TY> &b, int spare, int *parts, cuda
   if (nv == 1) return stream_rows<TX, TY, 1, kThreads, APART>(b, lanes, parts, s);
   if (nv < NV) return stream_rows<TX, TY, 2, kThreads, APART>(b, lanes, parts, s);
   return stream_rows<TX, TY, NV, kThreads, APART>(b, lanes, parts, s);
+}
+
+// Rows of a cluster's blocks.
+template <class TX, class TY, bool WRAPS, bool APART>
+cudaError_t backward_spread(const Back<TX, TY> &b, int blocks, int *parts, cudaStream_t s) {
+  constexpr int W = kWidth<TX, TY>, NV = kMost / W, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;
+  constexpr int bytes = stages * R * (Source<W, NV, kThreads, APART, TX>::kBytes + Source<W, NV, kThreads, APART, TY>::kBytes);
+  auto kernel = ln_backward_stream<TX, TY, W, NV, kThreads, R, stages, WRAPS, APART, true>;
+  if (cudaError_t e = allow_shared(kernel, bytes)) return e;
+  int most = 0;
+  if (cudaError_t e = resident_clusters(kernel, blocks, kThreads, bytes, &most)) return e;
+  *parts = stream_grid(b.rows, 1, most < kGradBlocks / blocks ? most : kGradBlocks / blocks, W);
+  return launch_clusters(kernel, *parts, blocks, kThreads, bytes, s, b, row_walk(b.gr, *parts), row_walk(b.xr, *parts),
+                         row_walk(b.dr, *parts), blocks * kThreads);
 }
 
 // Two passes over each batch of longer rows: shares(first, cut, grid), where dx is
@@ -705,6 +739,11 @@ cudaError_t backward_of(const Back<TX, TY> &b, void *ws, int *parts, cudaStream_
     const bool whole = b.dx ? vec_rows(b.dx, b.dr, b.rows, sizeof(TX), W) : vec_rows(b.x, b.xr, b.rows, sizeof(TX), W);
     const int spare = whole ? 0 : W - 1;
     if (b.cols + spare <= kHeld) return same ? backward_streamed<TX, TY, false>(b, spare, parts, s) : backward_streamed<TX, TY, true>(b, spare, parts, s);
+    if (b.cols + spare <= kSpread * kThreads * kMost) {
+      const int blocks = spread_blocks(b.cols + spare);
+      if (!same) return backward_spread<TX, TY, true, true>(b, blocks, parts, s);
+      return wraps(b) ? backward_spread<TX, TY, true, false>(b, blocks, parts, s) : backward_spread<TX, TY, false, false>(b, blocks, parts, s);
+    }
     if (!same) return backward_cut<TX, TY, true, true>(b, ws, parts, s);
     return wraps(b) ? backward_cut<TX, TY, true, false>(b, ws, parts, s) : backward_cut<TX, TY, false, false>(b, ws, parts, s);
   }
@@ -743,7 +782,9 @@ size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   const int64_t runs = most_runs(cols), batch = batch_rows(rows, cols, 4);
   const size_t cut = round16((size_t)cut_parts(batch, runs, kGradBlocks, 8) * 2 * (size_t)cols * sizeof(float)) +
                      (size_t)batch * (size_t)runs * kCutWarps * sizeof(float2);
-  return whole > cut ? whole : cut;
+  const int64_t teams = cols <= kSpread * kThreads * kMost ? kGradBlocks / spread_blocks(cols) : 0;
+  const size_t spread = (size_t)(rows < teams ? rows : teams) * 2 * (size_t)cols * sizeof(float), most = whole > cut ? whole : cut;
+  return most > spread ? most : spread;
 }
 
 cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s) {
