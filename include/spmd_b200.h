@@ -501,7 +501,7 @@ int spmdb200_jacobi3d(float *U_base, float *U_aligned, int64_t U_offset,
  * are equal, or one of them is SPMDB200_F32.  Sums are f32; y is rounded once.
  * y may be x (same view); other overlaps are undefined.  ws: device memory of at
  * least spmdb200_layer_norm_forward_workspace_bytes(rows, N) bytes, 16-byte
- * aligned, contents irrelevant; 0 bytes (NULL) for rows of up to 8185 elements.
+ * aligned, contents irrelevant; 0 bytes (NULL) for rows of up to 49145 elements.
  * Calls that share ws must not overlap on the GPU. */
 size_t spmdb200_layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols);
 int spmdb200_layer_norm(int rank, const int64_t *sizes, const void *x, int x_type, const int64_t *x_strides,
@@ -529,7 +529,9 @@ int spmdb200_layer_norm_backward(int rank, const int64_t *sizes, const void *dy,
  * scale is not NULL, *scale = min(1, max_norm / *norm), NaN when the norm is
  * not finite (device f32 scalars).  grads[k] holds sizes[k] elements of
  * types[k], unit stride (host arrays of `count` entries; a size may be 0).
- * Squares and sums are f64, one rounding, identical bits on every call.  ws:
+ * Eight squares at a time are added up in f32 (their sum is off by 2^-22 of
+ * itself at most, in f64 where it would leave f32's range), these in f64, in a
+ * fixed order: identical bits on every call.  ws:
  * spmdb200_grad_norm_workspace_bytes(count) bytes of device memory, 16-byte
  * aligned, contents irrelevant; calls that share ws must not overlap on the
  * GPU. */

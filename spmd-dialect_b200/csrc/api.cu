@@ -19,6 +19,8 @@
 #include "../../include/spmd_b200.h"
 #include "internal.h"
 
+static_assert(SPMDB200_STATE_BLOCK == spmdb200::kStateBlock, "elements of one scale of an 8-bit state");
+
 using namespace spmdb200;
 
 namespace {

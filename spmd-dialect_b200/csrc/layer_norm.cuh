@@ -1,16 +1,18 @@
 // layer_norm.cuh -- what the two directions of the layer norm share.
 //
-// A row is taken by `lanes` threads (a power of two), each with NV vectors of W
-// elements; W is what 16 bytes of the wider type hold.  Two layouts:
+// A row is taken by `lanes` threads (a power of two in a block, or the threads of
+// up to twelve blocks, a cluster), each with NV vectors of W elements; W is what 16
+// bytes of the wider type hold.  Two layouts:
 // - Vectors: thread t has the aligned vectors t, t + lanes, ... that cover the
 //   row, whose last dimension is contiguous.  The row may start `shift` elements
-//   into its first vector (odd lengths, odd addresses).
+//   into its first vector (odd lengths, odd addresses), an input's elsewhere than
+//   the output's (Source).
 // - Any strides and addresses: single elements t, t + lanes, ...
 // A block that goes through rows with vectors does so with a stride of rows that
 // is a multiple of W, so that a thread's rows all have one shift, and its
 // columns, with their weights and sums in registers, are the same in all of them.
-// Columns are 32-bit numbers: a block holds at most a few thousand, longer rows
-// are cut into runs.
+// Columns are 32-bit numbers: a cluster holds at most some fifty thousand, longer
+// rows are cut into runs.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -140,7 +142,13 @@ __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
 // Sums over a cluster's blocks: every warp puts its own into each block's shared
 // memory, where `sh` has an entry for each warp of the cluster.  Two uses in turn of
 // two of them need no other barrier.
-constexpr int kSpread = 8;  // blocks of a cluster at most
+//
+// Twelve blocks at most: the more, the longer a row waits for all of them, and the
+// fewer clusters fit the groups of SMs that hold them.  Against the two passes
+// below, us: 4096 x 40001 f32 343 to 462 forward, 554 to 784 backward, bf16 249 to 316
+// and 306 to 519; 4096 x 49152 f32 382 to 472 and 604 to 711, bf16 302 to 311 and 399 to
+// 491; with sixteen blocks 2048 x 65536 bf16 took 335 forward against some 200.
+constexpr int kSpread = 12;
 __device__ __forceinline__ float *in_block(float *p, int rank) {
   return cooperative_groups::this_cluster().map_shared_rank(p, rank);
 }
@@ -150,8 +158,10 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Four values of a warp into its entry of every block's `sh`.
 __device__ __forceinline__ void cluster_share(F4 s, int blocks, int entry, float4 *sh) {
   const int lane = threadIdx.x & 31, which = lane >> 3;
-  if ((lane & 7) < blocks)
-    *in_block(reinterpret_cast<float *>(sh + entry) + which, lane & 7) = which < 2 ? (which ? s.a.y : s.a.x) : which == 2 ? s.b.x : s.b.y;
+  const float mine = which < 2 ? (which ? s.a.y : s.a.x) : which == 2 ? s.b.x : s.b.y;
+#pragma unroll
+  for (int o = 0; o < kSpread; o += 8)
+    if (const int r = o + (lane & 7); r < blocks) *in_block(reinterpret_cast<float *>(sh + entry) + which, r) = mine;
 }
 template <int MAXT>
 __device__ __forceinline__ F4 cluster_sum4(F4 v, int blocks, int entry, float4 *sh) {
@@ -486,7 +496,7 @@ __device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, const H
   return t;
 }
 
-// ---- rows longer than a block holds -----------------------------------------------------
+// ---- rows longer than a cluster holds ---------------------------------------------------
 // They are cut into runs of kRun columns (of the row's vectors).  Two passes over
 // as many rows as L2 holds: each warp's share of a row's sums into the workspace,
 // with no barrier, then the rest of the work.  Block (run, part) takes every
@@ -576,6 +586,8 @@ inline int spread_blocks(int64_t cols) { return (int)((cols + kThreads * 16 - 1)
 // Clusters of `blocks` blocks that run at once.
 template <class Kernel>
 cudaError_t resident_clusters(Kernel kernel, int blocks, int threads, int bytes, int *clusters) {
+  if (blocks > 8)
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
 // while R are computed, their mean and rstd with them.  The row's sums come first,
 // then, with x and dy read from shared memory once more, dx and the column sums:
 // holding them in registers over the reduction would leave no room for a second
-// row, whose instructions fill the reduction's waits.
+// row, whose instructions fill the reduction's waits.  SPREAD: a row is held by the
+// `lanes` threads of a cluster's blocks.
 constexpr int kStages = 3;
 template <class TX, class TY>
 constexpr int kRowsAtOnce = sizeof(TX) + sizeof(TY) <= 6 ? 2 : 1;  // as two blocks' stages fit an SM
@@ -657,7 +658,7 @@ cudaError_t backward_streamed(const Back<TX, TY> &b, int spare, int *parts, cuda
   return stream_rows<TX, TY, NV, kThreads, APART>(b, lanes, parts, s);
 }
 
-// Rows of a cluster's blocks.
+// Rows of a cluster's blocks: a column's sums stay one thread's.
 template <class TX, class TY, bool WRAPS, bool APART>
 cudaError_t backward_spread(const Back<TX, TY> &b, int blocks, int *parts, cudaStream_t s) {
   constexpr int W = kWidth<TX, TY>, NV = kMost / W, R = kRowsAtOnce<TX, TY>, stages = R == 2 ? 2 : kStages;

@@ -288,7 +288,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     rstd * weight + bias.  x is any strided view; out has `dtype` (default
     x's; one of the two may be float32) and may be x itself.  mean and rstd
     (float32, x's leading shape) are what layer_norm_backward takes; stats=False
-    leaves them out (None).  Rows of more than 8185 elements use a workspace of
+    leaves them out (None).  Rows of more than 49145 elements use a workspace of
     layer_norm_workspace(rows, cols, backward=False)."""
     dev = x.get_device()
     if _elsewhere(dev, stream):
@@ -316,7 +316,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         m, r = mean.data_ptr(), rstd.data_ptr()
     xv, ov = _norm_rows("x", x), _norm_rows("out", out)
     rank, room, room_bytes = xv.dim(), None, 0
-    if ws is not None or shape[-1] > 8185:
+    if ws is not None or shape[-1] > 49145:
         ws = _norm_room(ws, math.prod(shape[:-1]), shape[-1], x, False)
         room, room_bytes = ws.data_ptr(), ws.nbytes
     dims = array("q", (*xv.shape, *xv.stride(), *ov.stride()))

@@ -105,6 +105,16 @@ def test_long_rows_in_batches(kernels, rows, cols):
 
 
 @pytest.mark.parametrize("x_t,y_t", PAIRS)
+@pytest.mark.parametrize("rows,cols", [(700, 8193), (501, 12289), (150, 28672), (301, 40968), (77, 49145), (75, 49152), (75, 49153)])
+def test_rows_spread_over_blocks(kernels, rows, cols, x_t, y_t):
+    """Rows held by two to twelve blocks, more of them than are resident at once."""
+    x, dy = make((rows, cols), x_t, 1), make((rows, cols), y_t, 2)
+    w, b = weights(cols, F32, 3)
+    _, mean, rstd = check_forward(kernels, x, w, b, ydtype=y_t)
+    check_backward(kernels, dy, x, w, stats=(mean, rstd))
+
+
+@pytest.mark.parametrize("x_t,y_t", PAIRS)
 @pytest.mark.parametrize("w_t", [None, F32, F16, BF16])
 def test_types(kernels, x_t, y_t, w_t):
     for rows, cols in ((33, 320), (9, 1026)):
@@ -162,7 +172,7 @@ def within_nan(t, pitch, at):
 
 
 @pytest.mark.parametrize("x_t,y_t", [(F32, F32), (BF16, BF16), (F16, F32), (F32, BF16)])
-@pytest.mark.parametrize("cols", [1, 3, 8, 15, 33, 100, 257, 1001, 2047, 4090, 4096, 5003, 8185, 8192, 9001, 20001, 70000])
+@pytest.mark.parametrize("cols", [1, 3, 8, 15, 33, 100, 257, 1001, 2047, 4090, 4096, 5003, 8185, 8192, 9001, 20001, 49150, 70000])
 def test_rows_that_start_apart(kernels, x_t, y_t, cols):
     """Inputs and outputs whose rows start at different places within a vector, all with NaN around them."""
     for seed, (rows, px, ax, py, ay, pd, ad) in enumerate((

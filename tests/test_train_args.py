@@ -46,7 +46,7 @@ def test_layer_norm_refuses(bad):
 def test_layer_norm_refuses_type_pairs_and_many_rows():
     assert norm_args(xt=1, yt=2) == -4
     assert norm_args(rank=3, sizes=[1 << 30, 1 << 30, 4], xs=[4, 4, 1], ys=[1 << 32, 4, 1]) == -1
-    long = {"sizes": [4, 20000], "xs": [20000, 1], "ys": [20000, 1]}  # rows that need a workspace
+    long = {"sizes": [4, 60000], "xs": [60000, 1], "ys": [60000, 1]}  # rows that need a workspace
     assert norm_args(**long) == -5 and norm_args(**long, ws=7 * P + 8, bytes=1 << 30) == -5
     assert norm_args(**long, ws=7 * P, bytes=64) == -5
 
@@ -90,7 +90,9 @@ def test_workspace_sizes():
             # Column sums of at most 444 rows of 8192 or so, or eight partial rows; shares of 72 MB of rows, or of eight.
             assert 8 * cols <= f(rows, cols) <= (32 << 20) + 80 * cols, (rows, cols)
             assert lib().spmdb200_layer_norm_forward_workspace_bytes(rows, cols) <= (8 << 20) + 2 * cols, (rows, cols)
-    assert lib().spmdb200_layer_norm_forward_workspace_bytes(1000, 8185) == 0
+    for cols in (8185, 20000, 49145):
+        assert lib().spmdb200_layer_norm_forward_workspace_bytes(1000, cols) == 0
+    assert lib().spmdb200_layer_norm_forward_workspace_bytes(1000, 49146) > 0
     g = lib().spmdb200_grad_norm_workspace_bytes
     assert 0 < g(0) <= g(1) <= g(5000) <= 1 << 20
 
