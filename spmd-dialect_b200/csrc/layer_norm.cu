@@ -118,9 +118,11 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 }
 
 // Longer rows that a cluster's blocks hold, several at a time.  One exchange gives
-// both statistics: each warp's sum, and its squares around its own mean (two
-// exchanges, as above: 8192 x 16384 f32 239 us, so 208).  An exchange costs the more
-// the fewer bytes are under way: 16-bit rows go four at a time (148 us, two: 174).
+// both statistics: each warp's sum, and its squares around its own mean (8192 x
+// 16384 f32: 208 us, with two exchanges as above 239).  An exchange costs the more
+// the fewer bytes are under way: 16-bit rows go four at a time (148 us, two 174).
+// As many clusters as are resident, whatever rows they take where all start
+// alike: 201 and 136 us, 5.3 and 3.9 TB/s; what is left is the exchange's wait.
 constexpr int kSpreadStages = 3;
 template <class TX>
 constexpr int kSpreadRows = 8 / (int)sizeof(TX);
@@ -568,7 +570,7 @@ cudaError_t forward_spread(const LayerNormProblem &p, int blocks, cudaStream_t s
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   int most = 0;
   if (cudaError_t e = resident_clusters(kernel, blocks, kThreads, bytes, &most)) return e;
-  const int clusters = stream_grid(p.rows, 1, most, W);
+  const int clusters = stream_grid(p.rows, 1, most, APART ? W : row_period(p.xr, p.rows, W));
   return launch_clusters(kernel, clusters, blocks, kThreads, bytes, s, static_cast<const TX *>(p.x), row_walk(p.xr, clusters),
                          static_cast<TY *>(p.y), row_walk(p.yr, clusters), p.w, p.b, p.wtype, p.rows, (int)p.cols, p.eps, p.mean,
                          p.rstd, blocks);

@@ -667,7 +667,7 @@ cudaError_t backward_spread(const Back<TX, TY> &b, int blocks, int *parts, cudaS
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   int most = 0;
   if (cudaError_t e = resident_clusters(kernel, blocks, kThreads, bytes, &most)) return e;
-  *parts = stream_grid(b.rows, 1, most < kGradBlocks / blocks ? most : kGradBlocks / blocks, W);
+  *parts = stream_grid(b.rows, 1, most < kGradBlocks / blocks ? most : kGradBlocks / blocks, APART ? W : row_period(b.xr, b.rows, W));
   return launch_clusters(kernel, *parts, blocks, kThreads, bytes, s, b, row_walk(b.gr, *parts), row_walk(b.xr, *parts),
                          row_walk(b.dr, *parts), blocks * kThreads);
 }

@@ -7,10 +7,15 @@ JSON line with the CUDA-event time per rep and the bandwidth it implies.
     python spmd-dialect_b200/run.py jacobi2d --shape 16384x16384 --sweeps 2 --reps 1
     python spmd-dialect_b200/run.py sum_f32 --size 16777216
     python spmd-dialect_b200/run.py jacobi3d --shape 512x512x512 --sweeps 4
+    python spmd-dialect_b200/run.py layer_norm_backward --shape 32768x4096 --dtype bfloat16
+    python spmd-dialect_b200/run.py adamw --size 268435456 --tensors 300 --dtype bfloat16 --bits 8
 
 Kernels: ewise, axpy, sum_f32, sum_i32, hierarchical_sum, stencil3, jacobi2d,
 jacobi3d, reduce_f32 / reduce_i32 (--kind add|mul|max|min|and|or|xor), forall_map
-(--body axpy: y = 2.5*x + y in place; --body 3in: r = sqrt(|a*b - c|)).  No checking
+(--body axpy: y = 2.5*x + y in place; --body 3in: r = sqrt(|a*b - c|)), and the
+operators of a training step: layer_norm and layer_norm_backward on rows of
+--shape, grad_norm and adamw on --tensors equal tensors that --size elements are
+split into (--dtype; --bits for adamw's states).  No checking
 happens here (the parity tests compare against the
 oracle); this is for timing and for profiler captures.
 """
@@ -29,7 +34,8 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["ewise", "axpy", "sum_f32", "sum_i32", "hierarchical_sum", "stencil3",
-                                       "stencil_nd", "jacobi2d", "jacobi3d", "reduce_f32", "reduce_i32", "forall_map"])
+                                       "stencil_nd", "jacobi2d", "jacobi3d", "reduce_f32", "reduce_i32", "forall_map",
+                                       "layer_norm", "layer_norm_backward", "grad_norm", "adamw"])
     ap.add_argument("--kind", default="max", help="reduction kind for reduce_f32 / reduce_i32")
     ap.add_argument("--body", default="3in", choices=["axpy", "3in"], help="forall_map body")
     ap.add_argument("--layout", default="vec", choices=["vec", "contig", "strided"],
@@ -37,6 +43,10 @@ def main() -> None:
                          "4097-element pitch")
     ap.add_argument("--size", type=int, default=1 << 24)
     ap.add_argument("--shape", default="4096x4096")
+    ap.add_argument("--dtype", default="float32", choices=["float32", "float16", "bfloat16"],
+                    help="of rows, parameters and gradients (norm weights are float32)")
+    ap.add_argument("--tensors", type=int, default=1)
+    ap.add_argument("--bits", type=int, default=32, choices=[8, 32])
     ap.add_argument("--sweeps", type=int, default=100)
     ap.add_argument("--res-every", type=int, default=10)
     ap.add_argument("--reps", type=int, default=5)
@@ -84,6 +94,32 @@ def main() -> None:
             out = view(torch.empty(alloc, device=dev))
             fn = lambda: k.forall_map(xs, out, code, n_regs=n_regs)  # noqa: E731
             work_bytes = 16 * a.size
+    elif a.kernel in ("layer_norm", "layer_norm_backward"):
+        kind = getattr(torch, a.dtype)
+        x = torch.randn(shape, device=dev, generator=g).to(kind)
+        w, b = torch.rand(shape[-1], device=dev, generator=g), torch.rand(shape[-1], device=dev, generator=g)
+        y, mean, rstd = k.layer_norm(x, w, b)
+        a.size = x.numel()
+        if a.kernel == "layer_norm":
+            ws = k.layer_norm_workspace(x.numel() // shape[-1], shape[-1], dev, backward=False)
+            fn = lambda: k.layer_norm(x, w, b, out=y, ws=ws)  # noqa: E731
+            work_bytes = 2 * x.nbytes
+        else:
+            ws = k.layer_norm_workspace(x.numel() // shape[-1], shape[-1], dev)
+            dx = torch.empty_like(x)
+            fn = lambda: k.layer_norm_backward(y, x, mean, rstd, w, dx=dx, ws=ws)  # noqa: E731
+            work_bytes = 3 * x.nbytes
+    elif a.kernel in ("grad_norm", "adamw"):
+        each = [a.size // a.tensors + (i < a.size % a.tensors) for i in range(a.tensors)]
+        grads = [torch.randn(n, device=dev, generator=g).to(getattr(torch, a.dtype)) for n in each]
+        work_bytes = sum(t.nbytes for t in grads)
+        if a.kernel == "grad_norm":
+            fn = lambda: k.grad_norm(grads, 1.0)  # noqa: E731
+        else:
+            params = [torch.randn(n, device=dev, generator=g).to(getattr(torch, a.dtype)) for n in each]
+            state = k.adamw_state(params, a.bits)
+            work_bytes = 3 * work_bytes + sum(2 * t.nbytes for v in state.values() for t in v)
+            fn = lambda: k.adamw(params, grads, **state, step=1, lr=1e-3)  # noqa: E731
     elif a.kernel in ("sum_f32", "hierarchical_sum"):
         x = torch.rand(a.size, device=dev, generator=g)
         o = torch.zeros(1, device=dev)
