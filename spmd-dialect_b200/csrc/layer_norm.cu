@@ -315,7 +315,7 @@ __device__ __forceinline__ Moments join_warp(Moments a) {
   return {__shfl_sync(0xffffffffu, a.n, 0), __shfl_sync(0xffffffffu, a.mean, 0), __shfl_sync(0xffffffffu, a.m2, 0)};
 }
 
-// Longer rows, first pass: moments of each warp's share of a run.
+// Longer rows, first pass: moments of each run of a row.
 constexpr int kCutStages = 4;
 
 template <class TX, int W, bool WRAPS>
@@ -325,6 +325,7 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   using In = Source<W, NV, kThreads, false, TX>;
   constexpr int kStage = In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ Moments warps[kCutRows][kCutWarps];
   const CutPlace at = cut_place(cut);
   pdl_trigger();
   if (at.rows == 0) return pdl_wait();
@@ -355,7 +356,6 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
   };
 #pragma unroll
   for (int q = 0; q < kCutStages - 1; ++q) fetch();
-  pdl_wait();  // the shares of the batch before have been read
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
     copy_wait<kCutStages - 1>();
@@ -373,10 +373,17 @@ ln_moments(const TX *x, const __grid_constant__ RowWalk xr, int64_t cols, const 
     t = deviations<W, NV>(v, mean, have);
     const float warp_mean = warp_sum_f32(sum) * inv_all, d = mean - warp_mean;
     const float m2 = warp_sum_f32(fmaf(count * d, d, t.x + t.y));
-    if ((lane & 31) == 0)
-      shares[((at.i - cut.first + (int64_t)turn * cut.parts) * cut.runs + at.run) * kCutWarps + (lane >> 5)] = make_float4(all, warp_mean, m2, 0.0f);
+    if ((lane & 31) == 0) warps[turn][lane >> 5] = {all, warp_mean, m2};
   }
   copy_wait<0>();
+  __syncthreads();
+  pdl_wait();  // the shares of the batch before have been read
+  if (lane < at.rows) {
+    Moments m = warps[lane][0];
+#pragma unroll
+    for (int k = 1; k < kCutWarps; ++k) m = join(m, warps[lane][k]);
+    shares[(at.i - cut.first + (int64_t)lane * cut.parts) * cut.runs + at.run] = make_float4(m.n, m.mean, m.m2, 0.0f);
+  }
 }
 
 // Second pass: the rows' statistics from the shares, and the output.
@@ -425,8 +432,8 @@ ln_outputs(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_
   for (int r = lane >> 5; r < at.rows; r += kCutWarps) {  // a warp a row, in one order
     const int64_t i = at.i + (int64_t)r * cut.parts;
     Moments m{0.0f, 0.0f, 0.0f};
-    for (int64_t q = lane & 31; q < cut.runs * kCutWarps; q += 32) {
-      const float4 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
+    for (int64_t q = lane & 31; q < cut.runs; q += 32) {
+      const float4 s = shares[(i - cut.first) * cut.runs + q];
       m = join(m, {s.x, s.y, s.z});
     }
     m = join_warp(m);
@@ -657,7 +664,7 @@ cudaError_t forward(const LayerNormProblem &p, cudaStream_t s) {
 
 size_t layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols) {
   if (cols <= kSpread * kHeld - 7) return 0;
-  return (size_t)batch_rows(rows, cols, 2) * (size_t)most_runs(cols) * kCutWarps * sizeof(float4);
+  return (size_t)batch_rows(rows, cols, 2) * (size_t)most_runs(cols) * sizeof(float4);
 }
 
 cudaError_t launch_layer_norm(const LayerNormProblem &p, cudaStream_t s) {

@@ -498,13 +498,13 @@ __device__ __forceinline__ F2 deviations(F2 (&v)[NV][W / 2], float mean, const H
 
 // ---- rows longer than a cluster holds ---------------------------------------------------
 // They are cut into runs of kRun columns (of the row's vectors).  Two passes over
-// as many rows as L2 holds: each warp's share of a row's sums into the workspace,
-// with no barrier, then the rest of the work.  Block (run, part) takes every
+// as many rows as L2 holds: each run's share of its rows' sums into the workspace,
+// with no barrier between rows, then the rest of the work.  Block (run, part) takes every
 // parts-th of the rows `first` to `last`, streamed, its columns' weights in
 // registers.
 constexpr int kCutMost = 16;                // elements of a run in a thread
 constexpr int kRun = kThreads * kCutMost;
-constexpr int kCutWarps = kThreads / 32;    // shares of a run
+constexpr int kCutWarps = kThreads / 32;
 constexpr int kCutRows = 64;                // rows of a block at most
 
 struct Cut {

@@ -280,7 +280,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
   }
 }
 
-// Longer rows (layer_norm.cuh), first pass: each warp's share of a row's two sums.
+// Longer rows (layer_norm.cuh), first pass: each run's share of a row's two sums.
 template <class TX, class TY, int W, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
@@ -290,7 +290,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   using InG = Source<W, NV, kThreads, APART, TY>;
   constexpr int kStage = InX::kBytes + InG::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float2 stats[kCutRows];
+  __shared__ float2 stats[kCutRows], warps[kCutRows][kCutWarps];
   const CutPlace at = cut_place(cut);
   pdl_trigger();
   if (at.rows == 0) return pdl_wait();
@@ -327,7 +327,6 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
   float w[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k) load_weight<W, true>(p.w, p.wtype, first + low, 0, n, k, lane, kThreads, shift, 1.0f, w[k]);
-  pdl_wait();  // the shares of the batch before have been read
   __syncthreads();
   for (int turn = 0; turn < at.rows; ++turn) {
     fetch();
@@ -350,10 +349,17 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
     const F2 s = row_sum2<kThreads>({s1.x + s1.y, s2.x + s2.y}, 32, nullptr);
-    if ((lane & 31) == 0)
-      shares[((at.i - cut.first + (int64_t)turn * cut.parts) * cut.runs + at.run) * kCutWarps + (lane >> 5)] = make_float2(s.x, s.y);
+    if ((lane & 31) == 0) warps[turn][lane >> 5] = make_float2(s.x, s.y);
   }
   copy_wait<0>();
+  __syncthreads();
+  pdl_wait();  // the shares of the batch before have been read
+  if (lane < at.rows) {
+    float2 s = warps[lane][0];
+#pragma unroll
+    for (int k = 1; k < kCutWarps; ++k) s = make_float2(s.x + warps[lane][k].x, s.y + warps[lane][k].y);
+    shares[(at.i - cut.first + (int64_t)lane * cut.parts) * cut.runs + at.run] = s;
+  }
 }
 
 // Second pass: dx and the column sums, which go on from what the batches before
@@ -427,8 +433,8 @@ ln_grads(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk
     const int64_t i = at.i + (int64_t)r * cut.parts;
     float c1 = 0.0f, c2 = 0.0f;
     if (p.dx)
-      for (int64_t q = lane & 31; q < cut.runs * kCutWarps; q += 32) {
-        const float2 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
+      for (int64_t q = lane & 31; q < cut.runs; q += 32) {
+        const float2 s = shares[(i - cut.first) * cut.runs + q];
         c1 += s.x;
         c2 += s.y;
       }
@@ -505,8 +511,7 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_shares(const __grid_co
       }
     }
     s = row_sum2<kThreads>(s, kThreads, sh[turn & 1]);
-    if (threadIdx.x < kCutWarps)
-      shares[((i - cut.first) * cut.runs + at.run) * kCutWarps + threadIdx.x] = threadIdx.x ? make_float2(0.0f, 0.0f) : make_float2(s.x, s.y);
+    if (threadIdx.x == 0) shares[(i - cut.first) * cut.runs + at.run] = make_float2(s.x, s.y);
   }
 }
 
@@ -536,8 +541,8 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
     const float mean = p.mean[i], rstd = p.rstd[i];
     float c1 = 0.0f, c2 = 0.0f;
     if (p.dx) {  // every warp adds up the row's shares for itself, in one order
-      for (int64_t q = threadIdx.x & 31; q < cut.runs * kCutWarps; q += 32) {
-        const float2 s = shares[(i - cut.first) * cut.runs * kCutWarps + q];
+      for (int64_t q = threadIdx.x & 31; q < cut.runs; q += 32) {
+        const float2 s = shares[(i - cut.first) * cut.runs + q];
         c1 += s.x;
         c2 += s.y;
       }
@@ -782,7 +787,7 @@ size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
   // The fewest bytes an element leave the most rows to a batch; parts grow with rows and the period.
   const int64_t runs = most_runs(cols), batch = batch_rows(rows, cols, 4);
   const size_t cut = round16((size_t)cut_parts(batch, runs, kGradBlocks, 8) * 2 * (size_t)cols * sizeof(float)) +
-                     (size_t)batch * (size_t)runs * kCutWarps * sizeof(float2);
+                     (size_t)batch * (size_t)runs * sizeof(float2);
   const int64_t teams = cols <= kSpread * kThreads * kMost ? kGradBlocks / spread_blocks(cols) : 0;
   const size_t spread = (size_t)(rows < teams ? rows : teams) * 2 * (size_t)cols * sizeof(float), most = whole > cut ? whole : cut;
   return most > spread ? most : spread;
