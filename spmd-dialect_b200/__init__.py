@@ -1,11 +1,13 @@
 """spmd-dialect_b200: B200 (sm_100a) kernels for the three kernel families
 spmd-dialect's SPMDToGPU lowering emits -- elementwise foralls, promoted
 stencil sweeps (3-point, Jacobi-2D, Jacobi-3D) and hierarchical reductions --
-behind the C ABI of include/spmd_b200.h.
+and the memory-bound operators of a training step (layer norm and its
+gradients, gradient norm, AdamW), behind the C ABI of include/spmd_b200.h.
 
 Layout of the package:
     csrc/            CUDA kernels (sm_100a) and the C ABI (api.cu)
     build.py         nvcc build of libspmdb200.so + spmdb200_kernels.cubin
+    csrc/tensor_lists.cpp  reads lists of tensors for kernels.py (_tensor_lists.so)
     _lib.py          ctypes binding of the C ABI (no fallback: raises if missing)
     kernels.py       device entries over torch tensors
     host.py          host-buffer entries in harness/run_host.py's convention

@@ -313,14 +313,14 @@ __device__ __forceinline__ void take_chunks(const uint4 (&slot)[N][32], int lane
 }
 
 // A warp takes state blocks of 256 elements, eight consecutive ones a lane: the
-// block's largest magnitudes are one integer maximum over the warp each.  10
-// bytes an element against some 30 instructions, so that instructions and the
-// wait for memory both count: a warp has `units` blocks of a tensor in a row,
-// one look-up for all of them, and the next on its way to shared memory while
-// one is computed.  A grid of all pieces hides a block's first wait behind
-// others (217 us for 2^27 bf16 parameters, 6.2 TB/s; 240 with three blocks an
-// SM that loop).  Two stages and 80 registers (three blocks an SM) measured
-// best: 238 looping, three stages 245, 64 registers and four blocks 245.
+// block's largest magnitudes are one integer maximum over the warp each.  2^27
+// bf16 parameters take 267 us, 5.05 TB/s of 10 bytes an element, bound by
+// instructions (an SM issues in 72 % of the cycles): the states' roundings are the
+// formula's, one by one, which costs 36 us of it.  A warp has `units` blocks of a
+// tensor in a row, one look-up for all of them, and the next on its way to shared
+// memory while one is computed.  Measured before the roundings were exact: a grid
+// of all pieces, whose blocks hide each other's first wait, 217 us, three blocks an
+// SM that loop 238 (with three stages 245, with four blocks of 64 registers 245).
 template <class P, class G, int CAP>
 __global__ void __launch_bounds__(kThreads, 3) adamw_8(const __grid_constant__ AdamTable<CAP> t, int units) {
   extern __shared__ __align__(16) unsigned char smem[];
@@ -421,7 +421,8 @@ cudaError_t launch(AdamTable<CAP> &t, bool bits8, unsigned sms, cudaStream_t s) 
     return cudaGetLastError();
   }
   // As many state blocks in a row per warp as leave every SM 32 pieces, up to
-  // kMostUnits (234 us at 4 for 2^27 parameters, 217 at 8, 16 and 32).
+  // kMostUnits (for 2^27 parameters 234 us at 4, 217 at 8, 16 and 32, before the
+  // roundings were exact).
   int units = 1;
   while (units < kMostUnits && pieces >= (int64_t)units * 2 * 32 * sms) units *= 2;
   int64_t at = 0;

@@ -123,15 +123,16 @@ ln_forward_stream(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
 // the fewer bytes are under way: 16-bit rows go four at a time (148 us, two 174).
 // As many clusters as are resident, whatever rows they take where all start
 // alike: 201 and 136 us, 5.3 and 3.9 TB/s; what is left is the exchange's wait.
-constexpr int kSpreadStages = 3;
 template <class TX>
 constexpr int kSpreadRows = 8 / (int)sizeof(TX);
+template <class TX, bool APART>
+constexpr int kSpreadStages = APART && sizeof(TX) == 2 ? 2 : 3;  // as two blocks' stages and sums fit an SM
 
 template <class TX, class TY, int W, bool WRAPS, bool APART>
 __global__ void __launch_bounds__(kThreads, 2)
 ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const __grid_constant__ RowWalk yr, const void *w,
                   const void *b, int wtype, int64_t rows, int cols, float eps, float *mean_out, float *rstd_out, int blocks) {
-  constexpr int NV = kMost / W, R = kSpreadRows<TX>, kWarps = kThreads / 32;
+  constexpr int NV = kMost / W, R = kSpreadRows<TX>, kWarps = kThreads / 32, kStages = kSpreadStages<TX, APART>;
   using In = Source<W, NV, kThreads, APART, TX>;
   constexpr int kStage = R * In::kBytes;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -147,7 +148,7 @@ ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   const int shift = (int)((APART ? (uintptr_t)to / sizeof(TY) : (uintptr_t)from / sizeof(TX)) % W);
   const Held<W, NV> have = held<W, NV>(cols, lane, lanes, shift);
   In in;
-  in.place(from, cols, lane, lanes, shift, have, smem, kSpreadStages * R, In::kBytes);
+  in.place(from, cols, lane, lanes, shift, have, smem, kStages * R, In::kBytes);
   to += lane * W - shift;
   from += in.start;
   int stage_in = 0, stage = 0, fetched = 0;
@@ -160,10 +161,10 @@ ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
       from = next_row<WRAPS>(from, x + in.start, xr, i + fetched * step);
     }
     copy_commit();  // empty past the last row, so that the count of groups stays
-    stage_in = stage_in == (kSpreadStages - 1) * kStage ? 0 : stage_in + kStage;
+    stage_in = stage_in == (kStages - 1) * kStage ? 0 : stage_in + kStage;
   };
 #pragma unroll
-  for (int q = 0; q < kSpreadStages - 1; ++q) fetch();
+  for (int q = 0; q < kStages - 1; ++q) fetch();
   for (int e = threadIdx.x; e < blocks * kWarps; e += kThreads) {  // as held() has it
     int n = 0;
 #pragma unroll
@@ -184,7 +185,7 @@ ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
   cluster_wait();  // the others have begun
   for (int turn = 0, space = 0; turn < turns; turn += R, space ^= 1) {
     fetch();
-    copy_wait<kSpreadStages - 1>();
+    copy_wait<kStages - 1>();
     F2 t[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -248,7 +249,7 @@ ln_forward_spread(const TX *x, const __grid_constant__ RowWalk xr, TY *y, const 
       }
       to = next_row<WRAPS>(to, y + lane * W - shift, yr, i + (turn + q + 1) * step);
     }
-    stage = stage == (kSpreadStages - 1) * kStage ? 0 : stage + kStage;
+    stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;
   }
   copy_wait<0>();
 }
@@ -572,7 +573,7 @@ cudaError_t forward_streamed(const LayerNormProblem &p, int spare, cudaStream_t 
 
 template <class TX, class TY, bool WRAPS, bool APART>
 cudaError_t forward_spread(const LayerNormProblem &p, int blocks, cudaStream_t s) {
-  constexpr int W = kWidth<TX, TY>, bytes = kSpreadStages * kSpreadRows<TX> * Source<W, kMost / W, kThreads, APART, TX>::kBytes;
+  constexpr int W = kWidth<TX, TY>, bytes = kSpreadStages<TX, APART> * kSpreadRows<TX> * Source<W, kMost / W, kThreads, APART, TX>::kBytes;
   auto kernel = ln_forward_spread<TX, TY, W, WRAPS, APART>;
   if (cudaError_t e = allow_shared(kernel, bytes)) return e;
   int most = 0;

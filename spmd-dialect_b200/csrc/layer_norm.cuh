@@ -145,9 +145,10 @@ __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
 //
 // Twelve blocks at most: the more, the longer a row waits for all of them, and the
 // fewer clusters fit the groups of SMs that hold them.  Against the two passes
-// below, us: 4096 x 40001 f32 343 to 462 forward, 554 to 784 backward, bf16 249 to 316
-// and 306 to 519; 4096 x 49152 f32 382 to 472 and 604 to 711, bf16 302 to 311 and 399 to
-// 491; with sixteen blocks 2048 x 65536 bf16 took 335 forward against some 200.
+// below, us: the gradient of 4096 x 40001 f32 554 to 748, bf16 305 to 464, of 4096 x
+// 49152 579 to 656 and 314 to 416; the forward pass of 49152 is 370 to some 410 in
+// f32 and level in bf16 (243 to some 235).  Sixteen blocks are behind on both: 2048 x
+// 65536 bf16 335 forward and 407 backward, two passes some 160 and 300.
 constexpr int kSpread = 12;
 __device__ __forceinline__ float *in_block(float *p, int rank) {
   return cooperative_groups::this_cluster().map_shared_rank(p, rank);
@@ -514,10 +515,11 @@ struct Cut {
 
 // Runs at the most: a start within a vector may need one more.
 inline int64_t most_runs(int64_t cols) { return (cols + 7 + kRun - 1) / kRun; }
-// Rows of a batch at `bytes` read per column.
+// Rows of a batch at `bytes` read per column: 88 MB, of the L2's 126 (72 MB: the
+// gradient of 1024 x 131072 bf16 297 us, so 273; 56 MB: 5 % slower still).
 inline int64_t batch_rows(int64_t rows, int64_t cols, int bytes) {
   if (rows <= 8 || rows * cols * bytes <= (int64_t)100 << 20) return rows;
-  const int64_t fit = ((int64_t)72 << 20) / bytes / cols, batch = fit < 8 ? 8 : fit / 8 * 8;
+  const int64_t fit = ((int64_t)88 << 20) / bytes / cols, batch = fit < 8 ? 8 : fit / 8 * 8;
   return batch < rows ? batch : rows;
 }
 // Parts of a batch that give about `blocks` blocks.  A block's rows have one

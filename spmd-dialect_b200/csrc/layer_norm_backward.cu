@@ -282,7 +282,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
 
 // Longer rows (layer_norm.cuh), first pass: each run's share of a row's two sums.
 template <class TX, class TY, int W, bool WRAPS, bool APART>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, sizeof(TX) + sizeof(TY) == 4 ? 4 : 2)
 ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWalk gr, const __grid_constant__ RowWalk xr,
           const __grid_constant__ Cut cut, float2 *shares) {
   constexpr int NV = kCutMost / W;

@@ -380,6 +380,42 @@ def test_other_stream_and_capture(kernels):
         assert all(torch.equal(p, q) for p, q in zip((*a, *g), (*e, *eg)))
 
 
+@pytest.mark.parametrize("rows,cols", [(40, 12289), (500, 30000), (300, 200000), (1500, 60000)])
+def test_long_rows_captured_and_on_two_streams(kernels, rows, cols):
+    """Rows over several blocks and in batches, whose kernels overlap: captured, replayed back to
+    back, and on two streams at once, each call gives the bits that it gives alone."""
+    args = []
+    for seed in (1, 5):
+        x, dy = make((rows, cols), BF16, seed), make((rows, cols), BF16, seed + 1)
+        w, b = weights(cols, F32, seed + 2)
+        y, mean, rstd = kernels.layer_norm(x, w, b)
+        args.append((x, dy, w, b, (y, mean, rstd, *kernels.layer_norm_backward(dy, x, mean, rstd, w))))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for k, (x, dy, w, b, _) in enumerate(args):
+            with torch.cuda.stream(streams[k]):
+                y, mean, rstd = kernels.layer_norm(x, w, b)
+                got[k].append((y, mean, rstd, *kernels.layer_norm_backward(dy, x, mean, rstd, w)))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            assert all(torch.equal(p, q) for p, q in zip(g, args[k][4]))
+    got.clear()
+    x, dy, w, b, want = args[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, mean, rstd = kernels.layer_norm(x, w, b)
+        grads = kernels.layer_norm_backward(dy, x, mean, rstd, w)
+    for _ in range(3):
+        for t in (y, mean, rstd, *grads):
+            t.fill_(float("nan"))
+        graph.replay()
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip((y, mean, rstd, *grads), want))
+
+
 def test_refusals(kernels):
     err = spmd_mod("_lib").SpmdError
     x, w = make((4, 32), F32, 1), make((32,), F32, 2)
