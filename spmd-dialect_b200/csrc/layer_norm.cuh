@@ -148,7 +148,7 @@ __device__ __forceinline__ F4 row_sum4(F4 v, int lanes, float4 *sh) {
 // below, us: the gradient of 4096 x 40001 f32 554 to 748, bf16 305 to 464, of 4096 x
 // 49152 579 to 656 and 314 to 416; the forward pass of 49152 is 370 to some 410 in
 // f32 and level in bf16 (243 to some 235).  Sixteen blocks are behind on both: 2048 x
-// 65536 bf16 335 forward and 407 backward, two passes some 160 and 300.
+// 65536 bf16 335 forward and 407 backward, two passes 145 and 274 (of 8192 rows).
 constexpr int kSpread = 12;
 __device__ __forceinline__ float *in_block(float *p, int rank) {
   return cooperative_groups::this_cluster().map_shared_rank(p, rank);
