@@ -298,7 +298,9 @@ ln_forward(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, i
   }
 }
 
-// Two sets' count, mean and sum of squares around it join into those of both.
+// Two sets' count, mean and sum of squares around it join into those of both.  An
+// empty set's d is the other's whole mean, whose square may leave f32: the product
+// begins with the counts, which are zero then.
 struct Moments {
   float n, mean, m2;
 };
@@ -306,7 +308,7 @@ __device__ __forceinline__ Moments join(Moments a, Moments b) {
   const float n = a.n + b.n;
   if (n == 0.0f) return a;
   const float d = b.mean - a.mean, share = b.n / n;
-  return {n, fmaf(d, share, a.mean), a.m2 + b.m2 + d * d * a.n * share};
+  return {n, fmaf(d, share, a.mean), a.m2 + b.m2 + d * (d * (a.n * share))};
 }
 __device__ __forceinline__ Moments join_warp(Moments a) {
 #pragma unroll
