@@ -279,9 +279,12 @@ __device__ __forceinline__ Scales step8(float p[8], float g[8], float m[8], floa
       r[e] = sqrtf(g[e]) / now.v;
     }
   }
+  // With an infinite scale (a square past f32) every code has to stay 0 or NaN, which both decode to NaN: the least
+  // code would stand for infinity, and the block would silently stop moving.
+  const float least = isinf(now.v) ? 0.0f : kLeastCode;
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    if (g[e] > 0.0f) r[e] = at_least(r[e], kLeastCode);
+    if (g[e] > 0.0f) r[e] = at_least(r[e], least);
   return now;
 }
 
