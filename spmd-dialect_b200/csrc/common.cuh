@@ -184,8 +184,11 @@ __device__ __forceinline__ void st_f4(float *p, float4 v) {
 // A kernel launched with launch_pdl() may start while the previous kernel of
 // its stream is finishing (its launch and prologue overlap that kernel's
 // tail); pdl_wait() then blocks until the previous kernel has completed and
-// its memory is visible, so nothing may read or write global memory before
-// it (an L2 prefetch, which returns no data, may run earlier).
+// its memory is visible.  Before it nothing may be written, and nothing read that
+// a kernel still running may write: where the first kernel of a call is launched
+// plainly, the later ones may begin to read the call's inputs (an L2 prefetch, which
+// returns no data, may run earlier anywhere).  What is read after it is not
+// read-only for the kernel's lifetime: no const __restrict__, no __ldg.
 // pdl_trigger() lets the next such launch start early.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ unsigned atom_add_acq_rel_gpu(unsigned *p, unsigned v) {

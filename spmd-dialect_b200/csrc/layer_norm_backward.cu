@@ -580,9 +580,10 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
 }
 
 // dw and db from the partial rows (part p: dw at row 2p, db at row 2p + 1): `depth`
-// threads a column, each of them every depth-th part.
+// threads a column, each of them every depth-th part.  It may start while the kernel
+// before still writes `part`, which therefore is no read-only memory.
 __global__ void __launch_bounds__(1024)
-ln_finish(const float *__restrict__ part, int parts, int64_t cols, int depth, void *dw, void *db, int type) {
+ln_finish(const float *part, int parts, int64_t cols, int depth, void *dw, void *db, int type) {
   __shared__ float sh[2][1024];
   pdl_wait();
   const int width = blockDim.x / depth, tx = threadIdx.x % width, ty = threadIdx.x / width;
