@@ -196,7 +196,8 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
     F2 c[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      // An element outside the row, or of a row past the last, has g = 0 and a finite x: it adds nothing to any sum.
+      // An element outside the row has g = 0 and x = 0: it adds nothing to any sum, as rstd multiplies a, which is
+      // zero there, and not mean, which may take it past f32.  The sums of a row past the last are not used.
       const bool live = turn + q < mine;
       const int here = stage * kStage + q * kRow;
       stat[q] = live ? stats[stage * R + q][slot] : make_float2(0.0f, 0.0f);
@@ -212,7 +213,7 @@ ln_backward_stream(const __grid_constant__ Back<TX, TY> p, const __grid_constant
         for (int e = 0; e < W / 2; ++e) {
           const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
           s1 = add2(s1, a);
-          s2 = fma2(a, mul2(add2(x[e], both(-stat[q].x)), both(stat[q].y)), s2);
+          s2 = fma2(mul2(a, both(stat[q].y)), add2(x[e], both(-stat[q].x)), s2);
         }
       }
       c[q] = {s1.x + s1.y, s2.x + s2.y};
@@ -344,7 +345,7 @@ ln_shares(const __grid_constant__ Back<TX, TY> p, const __grid_constant__ RowWal
       for (int e = 0; e < W / 2; ++e) {
         const F2 a = mul2(g[e], {w[k][2 * e], w[k][2 * e + 1]});
         s1 = add2(s1, a);
-        s2 = fma2(a, mul2(add2(x[e], both(stat.x)), both(stat.y)), s2);
+        s2 = fma2(mul2(a, both(stat.y)), add2(x[e], both(stat.x)), s2);
       }
     }
     stage = stage == (kStages - 1) * kStage ? 0 : stage + kStage;

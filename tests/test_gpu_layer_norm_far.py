@@ -8,6 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from test_gpu_layer_norm import BF16, F32, check_forward, make, weights  # noqa: E402
+from train_ref import assert_within, norm_back_ref, rounded  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,21 @@ def test_a_bad_row_stays_alone_in_long_and_strided_rows(kernels, cols, kind):
         assert torch.equal(p[good], q[good])
     for t in (y1, dx1):
         assert all(bool(t[k].isnan().all()) for k in (4, 6, 7))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("cols", [5, 37, 100, 1001, 4096, 5003, 8200, 20001, 60001])
+def test_gradients_of_constant_far_rows(kernels, cols, apart, dtype):
+    """A constant row has xh = 0 and a finite gradient, also where mean * rstd leaves f32."""
+    x, dy = torch.full((5, cols), 1e33, device="cuda"), make((5, cols), dtype, 2)
+    x[1] = 0.0
+    x[2] = -1e36
+    x = x.to(dtype)
+    mean, rstd = x[:, 0].float().contiguous(), torch.full((5,), 1e6, device="cuda")
+    if apart:
+        x, dy = (torch.nn.functional.pad(t, (at, 9 - at))[:, at:at + cols] for t, at in ((x, 3), (dy, 2)))
+    w, _ = weights(cols, F32, 3)
+    want = norm_back_ref(dy, x, mean, rstd, w)
+    dx, _, _ = kernels.layer_norm_backward(dy, x, mean, rstd, w, wgrad=False)
+    assert_within(dx, want[0], want[3] + rounded(want[0].abs() + want[3], dtype), "dx")
