@@ -117,10 +117,11 @@ __global__ void __launch_bounds__(kThreads) norm_finish(const double *parts, int
   acc = block_sum(acc, sh);
   if (threadIdx.x == 0) {
     const double len = sqrt(acc);
-    *norm = (float)len;
-    // A norm that is not finite gives NaN, not 0: 0 times an infinite gradient
+    const float f = (float)len;
+    *norm = f;
+    // A norm that is not finite, as f32 holds it, gives NaN, not 0: 0 times an infinite gradient
     // would be NaN anyway, and a step that sees a NaN factor leaves all as it was.
-    if (scale) *scale = isfinite(len) ? (len > (double)max_norm ? (float)((double)max_norm / len) : 1.0f) : nanf("");
+    if (scale) *scale = isfinite(f) ? (len > (double)max_norm ? (float)((double)max_norm / len) : 1.0f) : nanf("");
   }
 }
 

@@ -6,7 +6,8 @@ import math
 import pytest
 
 torch = pytest.importorskip("torch")
-from test_gpu_adamw import F32, HYPER, decode, rand, state_8  # noqa: E402
+from test_gpu_adamw import F32, HYPER, decode, lists, rand, state_8  # noqa: E402
+from train_ref import U  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,17 @@ def test_step_8_bits_overflow_makes_the_block_nan(kernels, bad, v_only):
     kernels.adamw(p, g, **clean, **{**HYPER, "step": 8})
     kernels.adamw(q, g, **s, **{**HYPER, "step": 8})
     assert torch.equal(p[0][keep], q[0][keep]) and bool(q[0][~keep].isnan().all())
+
+
+def test_norm_past_f32(kernels):
+    """A norm that f32 does not hold is infinite, its scale NaN, and the step leaves everything as it was."""
+    p, g, m, v = lists([1000, 70], F32, F32)
+    g = [torch.full_like(t, 3e38) for t in g]
+    norm, scale = kernels.grad_norm(g, 1.0)
+    assert math.isinf(norm.item()) and math.isnan(scale.item())
+    before = [t.clone() for t in p + m + v]
+    kernels.adamw(p, g, m, v, grad_scale=scale, **HYPER)
+    assert all(torch.equal(a, b) for a, b in zip(before, p + m + v))
+    # The largest norms that f32 holds are finite, and clipped.
+    norm, scale = kernels.grad_norm([torch.full((4,), 1.5e38, device="cuda")], 1.0)
+    assert norm.item() == pytest.approx(3e38, rel=4 * U) and scale.item() == pytest.approx(1 / 3e38, rel=4 * U, abs=2.0 ** -150)
