@@ -553,6 +553,7 @@ int spmdb200_grad_norm(int count, const void *const *grads, const int64_t *sizes
  * code * scale, scale = max(largest magnitude / 448, 2^-120); a root above
  * zero keeps the smallest code at least.  A NaN or infinity in m, or in v
  * (whose squares may overflow), makes that state of the whole block NaN.
+ * With them an eps above zero counts as 2^-126 at least.
  * lr_dev, step_dev: device scalars read in place of lr and step where not NULL
  * (a step below 1 counts as 1), so that a captured launch can be replayed with
  * new values.  grad_scale: device factor, NULL for 1; when it is NaN or

@@ -505,6 +505,9 @@ cudaError_t launch_adamw(const AdamWProblem &p, cudaStream_t s) {
   h.beta1 = (float)p.beta1, h.beta2 = (float)p.beta2;
   h.rest1 = (float)(1.0 - p.beta1), h.rest2 = (float)(1.0 - p.beta2);
   h.eps = (float)p.eps;
+  // rcp_near takes a subnormal for zero, and zero over zero is NaN where an element has no gradient yet.  A root above
+  // zero is 2^-75 at least, beside which any such eps is lost.
+  if (p.bits8 && p.eps > 0.0 && h.eps < 0x1p-126f) h.eps = 0x1p-126f;
   h.beta1_d = p.beta1, h.beta2_d = p.beta2;
   h.lr = (float)p.lr;
   h.step = p.step;

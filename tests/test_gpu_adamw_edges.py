@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from test_gpu_adamw import F32, HYPER, decode, lists, rand, state_8  # noqa: E402
-from train_ref import U  # noqa: E402
+from train_ref import U, assert_within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +38,25 @@ def test_step_8_bits_overflow_makes_the_block_nan(kernels, bad, v_only):
     kernels.adamw(p, g, **clean, **{**HYPER, "step": 8})
     kernels.adamw(q, g, **s, **{**HYPER, "step": 8})
     assert torch.equal(p[0][keep], q[0][keep]) and bool(q[0][~keep].isnan().all())
+
+
+@pytest.mark.parametrize("n", [100, 256, 4096, 70001])
+@pytest.mark.parametrize("eps", [1e-38, 1e-40, 1e-45])
+def test_step_8_bits_subnormal_eps(kernels, eps, n):
+    """An element whose gradient and states are zero only decays, however small eps is."""
+    p, g = [rand(n, F32, 1)], [rand(n, F32, 2)]
+    g[0][::3] = 0.0
+    s = kernels.adamw_state(p, bits=8)
+    before = p[0].clone()
+    kernels.adamw(p, g, **s, **{**HYPER, "step": 1, "eps": eps})
+    want = before[::3].double() * (1 - 1e-3)
+    assert_within(p[0][::3], want, 4 * U * want.abs(), "decayed only")
+    assert bool(p[0].isfinite().all())
+    moved = torch.ones(n, dtype=torch.bool, device="cuda")
+    moved[::3] = False
+    # From zeroed states the first step moves by lr: 12 roundings bound the quotient's.
+    want = before.double() * (1 - 1e-3) - 1e-2 * torch.sign(g[0].double())
+    assert_within(p[0][moved], want[moved], (4 * U * before.double().abs() + 12 * U * 1e-2 + 2 * U * want.abs())[moved], "moved")
 
 
 def test_norm_past_f32(kernels):
