@@ -8,7 +8,8 @@ dependency on libcuda, so the library also loads on machines without a GPU
 driver).  refabi.cu -- the kernels with the reference's PTX entry names -- is
 compiled to spmdb200_kernels.cubin for cuModuleLoadData callers.
 tensor_lists.cpp -- the reader of lists of torch tensors -- becomes the Python
-module _tensor_lists.so, against the installed torch's headers.
+module _tensor_lists.so, against the installed torch's headers (and anew when
+another torch or Python is installed; without torch it is left out).
 libspmdb200_checked.so is the same library with the general kernels
 (forall_map.cu, stencil_nd.cu) compiled with -DSPMDB200_CHECKED.  ptxas
 register / spill reports go to _build/ptxas.log.
@@ -35,6 +36,7 @@ CHECKED_LIB = PKG / "libspmdb200_checked.so"
 CHECKED_UNITS = ("forall_map.cu", "stencil_nd.cu")
 CUBIN = PKG / "spmdb200_kernels.cubin"
 LISTS = PKG / "_tensor_lists.so"
+LISTS_FOR = BUILD / "tensor_lists.for"  # the Python and torch that LISTS was built for
 INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -69,6 +71,23 @@ def _run(cmd: list[str]) -> str:
     return r.stdout + r.stderr
 
 
+def _lists_for() -> str | None:
+    """What _tensor_lists.so depends on besides its sources; None without torch."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    return f"Python {sys.version} torch {torch.__version__} {torch.version.git_version}"
+
+
+def lists_stale() -> bool:
+    now = _lists_for()
+    if now is None:
+        return False
+    return (_stale(LISTS, [CSRC / "tensor_lists.cpp", *INCLUDE.glob("*.h")]) or not LISTS_FOR.exists()
+            or LISTS_FOR.read_text() != now)
+
+
 def build_lists() -> None:
     """_tensor_lists.so: plain C++ against torch's and Python's headers."""
     import torch
@@ -79,6 +98,7 @@ def build_lists() -> None:
           *[f"-I{p}" for p in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"])],
           str(CSRC / "tensor_lists.cpp"), "-o", str(LISTS), *[f"-L{p}" for p in libs], *[f"-Wl,-rpath,{p}" for p in libs],
           "-ltorch_python", "-ltorch_cpu", "-lc10"])
+    LISTS_FOR.write_text(_lists_for())
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, checked: bool = True) -> Path:
@@ -91,14 +111,12 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, c
     logs: dict[str, str] = {}
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 4)) as ex:
         futs = {ex.submit(_run, [cc, *NVCC_FLAGS, "-c", str(u), "-o", str(o)]): u for u, o in todo}
-        lists = ex.submit(build_lists) if force or _stale(LISTS, [CSRC / "tensor_lists.cpp", *INCLUDE.glob("*.h")]) else None
+        lists = ex.submit(build_lists) if (force and _lists_for()) or lists_stale() else None
         cubin_src = CSRC / "refabi.cu"
         if force or _stale(CUBIN, [cubin_src] + deps):
             futs[ex.submit(_run, [cc, *NVCC_FLAGS, "-cubin", str(cubin_src), "-o", str(CUBIN)])] = cubin_src
         for f in cf.as_completed(futs):
             logs[futs[f].name] = f.result()
-        if lists is not None:
-            lists.result()
     if force or todo or _stale(LIB, objs):
         _run([cc, "-shared", *ARCH, "-cudart", "static", "-Xcompiler", "-fPIC", "-o", str(LIB),
               *map(str, objs), "-lpthread", "-ldl", "-lrt"])
@@ -126,6 +144,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, c
     if verbose:
         for name, text in sorted(logs.items()):
             print(f"==== {name}\n{text}")
+    if lists is not None:
+        lists.result()  # last: the library does not need it
     return LIB
 
 

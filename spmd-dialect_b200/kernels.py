@@ -14,7 +14,6 @@ from array import array
 import torch
 
 from ._lib import c_i, c_p, call, lib
-from ._tensor_lists import read as _read_list
 from .forall_program import insn as map_insn  # noqa: F401  (re-exported)
 
 _DTYPES = {torch.float32: "f32", torch.int32: "i32", torch.uint8: "u8", torch.float64: "f64"}
@@ -390,6 +389,19 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
          _TYPES[x.dtype], at + 16 * rank, mean.data_ptr(), rstd.data_ptr(), w, wtype, dv.data_ptr(), at + 24 * rank, dw,
          db, dtype, ws.data_ptr(), ws.nbytes, _raw_stream(dev))
     return dx, dweight, dbias
+
+
+def _read_list(*args):
+    """_tensor_lists.read, which takes this function's place at its first use:
+    nothing but lists of tensors needs the module, which belongs to one torch."""
+    global _read_list
+    try:
+        from ._tensor_lists import read
+    except ImportError as e:
+        raise ImportError("lists of tensors need _tensor_lists.so, built for this torch by "
+                          f"`python spmd-dialect_b200/build.py`: {e}") from e
+    _read_list = read
+    return read(*args)
 
 
 def _kinds(*dtypes: torch.dtype) -> int:
