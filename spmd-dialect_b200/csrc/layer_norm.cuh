@@ -645,8 +645,10 @@ inline int row_vectors(int64_t cols, int lanes, int w) {
 }
 
 // Blocks of streamed rows: a row each, at most `most`, and where they come
-// around again a stride of rows that is a multiple of w.
+// around again a stride of rows that is a multiple of w.  Where fewer than w are
+// resident at once (a part of a GPU), w of them take turns.
 inline int stream_grid(int64_t rows, int64_t groups, int most, int w) {
+  if (most < w) most = w;
   const int64_t blocks = (rows + groups - 1) / groups;
   if (blocks <= most) return (int)blocks;
   while (most * groups % w != 0) --most;
