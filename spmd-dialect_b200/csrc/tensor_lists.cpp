@@ -93,7 +93,27 @@ PyObject *read(PyObject *, PyObject *args) {
   return out;
 }
 
-PyMethodDef methods[] = {{"read", read, METH_VARARGS, "read(what, tensors, device, kinds, like)"}, {nullptr, nullptr, 0, nullptr}};
+// written(lists...): raises the version counter of every tensor of lists that a kernel
+// has written, as in-place operations of torch do, so that autograd refuses what
+// it saved of them.  A list, and an entry, may be None.
+PyObject *written(PyObject *, PyObject *args) {
+  for (Py_ssize_t a = 0; a < PyTuple_GET_SIZE(args); ++a) {
+    PyObject *list = PyTuple_GET_ITEM(args, a);
+    if (list == Py_None) continue;
+    if (!PyList_Check(list)) return PyErr_Format(PyExc_TypeError, "written: argument %zd is no list", a);
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(list); ++k) {
+      PyObject *o = PyList_GET_ITEM(list, k);
+      if (!THPVariable_Check(o)) continue;
+      const at::Tensor &x = THPVariable_Unpack(o);
+      if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // inference tensors have no counter
+    }
+  }
+  Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {{"read", read, METH_VARARGS, "read(what, tensors, device, kinds, like)"},
+                         {"written", written, METH_VARARGS, "written(lists...)"},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -215,8 +215,11 @@ def jacobi3d(u: torch.Tensor, v: torch.Tensor, sweeps: int, res_every: int = 0, 
 
 # ---- training-step operators ---------------------------------------------------
 # They take f32, f16 and bf16 tensors, run on the tensors' own device (current or
-# not) and on its current stream unless `stream` says otherwise, and read or
-# write no autograd state: gradients are what the *_backward entry returns.
+# not) and on its current stream unless `stream` says otherwise.  They record no
+# autograd graph: gradients are what the *_backward entry returns.  A given tensor
+# that a call writes has its version counter raised, so that autograd refuses a
+# graph that saved it before; adamw raises those of parameters and copies, which
+# graphs hold, and not its states' (the replay of a captured call raises none).
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _E4M3 = torch.float8_e4m3fn
 STATE_BLOCK = 256  # elements that share one scale of an 8-bit optimizer state
@@ -241,6 +244,9 @@ def _at(dev: int, stream):
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+_raise_versions = torch.autograd.graph.increment_version
 
 
 def _ptr(a: array) -> int:
@@ -296,10 +302,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     shape = x.shape
     if not shape:
         raise ValueError("layer_norm: x needs a dimension to normalise over")
-    if out is None:
-        out = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
-    else:
+    given = out is not None
+    if given:
         _norm_operand("out", out, shape, dev, dtype)
+    else:
+        out = torch.empty(shape, dtype=dtype or x.dtype, device=x.device)
     _norm_types(x, out.dtype)
     w = b = m = r = mean = rstd = None
     wtype = 0
@@ -322,6 +329,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     at = _ptr(dims)
     call("spmdb200_layer_norm", rank, at, xv.data_ptr(), _TYPES[x.dtype], at + 8 * rank, ov.data_ptr(),
          _TYPES[out.dtype], at + 16 * rank, w, b, wtype, eps, m, r, room, room_bytes, _raw_stream(dev))
+    if given:
+        _raise_versions(out)
     return out, mean, rstd
 
 
@@ -359,6 +368,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     _norm_types(x, dy.dtype)
     _norm_vector("mean", mean, shape[:-1], dev, torch.float32)
     _norm_vector("rstd", rstd, shape[:-1], dev, torch.float32)
+    written = [t for t in (dx, dweight, dbias) if t is not None]
     w = dw = db = None
     wtype = dtype = 0
     if weight is not None:
@@ -388,19 +398,21 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     call("spmdb200_layer_norm_backward", rank, at, gv.data_ptr(), _TYPES[dy.dtype], at + 8 * rank, xv.data_ptr(),
          _TYPES[x.dtype], at + 16 * rank, mean.data_ptr(), rstd.data_ptr(), w, wtype, dv.data_ptr(), at + 24 * rank, dw,
          db, dtype, ws.data_ptr(), ws.nbytes, _raw_stream(dev))
+    if written:
+        _raise_versions(written)
     return dx, dweight, dbias
 
 
 def _read_list(*args):
     """_tensor_lists.read, which takes this function's place at its first use:
     nothing but lists of tensors needs the module, which belongs to one torch."""
-    global _read_list
+    global _read_list, _written
     try:
-        from ._tensor_lists import read
+        from ._tensor_lists import read, written
     except ImportError as e:
         raise ImportError("lists of tensors need _tensor_lists.so, built for this torch by "
                           f"`python spmd-dialect_b200/build.py`: {e}") from e
-    _read_list = read
+    _read_list, _written = read, written
     return read(*args)
 
 
@@ -498,7 +510,8 @@ def adamw(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), e
         if m_blocks != blocks or v_blocks != blocks:
             raise ValueError(f"adamw: 8-bit states need one scale per {STATE_BLOCK} elements of each parameter")
     if copies is not None:
-        c, _, c_types = _read_list("adamw: copies", list(copies), dev, _COPIES, params)
+        copies = list(copies)
+        c, _, c_types = _read_list("adamw: copies", copies, dev, _COPIES, params)
     decay = array("d", weight_decay) if hasattr(weight_decay, "__len__") else array("d", [weight_decay]) * n
     if len(decay) != n:
         raise ValueError("adamw: weight_decay is a number or one per parameter")
@@ -511,4 +524,5 @@ def adamw(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), e
         factor = _scalar("grad_scale", grad_scale, dev, torch.float32)
     call("spmdb200_adamw", n, p, p_types, g, g_types, sizes, m, v, bits, m_scales, v_scales, c, c_types, _ptr(decay), lr,
          lr_dev, betas[0], betas[1], eps, step, step_dev, factor, _raw_stream(dev))
+    _written(params, copies)
     return params

@@ -89,3 +89,19 @@ def test_no_torch_no_reader(build, monkeypatch):
     """The library itself needs no torch: without one there is nothing to read lists of."""
     monkeypatch.setitem(sys.modules, "torch", None)
     assert not build.lists_stale()
+
+
+def test_written_raises_versions():
+    run("", """
+import torch
+kernels._read_list("list", [], 0, 1, None)
+a, b = torch.ones(3), torch.ones(5)
+with torch.inference_mode():
+    c = torch.ones(2)
+kernels._written([a, None, b, c], None, [a])
+assert a._version == 2 and b._version == 1
+try:
+    kernels._written((a,))
+except TypeError:
+    assert a._version == 2
+""")
