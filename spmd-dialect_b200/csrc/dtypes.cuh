@@ -38,11 +38,6 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ float load_as_f32(const void *p, int type, int64_t i) {
-  if (type == kF32) return static_cast<const float *>(p)[i];
-  if (type == kF16) return __half2float(static_cast<const __half *>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
 __device__ __forceinline__ void store_from_f32(void *p, int type, int64_t i, float v) {
   if (type == kF32) static_cast<float *>(p)[i] = v;
   else if (type == kF16) static_cast<__half *>(p)[i] = __float2half_rn(v);
@@ -119,12 +114,6 @@ __device__ __forceinline__ void unpack8(uint4 q, float v[8]) {
 template <class T>
 __device__ __forceinline__ void load8(const T *p, float v[8]) {
   unpack8<T>(ld_u4(p), v);
-}
-// W elements of a global tensor.
-template <int W, class T>
-__device__ __forceinline__ void load_vec(const T *p, float *v) {
-  if constexpr (W == 8) load8(p, v);
-  else load4(p, v);
 }
 // W elements that a thread has put into shared memory itself.
 template <int W, class T>

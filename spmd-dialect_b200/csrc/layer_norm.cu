@@ -267,7 +267,7 @@ ln_forward(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, i
   for (int64_t i = (int64_t)blockIdx.x * (kThreads / lanes) + group; i - group < rows; i += step) {
     const int n = i < rows ? cols : 0;
     float v[NV][W], s = 0.0f;
-    load_row<W, NV, false>(x + (n ? row_offset(xr, i) : 0), xr.sc, 0, n, lane, lanes, 0, 0.0f, v);
+    load_row<W, NV>(x + (n ? row_offset(xr, i) : 0), xr.sc, n, lane, lanes, 0.0f, v);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -290,7 +290,7 @@ ln_forward(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void *b, i
 #pragma unroll
       for (int e = 0; e < W; ++e) v[k][e] = fmaf(v[k][e] * rstd, wv[e], bv[e]);
     }
-    store_row<W, NV, false>(y + (n ? row_offset(yr, i) : 0), yr.sc, 0, n, lane, lanes, 0, v);
+    store_row<W, NV>(y + (n ? row_offset(yr, i) : 0), yr.sc, n, lane, lanes, v);
     if (lane == 0 && n) {
       if (mean_out) mean_out[i] = mean;
       if (rstd_out) rstd_out[i] = rstd;
@@ -488,7 +488,7 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
     float v[NV][W];
     for (int64_t r = rank; r < runs; r += blocks) {
       const int n = cols - r * kLongRun < kLongRun ? (int)(cols - r * kLongRun) : (int)kLongRun;
-      load_row<W, NV, false>(px + r * kLongRun * xr.sc, xr.sc, 0, n, threadIdx.x, kLongLanes, 0, 0.0f, v);
+      load_row<W, NV>(px + r * kLongRun * xr.sc, xr.sc, n, threadIdx.x, kLongLanes, 0.0f, v);
       Moments t{0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -515,7 +515,7 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
     const float rstd = 1.0f / sqrtf(m.m2 / (float)cols + eps);
     for (int64_t r = rank; r < runs; r += blocks) {
       const int n = cols - r * kLongRun < kLongRun ? (int)(cols - r * kLongRun) : (int)kLongRun;
-      load_row<W, NV, false>(px + r * kLongRun * xr.sc, xr.sc, 0, n, threadIdx.x, kLongLanes, 0, 0.0f, v);
+      load_row<W, NV>(px + r * kLongRun * xr.sc, xr.sc, n, threadIdx.x, kLongLanes, 0.0f, v);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         float wv[W], bv[W];
@@ -524,7 +524,7 @@ ln_forward_long(const TX *x, Rows xr, TY *y, Rows yr, const void *w, const void 
 #pragma unroll
         for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - m.mean) * rstd, wv[e], bv[e]);
       }
-      store_row<W, NV, false>(py + r * kLongRun * yr.sc, yr.sc, 0, n, threadIdx.x, kLongLanes, 0, v);
+      store_row<W, NV>(py + r * kLongRun * yr.sc, yr.sc, n, threadIdx.x, kLongLanes, v);
     }
     if (threadIdx.x == 0 && rank == 0) {
       if (mean_out) mean_out[i] = m.mean;

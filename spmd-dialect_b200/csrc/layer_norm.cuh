@@ -184,44 +184,30 @@ template <int W, bool VEC>
 __device__ __forceinline__ int column(int k, int e, int lane, int lanes, int shift) {
   return VEC ? (k * lanes + lane) * W + e - shift : (k * W + e) * lanes + lane;
 }
-// The part of a row that a thread has of columns low <= c < high; `rest` elsewhere.
-// `p` is column 0's address.
-template <int W, int NV, bool VEC, class T>
-__device__ __forceinline__ void load_row(const T *p, int64_t stride, int low, int high, int lane, int lanes, int shift, float rest,
-                                         float (&v)[NV][W]) {
+// The elements of a row of any stride that a thread has of columns c < high; `rest`
+// elsewhere.  `p` is column 0's address.
+template <int W, int NV, class T>
+__device__ __forceinline__ void load_row(const T *p, int64_t stride, int high, int lane, int lanes, float rest, float (&v)[NV][W]) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int j = column<W, VEC>(k, 0, lane, lanes, shift);
-    if (VEC && j >= low && j + W <= high) {
-      load_vec<W>(p + j, v[k]);
-    } else {
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const int c = column<W, VEC>(k, e, lane, lanes, shift);
-        v[k][e] = c >= low && c < high ? to_f32(p[VEC ? (int64_t)c : c * stride]) : rest;
-      }
+    for (int e = 0; e < W; ++e) {
+      const int c = column<W, false>(k, e, lane, lanes, 0);
+      v[k][e] = c < high ? to_f32(p[c * stride]) : rest;
     }
-  }
 }
-template <int W, int NV, bool VEC, class T>
-__device__ __forceinline__ void store_row(T *p, int64_t stride, int low, int high, int lane, int lanes, int shift,
-                                          const float (&v)[NV][W]) {
+template <int W, int NV, class T>
+__device__ __forceinline__ void store_row(T *p, int64_t stride, int high, int lane, int lanes, const float (&v)[NV][W]) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int j = column<W, VEC>(k, 0, lane, lanes, shift);
-    if (VEC && j >= low && j + W <= high) {
-      store_vec<W>(p + j, v[k]);
-    } else {
+  for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const int c = column<W, VEC>(k, e, lane, lanes, shift);
-        if (c >= low && c < high) p[VEC ? (int64_t)c : c * stride] = from_f32<T>(v[k][e]);
-      }
+    for (int e = 0; e < W; ++e) {
+      const int c = column<W, false>(k, e, lane, lanes, 0);
+      if (c < high) p[c * stride] = from_f32<T>(v[k][e]);
     }
-  }
 }
-// The same of one vector of weight or bias; `rest` without one.  Column 0 is
-// element `first`.
+// A vector of weight or bias that a thread has of columns low <= c < high, `rest`
+// elsewhere and without one.  Column 0 is element `first`.
 template <int W, bool VEC>
 __device__ __forceinline__ void load_weight(const void *p, int type, int64_t first, int low, int high, int k, int lane, int lanes,
                                             int shift, float rest, float (&v)[W]) {

@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     const int n = i < p.rows ? cols : 0;
     const float mean = n ? p.mean[i] : 0.0f, rstd = n ? p.rstd[i] : 0.0f;
     float g[NV][W], x[NV][W];
-    load_row<W, NV, false>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, 0, n, lane, lanes, 0, 0.0f, g);
-    load_row<W, NV, false>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, 0, n, lane, lanes, 0, mean, x);
+    load_row<W, NV>(p.dy + (n ? row_offset(p.gr, i) : 0), p.gr.sc, n, lane, lanes, 0.0f, g);
+    load_row<W, NV>(p.x + (n ? row_offset(p.xr, i) : 0), p.xr.sc, n, lane, lanes, mean, x);
     F2 s{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(MAXT) ln_backward(const __grid_constant__ Back
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int e = 0; e < W; ++e) g[k][e] = (g[k][e] - c1 - x[k][e] * c2) * rstd;
-    if (n) store_row<W, NV, false>(p.dx + row_offset(p.dr, i), p.dr.sc, 0, n, lane, lanes, 0, g);
+    if (n) store_row<W, NV>(p.dx + row_offset(p.dr, i), p.dr.sc, n, lane, lanes, g);
   }
   if (p.part)
     reduce_columns<W, NV>(sw, sb, lanes, cols, sums, p.part, [&](int k, int e) { return column<W, false>(k, e, lane, lanes, 0); });
@@ -497,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_shares(const __grid_co
     const int64_t i = at.i + (int64_t)turn * cut.parts;
     const float mean = p.mean[i], rstd = p.rstd[i];
     float g[NV][W], x[NV][W];
-    load_row<W, NV, false>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, 0, n, threadIdx.x, kThreads, 0, 0.0f, g);
-    load_row<W, NV, false>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, 0, n, threadIdx.x, kThreads, 0, mean, x);
+    load_row<W, NV>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
+    load_row<W, NV>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
     F2 s{0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
       c2 = warp_sum_f32(c2) * inv_n;
     }
     float g[NV][W], x[NV][W];
-    load_row<W, NV, false>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, 0, n, threadIdx.x, kThreads, 0, 0.0f, g);
-    load_row<W, NV, false>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, 0, n, threadIdx.x, kThreads, 0, mean, x);
+    load_row<W, NV>(p.dy + row_offset(p.gr, i) + first * p.gr.sc, p.gr.sc, n, threadIdx.x, kThreads, 0.0f, g);
+    load_row<W, NV>(p.x + row_offset(p.xr, i) + first * p.xr.sc, p.xr.sc, n, threadIdx.x, kThreads, mean, x);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float w[W];
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 2) ln_strided_grads(const __grid_con
         g[k][e] = (g[k][e] * w[e] - c1 - xh * c2) * rstd;
       }
     }
-    if (p.dx) store_row<W, NV, false>(p.dx + row_offset(p.dr, i) + first * p.dr.sc, p.dr.sc, 0, n, threadIdx.x, kThreads, 0, g);
+    if (p.dx) store_row<W, NV>(p.dx + row_offset(p.dr, i) + first * p.dr.sc, p.dr.sc, n, threadIdx.x, kThreads, g);
   }
   if (!p.part) return;
 #pragma unroll
