@@ -66,6 +66,10 @@ PyObject *read(PyObject *, PyObject *args) {
           PyErr_Format(PyExc_TypeError, "%s: tensor %zd has dtype %s", what, k, c10::toString(x.scalar_type()));
           break;
         }
+        if (x.is_neg()) {  // its memory holds the negated values
+          PyErr_Format(PyExc_ValueError, "%s: tensor %zd is negated lazily (resolve_neg gives its values)", what, k);
+          break;
+        }
         if (!x.is_contiguous()) {
           PyErr_Format(PyExc_ValueError, "%s: tensor %zd is not contiguous", what, k);
           break;

@@ -286,6 +286,13 @@ def _norm_types(x: torch.Tensor, y: torch.dtype) -> None:
         raise TypeError(f"layer_norm: {x.dtype} and {y}: equal, or one of them float32")
 
 
+def _plain(**views: torch.Tensor) -> None:
+    """Refuses views that torch negates lazily (the imaginary part of a conjugate): their memory holds other values."""
+    for name, t in views.items():
+        if t.is_neg():
+            raise ValueError(f"layer_norm: {name} is negated lazily (resolve_neg gives its values)")
+
+
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5, dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                stats: bool = True, ws: torch.Tensor | None = None, stream=None):
@@ -325,7 +332,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if ws is not None or shape[-1] > 49145:
         ws = _norm_room(ws, math.prod(shape[:-1]), shape[-1], x, False)
         room, room_bytes = ws.data_ptr(), ws.nbytes
-    dims = array("q", (*xv.shape, *xv.stride(), *ov.stride()))
+    xs, ys = xv.stride(), ov.stride()
+    if xs[-1] != 1 or ys[-1] != 1:  # a negated view's columns are spread
+        _plain(x=x, out=out)
+    dims = array("q", (*xv.shape, *xs, *ys))
     at = _ptr(dims)
     call("spmdb200_layer_norm", rank, at, xv.data_ptr(), _TYPES[x.dtype], at + 8 * rank, ov.data_ptr(),
          _TYPES[out.dtype], at + 16 * rank, w, b, wtype, eps, m, r, room, room_bytes, _raw_stream(dev))
@@ -393,7 +403,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     gv, xv, dv = _norm_rows("dy", dy), _norm_rows("x", x), _norm_rows("dx", dx)
     ws = _norm_room(ws, mean.numel(), shape[-1], x, True)
     rank = xv.dim()
-    dims = array("q", (*xv.shape, *gv.stride(), *xv.stride(), *dv.stride()))
+    gs, xs, ds = gv.stride(), xv.stride(), dv.stride()
+    if gs[-1] != 1 or xs[-1] != 1 or ds[-1] != 1:  # a negated view's columns are spread
+        _plain(dy=dy, x=x, dx=dx)
+    dims = array("q", (*xv.shape, *gs, *xs, *ds))
     at = _ptr(dims)
     call("spmdb200_layer_norm_backward", rank, at, gv.data_ptr(), _TYPES[dy.dtype], at + 8 * rank, xv.data_ptr(),
          _TYPES[x.dtype], at + 16 * rank, mean.data_ptr(), rstd.data_ptr(), w, wtype, dv.data_ptr(), at + 24 * rank, dw,
