@@ -223,6 +223,7 @@ def jacobi3d(u: torch.Tensor, v: torch.Tensor, sweeps: int, res_every: int = 0, 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _E4M3 = torch.float8_e4m3fn
 STATE_BLOCK = 256  # elements that share one scale of an 8-bit optimizer state
+HELD_COLUMNS = 49145  # of the longest rows for which layer_norm takes no workspace
 
 
 def _elsewhere(dev: int, stream) -> bool:
@@ -297,10 +298,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                eps: float = 1e-5, dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                stats: bool = True, ws: torch.Tensor | None = None, stream=None):
     """(out, mean, rstd): layer norm over the last dimension, out = (x - mean) *
-    rstd * weight + bias.  x is any strided view; out has `dtype` (default
+    rstd * weight + bias.  x is a strided view, of rank 1 to 3 or with leading
+    dimensions that merge into rows; out has `dtype` (default
     x's; one of the two may be float32) and may be x itself.  mean and rstd
     (float32, x's leading shape) are what layer_norm_backward takes; stats=False
-    leaves them out (None).  Rows of more than 49145 elements use a workspace of
+    leaves them out (None).  Rows of more than HELD_COLUMNS elements use a workspace of
     layer_norm_workspace(rows, cols, backward=False)."""
     dev = x.get_device()
     if _elsewhere(dev, stream):
@@ -329,7 +331,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         m, r = mean.data_ptr(), rstd.data_ptr()
     xv, ov = _norm_rows("x", x), _norm_rows("out", out)
     rank, room, room_bytes = xv.dim(), None, 0
-    if ws is not None or shape[-1] > 49145:
+    if ws is not None or shape[-1] > HELD_COLUMNS:
         ws = _norm_room(ws, math.prod(shape[:-1]), shape[-1], x, False)
         room, room_bytes = ws.data_ptr(), ws.nbytes
     xs, ys = xv.stride(), ov.stride()
