@@ -542,7 +542,9 @@ int spmdb200_grad_norm(int count, const void *const *grads, const int64_t *sizes
 /* One AdamW step over `count` tensors in place; step counts from 1:
  *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
- * in f32; a parameter is rounded once to its type, and once more to that of
+ * in f32 (with 8-bit states the root and the reciprocal within p's change may each
+ * be off by 2^-23 of themselves, twice a rounding); a parameter is rounded once to its
+ * type, and once more to that of
  * copies[k] (SPMDB200_F16 or BF16), where copies and copies[k] are not NULL.
  * Host arrays of `count` entries: params, param_types, grads, grad_types,
  * sizes (elements; 0 allowed), exp_avg, exp_avg_sq, decay.  All tensors have

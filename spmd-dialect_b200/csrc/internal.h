@@ -192,7 +192,7 @@ struct LayerNormProblem {
   int dwtype;
   void *ws;  // of the direction's layer_norm_..._workspace_bytes(rows, cols), contents irrelevant
 };
-size_t layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols);  // 0 for rows that a block holds
+size_t layer_norm_forward_workspace_bytes(int64_t rows, int64_t cols);  // 0 for rows that a cluster holds
 size_t layer_norm_workspace_bytes(int64_t rows, int64_t cols);
 cudaError_t launch_layer_norm(const LayerNormProblem &p, cudaStream_t s);
 cudaError_t launch_layer_norm_backward(const LayerNormProblem &p, cudaStream_t s);
