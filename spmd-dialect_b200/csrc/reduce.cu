@@ -47,7 +47,7 @@ size_t sum_f32_workspace_bytes(int64_t n) {
 // unrounded (a rank's share of a sum across GPUs).  The ticket and every
 // partial read are reset to 0, so the workspace is all-zero again for the
 // next call (the staged sum below relies on that).
-__global__ void __launch_bounds__(kSumThreads, 8) sum_f32_kernel(const float *__restrict__ a, int64_t sa,
+__global__ void __launch_bounds__(kSumThreads, 8) sum_f32_kernel(const float *a, int64_t sa,
                                                               int64_t n, float *out,
                                                               unsigned *ticket, double *partials,
                                                               double *f64_out) {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kSumThreads, 8) sum_f32_kernel(const float *__
   }
 }
 
-__global__ void __launch_bounds__(kSumThreads) sum_i32_kernel(const int32_t *__restrict__ a, int64_t sa,
+__global__ void __launch_bounds__(kSumThreads) sum_i32_kernel(const int32_t *a, int64_t sa,
                                                               int64_t n, int32_t *out) {
   __shared__ uint32_t sh[32];
   pdl_wait();
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_i32_kernel(const int32_t *__r
   if (threadIdx.x == 0 && b != 0u) atomicAdd(reinterpret_cast<unsigned *>(out), b);
 }
 
-__global__ void __launch_bounds__(kSumThreads, 8) hier_sum_f32_kernel(const float *__restrict__ a, int64_t sa,
+__global__ void __launch_bounds__(kSumThreads, 8) hier_sum_f32_kernel(const float *a, int64_t sa,
                                                                    int64_t n, float *out) {
   __shared__ double sh[32];
   pdl_wait();
@@ -108,7 +108,7 @@ __device__ int g_reduce_timeout;
 enum class BulkMode { kF32Det, kI32, kF32Atomic };
 
 template <BulkMode M>
-__global__ void __launch_bounds__(kBulkThreads) sum_bulk_kernel(const void *__restrict__ a, int64_t n, void *out,
+__global__ void __launch_bounds__(kBulkThreads) sum_bulk_kernel(const void *a, int64_t n, void *out,
                                                                unsigned *ticket, double *partials,
                                                                double *f64_out) {
   extern __shared__ __align__(128) unsigned char bulk_raw[];

@@ -100,7 +100,7 @@ __device__ __forceinline__ A shfl_xor(A v, int o) {
 }
 
 template <typename T, int K>
-__global__ void __launch_bounds__(kKindThreads) reduce_kind_kernel(const T *__restrict__ a, int64_t sa, int64_t n,
+__global__ void __launch_bounds__(kKindThreads) reduce_kind_kernel(const T *a, int64_t sa, int64_t n,
                                                                    T *out, T init, unsigned *ticket, void *partials_raw) {
   using O = KindOp<T, K>;
   using A = typename O::A;
@@ -164,7 +164,7 @@ __device__ __forceinline__ int32_t elem_as(int32_t, uint32_t u) { return (int32_
 // tree as reduce_kind_kernel.  Each thread combines a fixed subset in a fixed
 // order, so the result is deterministic for a given device.
 template <typename T, int K>
-__global__ void __launch_bounds__(kBulkThreads) reduce_kind_bulk_kernel(const T *__restrict__ a, int64_t n, T *out,
+__global__ void __launch_bounds__(kBulkThreads) reduce_kind_bulk_kernel(const T *a, int64_t n, T *out,
                                                                        T init, unsigned *ticket, void *partials_raw) {
   using O = KindOp<T, K>;
   using A = typename O::A;

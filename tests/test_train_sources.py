@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 
 CSRC = Path(__file__).resolve().parents[1] / "spmd-dialect_b200" / "csrc"
-OVERLAPPING = ["layer_norm.cu", "layer_norm_backward.cu", "grad_norm.cu"]
+OVERLAPPING = ["layer_norm.cu", "layer_norm_backward.cu", "grad_norm.cu", "reduce.cu", "reduce_kinds.cu"]
 
 
 def kernels_of(text: str):
